@@ -12,8 +12,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libchimere_b200_moe.so")
 
 TYPE_Q4_0, TYPE_Q8_0, TYPE_IQ3_S = 2, 8, 21
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
 ROUTE_SOFTMAX_RENORM, ROUTE_SIGMOID_NORM_SCALE = 0, 1
-ACT_SWIGLU, ACT_RELU2 = 0, 1
+ACT_NONE, ACT_SWIGLU, ACT_RELU2 = -1, 0, 1
 LAYOUT_GGML, LAYOUT_TILED32 = 0, 1
 
 
@@ -50,7 +51,7 @@ class PrefillWeights(C.Structure):
                 ("sh_gu", C.c_void_p), ("sh_down", C.c_void_p), ("rows_per_gu_tile", C.c_int32), ("reserved", C.c_int32)]
 
 
-_P = C.c_void_p
+_P, _L = C.c_void_p, C.c_int64
 _LAYER_P, _WS_P = C.POINTER(MoeLayer), C.POINTER(MoeWorkspace)
 
 # name -> (restype, argtypes); exactly the declarations of include/chimere_b200_moe.h
@@ -107,6 +108,14 @@ PROTOTYPES = {
     "chimere_b200_moe_shared_expert_prefill": (C.c_int, [_LAYER_P, C.POINTER(PrefillWeights), C.c_int, _WS_P, _P]),
     "chimere_b200_moe_experts_packed_prefill": (C.c_int, [_LAYER_P, C.POINTER(PrefillWeights), C.c_int, _P, C.c_int, _WS_P, _P]),
     "chimere_b200_moe_ep_pack_sorted": (C.c_int, [_LAYER_P, C.c_int, _WS_P, _P, _P, C.c_int, C.c_int, _P]),
+    "chimere_b200_quantize_i8": (C.c_int, [_P, C.c_int, _L, _L, _P, C.c_int, _L, C.c_int, _P, _L, _P, _P]),
+    "chimere_b200_matmul_w8a8": (C.c_int, [_P, _L, _P, _P, _L, _P, _P, _L, C.c_int, C.c_int, C.c_int, _P, C.c_int, _L, _P, _P]),
+    "chimere_b200_matmul_w8a8_grouped": (C.c_int, [_P, _L, _P, _P, _L, _L, _P, _P, _P, C.c_int, _L, C.c_int, C.c_int, C.c_int, _P, C.c_int, _L, _L, _P, _P, _P]),
+    "chimere_b200_linear_w8a8_bytes": (C.c_size_t, [_L, C.c_int]),
+    "chimere_b200_linear_w8a8": (C.c_int, [_P, C.c_int, _L, _P, _L, _P, _P, _L, C.c_int, C.c_int, C.c_int, _P, C.c_int, _L, _P, C.c_size_t, _P, _P]),
+    "chimere_b200_experts_w8a8_bytes": (C.c_size_t, [_L, C.c_int, C.c_int]),
+    "chimere_b200_experts_w8a8": (C.c_int, [_P, C.c_int, _L, _L, _P, _P, C.c_int, C.c_int, _P, _L, _L, _P, _P, _L, _L, _P, C.c_int, C.c_int, C.c_int,
+                                            _P, C.c_int, _L, _P, C.c_size_t, _P, _P]),
     "chimere_b200_rmsnorm": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_float, _P]),
     "chimere_b200_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(_P)]),
     "chimere_b200_gguf_close": (None, [_P]),

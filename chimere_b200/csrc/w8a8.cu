@@ -1,0 +1,789 @@
+// w8a8.cu -- products of 8-bit integers with a scale per token and a scale per channel, dense and grouped by expert, and the rows
+// that go into them (sm_100a).
+//
+// Math:   quantised row     scale = max|x| / 127,  q = rint(x / scale)
+//         product           y[m][n] = act( (sum_k xq[m][k] * wq[n][k]) * sx[m] * sw[n] + bias[n] )
+// The sums are exact (int32; |sum| <= 128 * 128 * K < 2^31 for K <= 131071), everything behind them is fp32, and the result is rounded
+// once to the output's type.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace chimere {
+namespace {
+
+constexpr int kF32 = CHIMERE_TYPE_F32, kF16 = CHIMERE_TYPE_F16, kBF16 = CHIMERE_TYPE_BF16;
+constexpr int kMaxGroups = 1024;
+constexpr int kMaxK = 131071;
+
+// ------------------------------------------------------------------ rows -> int8 ----
+// One CTA per row: a thread holds up to kQ_Vecs pieces of eight values in registers between the maximum and the division, so a row of up
+// to blockDim * 32 values is read once; what lies behind is read again (from L2).  Bound: memory.
+constexpr int kQ_Vecs = 4;
+
+struct QuantParams {
+    const void* x;
+    int64_t ldx;
+    int64_t x_rows;
+    const int32_t* rows;   // or null
+    int rows_div;
+    int K;
+    int8_t* q;
+    int64_t ldq;
+    float* scale;
+    int vec;               // x rows start on 16-byte boundaries
+};
+
+template <int TYPE> struct Elem;
+template <> struct Elem<kF32> {
+    using T = float;
+    __device__ static __forceinline__ float f(T v) { return v; }
+    __device__ static __forceinline__ void load8(const T* p, float (&v)[8]) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+template <> struct Elem<kF16> {
+    using T = __half;
+    __device__ static __forceinline__ float f(T v) { return __half2float(v); }
+    __device__ static __forceinline__ void load8(const T* p, float (&v)[8]) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = h2f(w[i] & 0xFFFFu); v[2 * i + 1] = h2f(w[i] >> 16); }
+    }
+};
+template <> struct Elem<kBF16> {
+    using T = __nv_bfloat16;
+    __device__ static __forceinline__ float f(T v) { return __bfloat162float(v); }
+    __device__ static __forceinline__ void load8(const T* p, float (&v)[8]) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    }
+};
+
+// The two quotients.  In the wide range of magnitudes both come correctly rounded from a reciprocal (div_by_recip), elsewhere from the
+// division operator; a scale below the normal numbers would make the quotients coarse, so it stays at 2^-126.
+struct RowScale {
+    float scale, recip;
+    bool plain;
+    __device__ __forceinline__ explicit RowScale(float amax) {
+        plain = !(amax > 1e-25f && amax < 1e25f);
+        scale = amax == 0.0f ? 0.0f : fmaxf(plain ? amax / 127.0f : div_by_recip(amax, 127.0f, 1.0f / 127.0f), 1.17549435e-38f);
+        recip = __frcp_rn(scale);
+    }
+    // nearest integer, ties to even: the sum with 1.5 * 2^23 holds it in its low byte (|x / scale| <= 127.5)
+    __device__ __forceinline__ uint32_t q(float x) const {
+        const float v = plain ? (scale == 0.0f ? 0.0f : x / scale) : div_by_recip(x, scale, recip);
+        return __float_as_uint(__fadd_rn(v, 12582912.0f)) & 0xFFu;
+    }
+};
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a | (b << 8) | (c << 16) | (d << 24); }
+
+template <int TYPE>
+__global__ void __launch_bounds__(1024) quantize_rows_kernel(QuantParams p) {
+    using E = Elem<TYPE>;
+    __shared__ uint32_t s_max[32];
+    const int tid = threadIdx.x, nt = blockDim.x;
+    griddep_wait();          // (in front of the next kernel's start: what lies before this kernel is then complete for that one too)
+    griddep_launch();
+    const int64_t row = blockIdx.x;
+    int64_t src = row;
+    if (p.rows) {
+        const int32_t r = p.rows[row];
+        src = r < 0 ? -1 : r / p.rows_div;
+    }
+    int8_t* q = p.q + row * p.ldq;
+    if (src < 0 || src >= p.x_rows) {   // no such row: zeros
+        for (int i = tid; i < p.K; i += nt) q[i] = 0;
+        if (tid == 0) p.scale[row] = 0.0f;
+        return;
+    }
+    const typename E::T* x = reinterpret_cast<const typename E::T*>(p.x) + src * p.ldx;
+    const int nv = p.vec ? p.K >> 3 : 0;
+    float v[kQ_Vecs][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kQ_Vecs; ++i)
+        if (tid + i * nt < nv) {
+            E::load8(x + 8 * (tid + i * nt), v[i]);
+        }
+#pragma unroll
+    for (int i = 0; i < kQ_Vecs; ++i)
+        if (tid + i * nt < nv) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(v[i][j])));   // (a NaN's bits lie above infinity's)
+        }
+    for (int i = tid + kQ_Vecs * nt; i < nv; i += nt) {
+        float w[8];
+        E::load8(x + 8 * i, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(w[j])));
+    }
+    for (int i = 8 * nv + tid; i < p.K; i += nt) m = max(m, __float_as_uint(fabsf(E::f(x[i]))));
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (nt > 32) {
+        if ((tid & 31) == 0) s_max[tid >> 5] = m;
+        __syncthreads();
+        m = __reduce_max_sync(0xffffffffu, (tid & 31) < (nt >> 5) ? s_max[tid & 31] : 0u);
+    }
+    if (m >= 0x7F800000u) {   // an infinity or a NaN in the row: the whole row of the product becomes NaN
+        for (int i = tid; i < p.K; i += nt) q[i] = 0;
+        if (tid == 0) p.scale[row] = __uint_as_float(0x7FC00000u);
+        return;
+    }
+    const RowScale s(__uint_as_float(m));
+    if (tid == 0) p.scale[row] = s.scale;
+    auto put = [&](int i, const float (&w)[8]) {
+        uint2 o;
+        o.x = pack4(s.q(w[0]), s.q(w[1]), s.q(w[2]), s.q(w[3]));
+        o.y = pack4(s.q(w[4]), s.q(w[5]), s.q(w[6]), s.q(w[7]));
+        *reinterpret_cast<uint2*>(q + 8 * i) = o;
+    };
+#pragma unroll
+    for (int i = 0; i < kQ_Vecs; ++i)
+        if (tid + i * nt < nv) put(tid + i * nt, v[i]);
+    for (int i = tid + kQ_Vecs * nt; i < nv; i += nt) {
+        float w[8];
+        E::load8(x + 8 * i, w);
+        put(i, w);
+    }
+    for (int i = 8 * nv + tid; i < p.K; i += nt) q[i] = (int8_t)s.q(E::f(x[i]));
+}
+
+cudaError_t launch_quantize(QuantParams p, int type, int64_t M, cudaStream_t stream, bool pdl) {
+    const int size = type == kF32 ? 4 : 2;
+    p.vec = ((uintptr_t)p.x & 15) == 0 && (p.ldx * size) % 16 == 0;
+    // two pieces of eight values per thread, at least a warp
+    int nt = (p.K + 15) / 16;
+    nt = nt > 1024 ? 1024 : (nt + 31) / 32 * 32;
+    const dim3 grid((unsigned)M);
+    auto go = [&](auto kernel) -> cudaError_t {
+        if (pdl) return launch_pdl(kernel, grid, nt, 0, stream, p);
+        kernel<<<grid, nt, 0, stream>>>(p);
+        return cudaGetLastError();
+    };
+    return type == kF32 ? go(quantize_rows_kernel<kF32>) : type == kF16 ? go(quantize_rows_kernel<kF16>) : go(quantize_rows_kernel<kBF16>);
+}
+
+// ------------------------------------------------------------------ product ----
+// tcgen05 kind::i8 with the weights as the MMA's 128 rows and the tokens as its columns, so that one kernel serves one token and
+// thousands: a tile is 128 weight rows (two such blocks, gate and up, where the activation joins them) x BN tokens, BN the narrowest of
+// 16 .. 256 that suits the batch.  Operands come by TMA as rows of 128 bytes (128-byte swizzle), zeros beyond K and beyond the last row.
+// Where a batch has fewer tiles than the GPU has SMs, a cluster of up to eight CTAs shares a tile, each with a part of K; their int32 sums
+// meet in shared memory over the cluster, exact in any order.
+//   warp 0     TMA            warp 1     MMA            warps 4..7   read the accumulators back, scale, store (thread = weight row)
+// All waits are bounded: one that runs out makes the tile's outputs NaN and raises the status word.
+constexpr int kMM_Threads = 256;
+constexpr int kMM_KBytes = 128;          // of K per stage
+constexpr int kMM_ABytes = 128 * kMM_KBytes;
+constexpr int kMM_MaxStages = 12;
+
+struct MatmulParams {
+    const float* sx;
+    const float* sw;
+    const float* bias;
+    void* y;
+    int64_t ldy, y_rows;
+    const int32_t* offsets;    // grouped: [E + 1], else null
+    const int32_t* out_rows;   // or null
+    int32_t* status;           // or null
+    int M, N, K, E;
+    int y_type, act;
+    int mt, nt;                // dense: token tiles; tiles of 128 outputs
+    int n_stages, split;
+    int early;                 // the weights, scales and offsets do not come from the previous kernel
+};
+
+struct MatmulShared {
+    uint64_t full[kMM_MaxStages], empty[kMM_MaxStages];
+    uint64_t tfull[2], tempty[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int failed;
+    float sx[2][256];
+    int row[2][256];
+    int scan[kMM_Threads / 32];
+};
+
+struct Tile { int expert, row0, ntok, n0; };
+
+__device__ __forceinline__ bool elect1() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// rows of 128 bytes, 128-byte swizzle: groups of eight rows 1024 bytes apart; a step of 32 along K is 32 bytes of the start address
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void ld16(uint32_t taddr, int* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Tile `id` of the call: token tiles fastest, so that the CTAs at work at a time share weight rows.
+__device__ __forceinline__ Tile take_tile(const MatmulParams& p, const int* prefix, int id, int BN) {
+    Tile t;
+    if (!p.offsets) {
+        const int m = id % p.mt;
+        t.expert = 0;
+        t.row0 = m * BN;
+        t.ntok = min(BN, p.M - t.row0);
+        t.n0 = id / p.mt * 128;
+        return t;
+    }
+    // prefix[e]: token tiles of the experts in front of e; largest e with prefix[e] * nt <= id
+    int lo = 0, hi = p.E - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (prefix[mid] * p.nt <= id) lo = mid; else hi = mid - 1;
+    }
+    const int c = prefix[lo + 1] - prefix[lo], local = id - prefix[lo] * p.nt, m = local % c;
+    const int start = min(max(p.offsets[lo], 0), p.M), end = min(max(p.offsets[lo + 1], start), p.M);
+    t.expert = lo;
+    t.row0 = start + m * BN;
+    t.ntok = min(BN, end - t.row0);
+    t.n0 = local / c * 128;
+    return t;
+}
+
+__device__ __forceinline__ void put(const MatmulParams& p, int64_t row, int n, float v) {
+    const int64_t at = row * p.ldy + n;
+    if (p.y_type == kF32) reinterpret_cast<float*>(p.y)[at] = v;
+    else if (p.y_type == kBF16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half*>(p.y)[at] = __float2half_rn(v);
+}
+// what one thread needs of its weight row(s)
+struct Channel { float sw, sw_up, b, b_up; };
+__device__ __forceinline__ Channel channel(const MatmulParams& p, bool dual, int expert, int n) {
+    Channel c{0.0f, 0.0f, 0.0f, 0.0f};
+    if (n < p.N) {
+        const int64_t at = (int64_t)expert * (dual ? 2 * (int64_t)p.N : p.N) + n;
+        c.sw = p.sw[at];
+        if (p.bias) c.b = p.bias[at];
+        if (dual) {
+            c.sw_up = p.sw[at + p.N];
+            if (p.bias) c.b_up = p.bias[at + p.N];
+        }
+    }
+    return c;
+}
+template <bool DUAL>
+__device__ __forceinline__ float finish(const MatmulParams& p, const Channel& c, float sx, int acc, int acc_up) {
+    // (the channel's scale first: a token's may lie anywhere in fp32's range, and then only a result that does not fit overflows)
+    float v = (float)acc * c.sw * sx + c.b;
+    if (DUAL) v = silu_mul_ref(v, (float)acc_up * c.sw_up * sx + c.b_up);
+    else if (p.act == CHIMERE_ACT_RELU2) { v = v > 0.0f || v != v ? v : 0.0f; v *= v; }
+    return v;
+}
+
+template <int BN, bool DUAL>
+__global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, MatmulParams p) {
+    constexpr uint32_t kStage = kMM_ABytes * (DUAL ? 2 : 1) + BN * kMM_KBytes;
+    constexpr uint32_t kAccCols = BN * (DUAL ? 2 : 1);
+    constexpr uint32_t kTmemCols = kAccCols * 2 < 32 ? 32 : kAccCols * 2;
+    static_assert(kTmemCols <= 512, "two accumulators fit");
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) MatmulShared sh;
+    __shared__ int prefix[kMaxGroups + 1];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int S = p.split, rank = S > 1 ? blockIdx.x % S : 0, first = blockIdx.x / S, step = gridDim.x / S;
+    const uint32_t stages = smem_u32(smem);
+
+    if (!p.early) griddep_wait();
+    int total = p.mt * p.nt;
+    if (p.offsets) {   // token tiles per expert, summed over the experts in front
+        int mine[kMaxGroups / kMM_Threads], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxGroups / kMM_Threads; ++i) {
+            const int e = tid * (kMaxGroups / kMM_Threads) + i;
+            mine[i] = 0;
+            if (e < p.E) {
+                const int start = min(max(p.offsets[e], 0), p.M), end = min(max(p.offsets[e + 1], start), p.M);
+                mine[i] = (end - start + BN - 1) / BN;
+            }
+            sum += mine[i];
+        }
+        int scan = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, scan, d);
+            if (lane >= d) scan += o;
+        }
+        if (lane == 31) sh.scan[warp] = scan;
+        __syncthreads();
+        int before = scan - sum;
+        for (int w = 0; w < warp; ++w) before += sh.scan[w];
+#pragma unroll
+        for (int i = 0; i < kMaxGroups / kMM_Threads; ++i) {
+            const int e = tid * (kMaxGroups / kMM_Threads) + i;
+            if (e <= p.E) prefix[e] = before;
+            before += mine[i];
+        }
+        if (tid == kMM_Threads - 1 && p.E == kMaxGroups) prefix[kMaxGroups] = before;
+        __syncthreads();
+        total = prefix[p.E] * p.nt;
+    }
+    if (first >= total) {   // (the whole cluster; nothing has been allocated)
+        griddep_launch();
+        return;
+    }
+
+    if (tid == 0) {
+        for (int i = 0; i < p.n_stages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.tfull[i], 1); mbar_init(&sh.tempty[i], 4); }
+        mbar_init(&sh.drain, 1);
+        sh.failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    if (tid == 0) griddep_launch();
+
+    const int nkb = (p.K + kMM_KBytes - 1) / kMM_KBytes;
+    const int kb0 = (int)((int64_t)rank * nkb / S), kb1 = (int)((int64_t)(rank + 1) * nkb / S);
+
+    if (warp == 0) {
+        int st = 0;
+        uint32_t ph = 0, used = 0;
+        bool ok = true, waited = !p.early;
+        for (int id = first; ok && id < total; id += step) {
+            const Tile t = take_tile(p, prefix, id, BN);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(&sh.empty[st], ph ^ 1u)) { ok = false; break; }
+                const uint32_t dst = stages + st * kStage;
+                if (elect1()) {
+                    mbar_expect_tx(&sh.full[st], kStage);
+                    tma_3d(dst, &map_w, kb * kMM_KBytes, t.n0, t.expert, &sh.full[st]);
+                    if (DUAL) tma_3d(dst + kMM_ABytes, &map_w, kb * kMM_KBytes, p.N + t.n0, t.expert, &sh.full[st]);
+                }
+                __syncwarp();
+                if (!waited) { griddep_wait(); waited = true; }
+                if (elect1()) tma_2d(dst + kMM_ABytes * (DUAL ? 2 : 1), &map_x, kb * kMM_KBytes, t.row0, &sh.full[st]);
+                __syncwarp();
+                used |= 1u << st;
+                if (++st == p.n_stages) { st = 0; ph ^= 1u; }
+            }
+        }
+        if (!ok) {   // the copies under way land before the CTA goes
+            sh.failed = 1;
+            for (int i = 0; i < p.n_stages; ++i)
+                if (used >> i & 1u) mbar_wait(&sh.full[i], (i < st ? ph : ph ^ 1u));
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((128u >> 4) << 24);
+        int st = 0, n = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int id = first; ok && id < total; id += step, ++n) {
+            const int buf = n & 1;
+            if (!mbar_wait(&sh.tempty[buf], ((n >> 1) & 1) ^ 1u)) { ok = false; break; }
+            fence_after();
+            const uint32_t d = tmem + buf * kAccCols;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(&sh.full[st], ph)) { ok = false; break; }
+                fence_after();
+                if (elect1()) {
+                    const uint32_t a = stages + st * kStage, b = a + kMM_ABytes * (DUAL ? 2 : 1);
+#pragma unroll
+                    for (int k = 0; k < kMM_KBytes / 32; ++k) {
+                        const uint32_t acc = kb > kb0 || k > 0;
+                        mma_i8(d, desc_sw128(a + 32 * k), desc_sw128(b + 32 * k), idesc, acc);
+                        if (DUAL) mma_i8(d + BN, desc_sw128(a + kMM_ABytes + 32 * k), desc_sw128(b + 32 * k), idesc, acc);
+                    }
+                    commit(&sh.empty[st]);
+                }
+                __syncwarp();
+                if (++st == p.n_stages) { st = 0; ph ^= 1u; }
+            }
+            if (ok && elect1()) commit(&sh.tfull[buf]);
+            __syncwarp();
+        }
+        if (!ok) {
+            sh.failed = 1;
+            if (elect1()) commit(&sh.drain);   // (the MMAs under way)
+            __syncwarp();
+            mbar_wait(&sh.drain, 0);
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, row = q * 32 + lane, et = tid - 128;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+        bool ok = true;
+        griddep_wait();   // (the tokens' scales; and nothing of y is written before what used its memory has ended)
+        int n = 0;
+        for (int id = first; id < total; id += step, ++n) {
+            const Tile t = take_tile(p, prefix, id, BN);
+            const int buf = n & 1;
+            const Channel ch = channel(p, DUAL, t.expert, t.n0 + row);
+            if (S == 1) {
+                for (int i = et; i < t.ntok; i += 128) {
+                    sh.sx[buf][i] = p.sx[t.row0 + i];
+                    sh.row[buf][i] = p.out_rows ? p.out_rows[t.row0 + i] : t.row0 + i;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            if (ok && !mbar_wait(&sh.tfull[buf], (n >> 1) & 1)) { ok = false; sh.failed = 1; }
+            fence_after();
+            if (S > 1) {   // this CTA's part of the sums, over the operands' buffers: [gate / up][token][128]
+                int* part = reinterpret_cast<int*>(smem);
+                for (int c0 = 0; c0 < t.ntok; c0 += 16)
+#pragma unroll
+                    for (int h = 0; h < (DUAL ? 2 : 1); ++h) {
+                        int v[16];
+                        ld16(taddr + buf * kAccCols + h * BN + c0, v);
+                        wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) part[(h * BN + c0 + j) * 128 + row] = v[j];
+                    }
+                fence_before();
+                break;
+            }
+            for (int c0 = 0; c0 < t.ntok; c0 += 16) {
+                int v[16], u[16];
+                ld16(taddr + buf * kAccCols + c0, v);
+                if (DUAL) ld16(taddr + buf * kAccCols + BN + c0, u);
+                wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int m = c0 + j;
+                    if (m < t.ntok && t.n0 + row < p.N) {
+                        const int64_t r = sh.row[buf][m];
+                        float o = finish<DUAL>(p, ch, sh.sx[buf][m], v[j], DUAL ? u[j] : 0);
+                        if (!ok) o = __uint_as_float(0x7FC00000u);
+                        if (r >= 0 && r < p.y_rows) put(p, r, t.n0 + row, o);
+                    }
+                }
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cta(&sh.tempty[buf]);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    if (S > 1) {
+        const Tile t = take_tile(p, prefix, first, BN);
+        griddep_wait();
+        cluster_sync();   // every part is there
+        bool bad = false;
+        for (int s = 0; s < S; ++s) bad |= ld_cluster(cluster_addr(smem_u32(&sh.failed), s)) != 0;
+        for (int i = rank * kMM_Threads + tid; i < t.ntok * 128; i += S * kMM_Threads) {
+            const int m = i >> 7, n = t.n0 + (i & 127);
+            if (n >= p.N) continue;
+            int acc = 0, up = 0;
+            for (int s = 0; s < S; ++s) {
+                acc += ld_cluster(cluster_addr(stages + 4 * i, s));
+                if (DUAL) up += ld_cluster(cluster_addr(stages + 4 * (i + BN * 128), s));
+            }
+            const int64_t r = p.out_rows ? p.out_rows[t.row0 + m] : t.row0 + m;
+            float o = finish<DUAL>(p, channel(p, DUAL, t.expert, n), p.sx[t.row0 + m], acc, up);
+            if (bad) o = __uint_as_float(0x7FC00000u);
+            if (r >= 0 && r < p.y_rows) put(p, r, n, o);
+        }
+        cluster_sync();   // ... and has been read
+    }
+    if (tid == 0 && sh.failed && p.status) atomicOr(p.status, kStatusWaitTimeout);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+    static EncodeFn fn = nullptr;   // (the same address whoever looks it up first)
+    if (!fn) {
+        void* at = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &at, 12000, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess)
+            fn = (EncodeFn)at;
+        else cudaGetLastError();
+    }
+    return fn;
+}
+// rows of K bytes as boxes of 128 bytes x box_rows
+bool make_map(CUtensorMap* map, const void* base, int K, int64_t rows, int64_t planes, int64_t ld, int64_t plane, int box_rows, int rank) {
+    const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)plane};
+    const cuuint32_t box[3] = {kMM_KBytes, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+    return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct MatmulCall {
+    const int8_t* x;
+    int64_t ldx;
+    const int8_t* w;
+    int64_t ldw, w_plane;
+    MatmulParams p;
+    bool dual;
+};
+
+template <int BN, bool DUAL>
+int launch_tile(const MatmulCall& c, int tiles, int split, bool pdl, cudaStream_t stream) {
+    constexpr int kStage = kMM_ABytes * (DUAL ? 2 : 1) + BN * kMM_KBytes;
+    static bool done[64];
+    CUtensorMap mx, mw;
+    MatmulParams p = c.p;
+    if (!make_map(&mx, c.x, p.K, p.M, 1, c.ldx, 0, BN, 2)) return -5;
+    if (!make_map(&mw, c.w, p.K, (DUAL ? 2 : 1) * (int64_t)p.N, p.E, c.ldw, c.w_plane, 128, 3)) return -5;
+    const int nkb = (p.K + kMM_KBytes - 1) / kMM_KBytes, most = (200 * 1024) / kStage;
+    int stages = (nkb + split - 1) / split;
+    const int parts = split > 1 ? (BN * (DUAL ? 2 : 1) * 512 + kStage - 1) / kStage : 1;   // room for the sums
+    stages = stages < parts ? parts : stages;
+    if (split == 1 && stages < 2) stages = 2;
+    stages = stages > most ? most : stages;
+    stages = stages > kMM_MaxStages ? kMM_MaxStages : stages;
+    p.n_stages = stages;
+    p.split = split;
+    p.mt = (p.M + BN - 1) / BN;
+    p.nt = (p.N + 127) / 128;
+    auto kernel = matmul_kernel<BN, DUAL>;
+    constexpr int kMostSmem = 1024 + 200 * 1024;
+    cudaError_t e = max_smem_once(kernel, kMostSmem, done);
+    if (e != cudaSuccess) return -(100 + (int)e);
+    const int grid = split > 1 ? tiles * split : tiles < sm_count() ? tiles : sm_count();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kMM_Threads);
+    cfg.dynamicSmemBytes = 1024 + (size_t)stages * kStage;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
+    if (split > 1) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = split; attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1; ++n; }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, p);
+    return e == cudaSuccess ? 0 : -(100 + (int)e);
+}
+
+// Token tiles of width bn: of a dense call exactly, of a grouped one at most.
+int64_t token_tiles(const MatmulCall& c, int bn) {
+    return c.p.offsets ? c.p.M / bn + (c.p.M < c.p.E ? c.p.M : c.p.E) : (c.p.M + bn - 1) / bn;
+}
+
+int launch_matmul(const MatmulCall& c, bool pdl, cudaStream_t stream) {
+    if (c.p.M == 0) return 0;
+    if (!encoder()) return -6;
+    const int64_t nt = (c.p.N + 127) / 128;
+    const int sms = sm_count();
+    // Width of the token tiles.  Cycles per 128 of K: the MMAs (2.1 per column and block of weight rows), or the tile's bytes through L2.
+    const int widest = c.dual ? 128 : 256;
+    int bn = 16;
+    double best = 1e30;
+    const int64_t per = c.p.offsets ? (c.p.M + c.p.E - 1) / c.p.E : c.p.M;   // (grouped: of an even load)
+    for (int b = 16; b <= widest; b *= 2) {
+        const double mma = 2.1 * b * (c.dual ? 2 : 1), load = (16384.0 * (c.dual ? 2 : 1) + 128.0 * b) / 50.0;
+        const int64_t tiles = (c.p.offsets ? c.p.E * ((per + b - 1) / b) : (per + b - 1) / b) * nt;
+        const double cost = (double)((tiles + sms - 1) / sms) * (mma > load ? mma : load);
+        if (cost < best) { best = cost; bn = b; }
+    }
+    const int64_t tiles = token_tiles(c, bn) * nt;
+    if (tiles > 0x7FFFFFFF) return -2;
+    int split = 1;
+    const int nkb = (c.p.K + kMM_KBytes - 1) / kMM_KBytes;
+    if (bn <= 64)
+        while (split < 8 && tiles * split * 2 <= sms && split * 4 <= nkb) split *= 2;
+    switch (bn + (c.dual ? 1 : 0)) {
+        case 16: return launch_tile<16, false>(c, (int)tiles, split, pdl, stream);
+        case 32: return launch_tile<32, false>(c, (int)tiles, split, pdl, stream);
+        case 64: return launch_tile<64, false>(c, (int)tiles, split, pdl, stream);
+        case 128: return launch_tile<128, false>(c, (int)tiles, split, pdl, stream);
+        case 256: return launch_tile<256, false>(c, (int)tiles, split, pdl, stream);
+        case 17: return launch_tile<16, true>(c, (int)tiles, split, pdl, stream);
+        case 33: return launch_tile<32, true>(c, (int)tiles, split, pdl, stream);
+        case 65: return launch_tile<64, true>(c, (int)tiles, split, pdl, stream);
+        default: return launch_tile<128, true>(c, (int)tiles, split, pdl, stream);
+    }
+}
+
+// ------------------------------------------------------------------ checks ----
+inline bool float_type(int t) { return t == kF32 || t == kF16 || t == kBF16; }
+inline int type_size(int t) { return t == kF32 ? 4 : 2; }
+inline bool misaligned(const void* p, int to) { return ((uintptr_t)p & (uintptr_t)(to - 1)) != 0; }
+
+int check_quantize(const void* x, int type, int64_t ldx, int64_t x_rows, const int32_t* rows, int rows_div, int64_t M, int K, const int8_t* q, int64_t ldq, const float* scale) {
+    if (M < 0 || M > 0x7FFFFFFF || x_rows < 0 || K <= 0 || K > kMaxK || ldx < K || ldq < K || ldq % 16 || rows_div <= 0) return -2;
+    if (!float_type(type)) return -3;
+    if (!rows && x_rows < M) return -2;
+    if (M == 0) return 0;
+    if ((!x && x_rows > 0) || !q || !scale) return -1;
+    if (misaligned(x, type_size(type)) || misaligned(q, 16) || misaligned(scale, 4) || misaligned(rows, 4)) return -5;
+    return 0;
+}
+int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, int E, int64_t M, int N, int K,
+                 int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows) {
+    const int64_t R = (act == CHIMERE_ACT_SWIGLU ? 2 : 1) * (int64_t)N;
+    if (M < 0 || M > 0x7FFFFFFF || N <= 0 || R > 0x7FFFFF00 || K <= 0 || K > kMaxK || E <= 0 || E > kMaxGroups) return -2;
+    if (ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldy < N || y_rows < 0) return -2;
+    if (E > 1 && (w_plane % 16 || w_plane < (R - 1) * ldw + K)) return -2;
+    if (act != CHIMERE_ACT_NONE && act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
+    if (!float_type(y_type)) return -3;
+    if (!out_rows && y_rows < M) return -2;
+    if (M == 0) return 0;
+    if (!x || !sx || !w || !sw || (!y && y_rows > 0)) return -1;
+    if (misaligned(x, 16) || misaligned(w, 16) || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4) || misaligned(y, type_size(y_type)) || misaligned(out_rows, 4)) return -5;
+    return 0;
+}
+MatmulCall matmul_call(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, const int32_t* offsets, int E,
+                       int64_t M, int N, int K, int act, void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows, int32_t* status, bool early) {
+    MatmulCall c{};
+    c.x = x; c.ldx = ldx; c.w = w; c.ldw = ldw;
+    c.dual = act == CHIMERE_ACT_SWIGLU;
+    c.w_plane = E > 1 ? w_plane : (c.dual ? 2 : 1) * (int64_t)N * ldw;
+    MatmulParams& p = c.p;
+    p.sx = sx; p.sw = sw; p.bias = bias; p.y = y; p.ldy = ldy; p.y_rows = y_rows; p.offsets = offsets; p.out_rows = out_rows; p.status = status;
+    p.M = (int)M; p.N = N; p.K = K; p.E = E; p.y_type = y_type; p.act = act; p.early = early;
+    return c;
+}
+inline int up16(int k) { return (k + 15) & ~15; }
+inline int up4(int k) { return (k + 3) & ~3; }
+inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+inline size_t rows_bytes(int64_t M, int K) { return up256((size_t)M * up16(K)) + up256((size_t)M * 4); }   // int8 rows and their scales
+struct Carver {
+    uint8_t* base;
+    size_t at;
+    void* take(size_t n) { void* r = (void*)((uintptr_t)base + at); at += up256(n); return r; }
+};
+inline int rc_of(cudaError_t e) { return e == cudaSuccess ? 0 : -(100 + (int)e); }
+
+}  // namespace
+}  // namespace chimere
+
+using namespace chimere;
+
+extern "C" {
+
+int chimere_b200_quantize_i8(const void* d_x, int x_type, int64_t ldx, int64_t x_rows, const int32_t* d_rows, int rows_div, int64_t M, int K,
+                             int8_t* d_q, int64_t ldq, float* d_scale, cudaStream_t stream) {
+    const int rc = check_quantize(d_x, x_type, ldx, x_rows, d_rows, rows_div, M, K, d_q, ldq, d_scale);
+    if (rc || M == 0) return rc;
+    return rc_of(launch_quantize(QuantParams{d_x, ldx, x_rows, d_rows, rows_div, K, d_q, ldq, d_scale, 0}, x_type, M, stream, false));
+}
+
+int chimere_b200_matmul_w8a8(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,
+                             int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy, int32_t* d_status, cudaStream_t stream) {
+    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
+    if (rc || M == 0) return rc;
+    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, false), false, stream);
+}
+
+int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, int64_t stride_w, const float* d_w_scale,
+                                     const float* d_bias, const int32_t* d_offsets, int E, int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy,
+                                     int64_t y_rows, const int32_t* d_out_rows, int32_t* d_status, cudaStream_t stream) {
+    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_out_rows);
+    if (rc || M == 0) return rc;
+    if (!d_offsets) return -1;
+    if (misaligned(d_offsets, 4)) return -5;
+    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, d_offsets, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_out_rows, d_status, false), false, stream);
+}
+
+size_t chimere_b200_linear_w8a8_bytes(int64_t M, int K) {
+    if (M < 0 || M > 0x7FFFFFFF || K <= 0 || K > kMaxK) return 0;
+    return rows_bytes(M, K) + 256;
+}
+
+int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias, int64_t M, int N, int K,
+                             int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes, int32_t* d_status, cudaStream_t stream) {
+    Carver ws{(uint8_t*)d_ws, 0};
+    int8_t* q = (int8_t*)ws.take((size_t)(M < 0 ? 0 : M) * up16(K));
+    float* scale = (float*)ws.take((size_t)(M < 0 ? 0 : M) * 4);
+    if (M > 0 && !d_ws) return -1;
+    if (misaligned(d_ws, 256)) return -5;
+    int rc = check_quantize(d_x, x_type, ldx, M, nullptr, 1, M, K, q, up16(K), scale);
+    if (rc) return rc;
+    rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
+    if (rc || M == 0) return rc;
+    if (ws_bytes < ws.at) return -4;
+    if (!encoder()) return -6;
+    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, 0}, x_type, M, stream, false));
+    if (rc) return rc;
+    return launch_matmul(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, true), true, stream);
+}
+
+size_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F) {
+    if (pairs < 0 || pairs > 0x7FFFFFFF || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return 0;
+    return rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up4(F) * 4) + 256;
+}
+
+int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
+                              const int8_t* d_w_up, int64_t ld_up, int64_t stride_up, const float* d_up_scale,
+                              const int8_t* d_w_down, int64_t ld_down, int64_t stride_down, const float* d_down_scale,
+                              int H, int F, int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes, int32_t* d_status, cudaStream_t stream) {
+    if (T < 0 || top_k <= 0 || T > 0x7FFFFFFF / top_k) return -2;
+    if (H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return -2;
+    if (act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
+    const int64_t P = T * top_k;
+    Carver ws{(uint8_t*)d_ws, 0};
+    int8_t* q = (int8_t*)ws.take((size_t)P * up16(H));
+    float* scale = (float*)ws.take((size_t)P * 4);
+    int8_t* hq = (int8_t*)ws.take((size_t)P * up16(F));
+    float* h_scale = (float*)ws.take((size_t)P * 4);
+    float* h = (float*)ws.take((size_t)P * up4(F) * 4);
+    if (P > 0 && (!d_ws || !d_perm || !d_offsets)) return -1;
+    if (misaligned(d_ws, 256) || misaligned(d_offsets, 4)) return -5;
+    int rc = check_quantize(d_x, x_type, ldx, T, d_perm, top_k, P, H, q, up16(H), scale);
+    if (rc) return rc;
+    rc = check_matmul(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, E, P, F, H, act, h, kF32, up4(F), P, nullptr);
+    if (rc) return rc;
+    rc = check_matmul(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm);
+    if (rc || P == 0) return rc;
+    if (ws_bytes < ws.at) return -4;
+    if (!encoder()) return -6;
+    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, d_perm, top_k, H, q, up16(H), scale, 0}, x_type, P, stream, false));
+    if (rc) return rc;
+    rc = launch_matmul(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up4(F), P, nullptr, d_status, true), true, stream);
+    if (rc) return rc;
+    rc = rc_of(launch_quantize(QuantParams{h, up4(F), P, nullptr, 1, F, hq, up16(F), h_scale, 0}, kF32, P, stream, true));
+    if (rc) return rc;
+    return launch_matmul(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm,
+                                     d_status, true), true, stream);
+}
+
+}  // extern "C"

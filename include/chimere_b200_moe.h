@@ -38,12 +38,15 @@ typedef struct CUstream_st* cudaStream_t;
 /* ggml tensor-type ids of the weight formats this path supports. */
 enum { CHIMERE_TYPE_Q4_0 = 2, CHIMERE_TYPE_Q8_0 = 8, CHIMERE_TYPE_IQ3_S = 21,
        /* K-quant super-blocks: plain GEMV entries (chimere_mmvq_q4k / _q5k / _q6k) only, not a chimere_moe_layer weight type */
-       CHIMERE_TYPE_Q4_K = 12, CHIMERE_TYPE_Q5_K = 13, CHIMERE_TYPE_Q6_K = 14 };
+       CHIMERE_TYPE_Q4_K = 12, CHIMERE_TYPE_Q5_K = 13, CHIMERE_TYPE_Q6_K = 14,
+       /* rows of the W8A8 and balance-loss entries */
+       CHIMERE_TYPE_F32 = 0, CHIMERE_TYPE_F16 = 1, CHIMERE_TYPE_BF16 = 30 };
 /* Router variants. */
 enum { CHIMERE_ROUTE_SOFTMAX_RENORM = 0,  /* softmax over E, top-k on probabilities, renormalise (chimere_kernels.cu:1150-1223) */
        CHIMERE_ROUTE_SIGMOID_NORM_SCALE = 1 /* sigmoid scores, top-k, normalise to sum 1, multiply by route_scale (Nemotron-H style) */ };
 /* Expert activation. */
-enum { CHIMERE_ACT_SWIGLU = 0,  /* silu(gate x) * (up x)   (fused_ops.rs:34-45) */
+enum { CHIMERE_ACT_NONE = -1,   /* W8A8 entries only */
+       CHIMERE_ACT_SWIGLU = 0,  /* silu(gate x) * (up x)   (fused_ops.rs:34-45) */
        CHIMERE_ACT_RELU2 = 1    /* relu(up x)^2, no gate matrix */ };
 
 /* Weight layouts.  GGML: the blocks exactly as the GGUF file holds them.  TILED32: the library's own
@@ -356,6 +359,52 @@ int chimere_b200_moe_experts_packed_prefill(const chimere_moe_layer* w_local, co
  * the rank ranges with one all-to-all of exact sizes. */
 int chimere_b200_moe_ep_pack_sorted(const chimere_moe_layer* w, int T, chimere_moe_workspace* ws, void* d_send, int32_t* d_slot,
                                     int experts_per_rank, int row_bytes, cudaStream_t stream);
+
+/* ------------------------------------------------------------ W8A8 ---------------------- */
+/* Matrices of 8-bit integers with one f32 scale per output channel, times rows of 8-bit integers with one f32 scale per token: the
+ * form int8 checkpoints have for the projections around the MoE layer and for experts.  No counterpart in the reference, whose weights
+ * are ggml blocks.  Rows of int8 start on 16-byte boundaries (base and row stride multiples of 16 bytes; the bytes behind a row's K values
+ * are not looked at); K <= 131071, so that every sum is exact in 32 bits.  *_type: CHIMERE_TYPE_F32, _F16 or _BF16.  M = 0 is no work.
+ * d_status (may be NULL): raised if a bounded wait ran out; the outputs concerned are NaN then.
+ * Errors: -1 null pointer, -2 bad dimension, -3 type, -4 workspace too small, -5 misaligned, -6 driver without tensor maps. */
+
+/* q[i][k] = rint(x[r][k] / scale[i]) with scale[i] = max|x[r]| / 127 (both quotients rounded to f32; ties to even; a scale of a row that is not
+ * zero is at least 2^-126) and r = d_rows ? d_rows[i] / rows_div : i, for i < M.  A row of zeros has scale 0.  A row with an infinity or a NaN gets
+ * scale NaN and zeros, so that its products are NaN.  An index outside [0, x_rows) gives a row of zeros with scale 0. */
+int chimere_b200_quantize_i8(const void* d_x, int x_type, int64_t ldx, int64_t x_rows, const int32_t* d_rows, int rows_div,
+                             int64_t M, int K, int8_t* d_q, int64_t ldq, float* d_scale, cudaStream_t stream);
+
+/* y[m][n] = act((sum_k x[m][k] * w[n][k]) * x_scale[m] * w_scale[n] + bias[n]), m < M, n < N.  CHIMERE_ACT_NONE; CHIMERE_ACT_RELU2; CHIMERE_ACT_SWIGLU: w,
+ * w_scale and bias have 2 N rows, N of the gate and then N of the up matrix, and y = silu(gate) * up.  d_bias may be NULL.  ldx, ldw in
+ * bytes, ldy in elements. */
+int chimere_b200_matmul_w8a8(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, const float* d_w_scale,
+                             const float* d_bias, int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy,
+                             int32_t* d_status, cudaStream_t stream);
+/* The same with a matrix per group of rows: rows d_offsets[e] .. d_offsets[e + 1] (device int32 [E + 1], as chimere_b200_moe_route leaves them in
+ * ws->offsets; E <= 1024) by matrix e, which starts e * stride_w bytes behind the first; w_scale and bias [E][N or 2 N].  With d_out_rows row i goes to row
+ * d_out_rows[i] of y.  Rows in no group, and rows whose index is not in [0, y_rows), are not written. */
+int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, int64_t stride_w,
+                                     const float* d_w_scale, const float* d_bias, const int32_t* d_offsets, int E, int64_t M, int N, int K,
+                                     int act, void* d_y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* d_out_rows,
+                                     int32_t* d_status, cudaStream_t stream);
+
+/* quantize_i8 of the M rows of x and matmul_w8a8 in one call.  d_ws: scratch of at least linear_w8a8_bytes(M, K), 256-byte aligned, used by no other call
+ * at the same time (0 from the size function: bad arguments). */
+size_t chimere_b200_linear_w8a8_bytes(int64_t M, int K);
+int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,
+                             int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes,
+                             int32_t* d_status, cudaStream_t stream);
+
+/* Routed experts in W8A8 behind the router of this library: y[pair] = down_e . act(gate|up_e . x[pair / top_k]) for the T * top_k pairs, e the expert whose range
+ * of d_perm (d_offsets[e] .. d_offsets[e + 1]) holds the pair; d_perm and d_offsets as chimere_b200_moe_route / _permute leave them.  The rows between the two products
+ * are held in f32 and quantised by token again.  w_up [E][2 F (SWIGLU: gate rows, then up) or F (RELU2)][H], w_down [E][H][F].  Rows of y whose pair is in no expert's range are
+ * not written.  Scratch as above. */
+size_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F);
+int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
+                              const int8_t* d_w_up, int64_t ld_up, int64_t stride_up, const float* d_up_scale,
+                              const int8_t* d_w_down, int64_t ld_down, int64_t stride_down, const float* d_down_scale,
+                              int H, int F, int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes,
+                              int32_t* d_status, cudaStream_t stream);
 
 /* RMSNorm with unit weight over rows of length H: y = x / sqrt(mean(x^2) + eps). Used between
  * stacked layers. */
