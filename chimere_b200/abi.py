@@ -116,6 +116,9 @@ PROTOTYPES = {
     "chimere_b200_experts_w8a8_bytes": (C.c_size_t, [_L, C.c_int, C.c_int]),
     "chimere_b200_experts_w8a8": (C.c_int, [_P, C.c_int, _L, _L, _P, _P, C.c_int, C.c_int, _P, _L, _L, _P, _P, _L, _L, _P, C.c_int, C.c_int, C.c_int,
                                             _P, C.c_int, _L, _P, C.c_size_t, _P, _P]),
+    "chimere_b200_balance_loss_bytes": (C.c_size_t, [_L, _L, C.c_int, C.c_int]),
+    "chimere_b200_balance_loss": (C.c_int, [_P, C.c_int, _L, _L, _P, _P, _L, _L, C.c_int, C.c_int, C.c_int, C.c_float, _P, _P, _P, _P, _P, _P, _L, _L, _P, C.c_size_t, _P]),
+    "chimere_b200_balance_loss_backward": (C.c_int, [_P, C.c_int, _L, _L, _P, _P, _P, _L, _L, C.c_int, C.c_int, C.c_int, C.c_float, _P, _P, _L, _L, _P]),
     "chimere_b200_rmsnorm": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_float, _P]),
     "chimere_b200_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(_P)]),
     "chimere_b200_gguf_close": (None, [_P]),

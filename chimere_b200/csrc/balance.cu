@@ -1,0 +1,481 @@
+// balance.cu -- the router's balance loss: pairs per expert, mean probability per expert, the loss of each sequence and its gradient.
+//
+// Math, per sequence of L rows (tokens) of E logits, of which the mask leaves n:
+//   p = softmax(l), or sigmoid(l_e) / sum of the sigmoids, which is the softmax of log sigmoid(l)
+//   f_e = number of ids equal to e,  P_e = sum of p_te,   loss = coef * E / (k n^2) * sum_e f_e P_e      (even load: coef)
+//   d l_te = d_loss * coef * E / (k n^2) * p_te * (f_e - sum_j f_j p_tj)  [ * (1 - sigmoid(l_te)) ]
+// The counts need the ids alone, which are a few percent of the bytes; with them known one pass over the logits gives both the sums
+// and the gradient, so every logit is read once and every gradient written once.  Bound: memory.
+//   count_kernel   pairs per expert of a piece of a sequence (integers; any order gives the same)
+//   balance_kernel a piece of a sequence per CTA, a row by 8, 16 or 32 lanes; sums of a piece in fp32, of the pieces in fp64 and always in
+//                  the same order, by the CTAs that finish last.  A sequence in one piece counts its pairs here as well: one launch.
+// In the gradient f_e is replaced by f_e - (sum_j f_j) / E, a constant less: it drops out (the p of a row add up to 1), and the difference
+// that remains does not lose the digits of the load all experts share.
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace chimere {
+namespace {
+
+constexpr int kB_Threads = 256, kB_Warps = kB_Threads / 32;
+constexpr int kB_Group = 32;          // pieces that are added up together, and groups of them
+constexpr int kB_MaxPieces = kB_Group * kB_Group;
+constexpr int kB_MaxCountPieces = 128;
+constexpr int kB_CountIds = 8192;     // ids of a counting CTA, where that gives few enough of them
+
+struct BalanceParams {
+    const void* logits;
+    int64_t ld, stride_s;
+    const int32_t* ids;               // null: the counts are given (backward)
+    const uint8_t* mask;              // or null
+    int S, L, E, k, mode;
+    float coef;
+    float* loss;                      // null: backward
+    int32_t* counts;
+    float* prob;
+    int32_t* tokens;
+    const float* d_loss;              // or null = 1
+    void* d_logits;                   // or null
+    int64_t ldd, stride_ds;
+    int vec;                          // rows of logits and gradient can be read and written four values at a time
+    int pieces, rows;                 // of a sequence; rows of a piece
+    int count_pieces, count_rows;     // (0: counted here)
+    int32_t* count_part;              // [S][count_pieces][E + 1]
+    float* part;                      // [S][pieces][E]
+    double* group_part;               // [S][groups][E]
+    int32_t* counters;                // [S][groups + 1]
+};
+__host__ __device__ inline int groups_of(int pieces) { return (pieces + kB_Group - 1) / kB_Group; }
+
+__device__ __forceinline__ bool counted(const BalanceParams& p, int64_t row) { return !p.mask || p.mask[row] != 0; }
+
+// Pairs and tokens of rows [r0, r1) of sequence s, added to hist[E] and *n (shared memory).
+__device__ __forceinline__ void count_rows(const BalanceParams& p, int s, int r0, int r1, int* hist, int* n) {
+    const int64_t base = (int64_t)s * p.L;
+    int mine = 0;
+    if (!p.mask) mine = threadIdx.x == 0 ? r1 - r0 : 0;
+    else for (int r = r0 + threadIdx.x; r < r1; r += kB_Threads) mine += p.mask[base + r] != 0;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if ((threadIdx.x & 31) == 0 && mine) atomicAdd(n, mine);
+    const int64_t total = (int64_t)(r1 - r0) * p.k;
+    const int32_t* ids = p.ids + (base + r0) * p.k;
+    for (int64_t i = threadIdx.x; i < total; i += kB_Threads) {
+        const int e = ids[i];
+        if (e >= 0 && e < p.E && (!p.mask || p.mask[base + r0 + i / p.k])) atomicAdd(hist + e, 1);
+    }
+}
+
+__global__ void __launch_bounds__(kB_Threads) count_kernel(BalanceParams p) {
+    __shared__ int hist[kMaxExperts + 1];
+    griddep_launch();
+    const int s = blockIdx.x / p.count_pieces, c = blockIdx.x % p.count_pieces;
+    for (int e = threadIdx.x; e <= p.E; e += kB_Threads) hist[e] = 0;
+    if (c == 0) {
+        const int n = groups_of(p.pieces) + 1;
+        for (int i = threadIdx.x; i < n; i += kB_Threads) p.counters[(int64_t)s * n + i] = 0;
+    }
+    __syncthreads();
+    const int r0 = (int)min((int64_t)c * p.count_rows, (int64_t)p.L), r1 = (int)min((int64_t)r0 + p.count_rows, (int64_t)p.L);
+    count_rows(p, s, r0, r1, hist, hist + p.E);
+    __syncthreads();
+    int32_t* out = p.count_part + (int64_t)blockIdx.x * (p.E + 1);
+    for (int e = threadIdx.x; e <= p.E; e += kB_Threads) out[e] = hist[e];
+}
+
+template <int TYPE> __device__ __forceinline__ float to_float(uint32_t bits) { return TYPE == CHIMERE_TYPE_F16 ? h2f(bits) : __uint_as_float(bits << 16); }
+template <int TYPE>
+__device__ __forceinline__ void load4(const void* base, int64_t at, int n, bool vec, float (&v)[4]) {   // n: values there are (0 .. 4)
+    if (TYPE == CHIMERE_TYPE_F32) {
+        const float* q = reinterpret_cast<const float*>(base) + at;
+        if (vec && n == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4*>(q));
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = i < n ? q[i] : __uint_as_float(0xFF800000u);
+        }
+    } else {
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(base) + at;
+        if (vec && n == 4) {
+            const uint2 a = __ldcs(reinterpret_cast<const uint2*>(q));
+            v[0] = to_float<TYPE>(a.x & 0xFFFFu); v[1] = to_float<TYPE>(a.x >> 16);
+            v[2] = to_float<TYPE>(a.y & 0xFFFFu); v[3] = to_float<TYPE>(a.y >> 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = i < n ? to_float<TYPE>(q[i]) : __uint_as_float(0xFF800000u);
+        }
+    }
+}
+template <int TYPE> __device__ __forceinline__ uint32_t from_float(float v) {
+    return TYPE == CHIMERE_TYPE_F16 ? (uint32_t)__half_as_ushort(__float2half_rn(v)) : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+template <int TYPE>
+__device__ __forceinline__ void store4(void* base, int64_t at, int n, bool vec, const float (&v)[4]) {
+    if (TYPE == CHIMERE_TYPE_F32) {
+        float* q = reinterpret_cast<float*>(base) + at;
+        if (vec && n == 4) __stcs(reinterpret_cast<float4*>(q), make_float4(v[0], v[1], v[2], v[3]));
+        else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i < n) q[i] = v[i];
+        }
+    } else {
+        uint16_t* q = reinterpret_cast<uint16_t*>(base) + at;
+        if (vec && n == 4) __stcs(reinterpret_cast<uint2*>(q), make_uint2(from_float<TYPE>(v[0]) | (from_float<TYPE>(v[1]) << 16), from_float<TYPE>(v[2]) | (from_float<TYPE>(v[3]) << 16)));
+        else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i < n) q[i] = (uint16_t)from_float<TYPE>(v[i]);
+        }
+    }
+}
+template <int LANES> __device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+}
+template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+
+struct BalanceShared {
+    int hist[kMaxExperts + 1];        // [E]: tokens
+    float g[kMaxExperts];
+    float part[kB_Warps][kMaxExperts];
+    double sum[kB_Warps];
+    int last;
+};
+
+// prob and loss from the probabilities' sums: sum_of(e), thread e % kB_Threads asks
+template <class Sum>
+__device__ __forceinline__ void finish_sequence(const BalanceParams& p, BalanceShared& sh, int s, Sum sum_of) {
+    const int n = sh.hist[p.E], tid = threadIdx.x;
+    double dot = 0.0;
+    for (int e = tid; e < p.E; e += kB_Threads) {
+        const double P = sum_of(e);
+        dot += (double)sh.hist[e] * P;
+        p.prob[(int64_t)s * p.E + e] = n > 0 ? (float)(P / n) : 0.0f;
+        p.counts[(int64_t)s * p.E + e] = sh.hist[e];
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    if ((tid & 31) == 0) sh.sum[tid >> 5] = dot;
+    __syncthreads();
+    if (tid == 0) {
+        dot = 0.0;
+        for (int w = 0; w < kB_Warps; ++w) dot += sh.sum[w];
+        p.loss[s] = n > 0 ? (float)((double)p.coef * p.E / ((double)p.k * n * n) * dot) : 0.0f;
+        p.tokens[s] = n;
+    }
+}
+
+// A row by LANES lanes, G groups of four values each: lane i owns values 4 (i + LANES g) .. + 3.
+template <int TYPE, int LANES, int G>
+__global__ void __launch_bounds__(kB_Threads) balance_kernel(BalanceParams p) {
+    constexpr int kRows = 32 / LANES, kU = G == 2 ? 2 : 4;   // rows of a warp at a time: kRows * kU
+    __shared__ BalanceShared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / LANES, i4 = 4 * (lane % LANES);
+    const int s = blockIdx.x / p.pieces, piece = blockIdx.x % p.pieces;
+    const int r0 = (int)min((int64_t)piece * p.rows, (int64_t)p.L), r1 = (int)min((int64_t)r0 + p.rows, (int64_t)p.L);
+    const bool stats = p.loss != nullptr, grad = p.d_logits != nullptr;
+
+    // the pairs of the whole sequence
+    for (int e = tid; e <= p.E; e += kB_Threads) sh.hist[e] = 0;
+    __syncthreads();
+    if (!p.ids) {
+        for (int e = tid; e < p.E; e += kB_Threads) sh.hist[e] = p.counts[(int64_t)s * p.E + e];
+        if (tid == 0) sh.hist[p.E] = p.tokens[s];
+    } else if (p.count_pieces == 0) {
+        count_rows(p, s, 0, p.L, sh.hist, sh.hist + p.E);
+    } else {
+        griddep_wait();
+        const int32_t* part = p.count_part + (int64_t)s * p.count_pieces * (p.E + 1);
+        for (int e = tid; e <= p.E; e += kB_Threads) {
+            int c = 0;
+#pragma unroll 8
+            for (int i = 0; i < p.count_pieces; ++i) c += __ldcg(part + (int64_t)i * (p.E + 1) + e);
+            sh.hist[e] = c;
+        }
+    }
+    __syncthreads();
+    if (grad) {
+        int all = 0;
+        for (int e = lane; e < p.E; e += 32) all += sh.hist[e];
+        all = __reduce_add_sync(0xffffffffu, all);
+        const double n = sh.hist[p.E], c = n > 0 ? (double)p.coef * p.E / (p.k * n * n) * (p.d_loss ? (double)p.d_loss[s] : 1.0) : 0.0;
+        for (int e = tid; e < p.E; e += kB_Threads) sh.g[e] = (float)(c * (sh.hist[e] - (double)all / p.E));
+        __syncthreads();
+    }
+    float g[G][4], acc[G][4];
+    int there[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+        const int e = i4 + 4 * LANES * j;
+        there[j] = max(0, min(4, p.E - e));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { acc[j][i] = 0.0f; g[j][i] = grad && e + i < p.E ? sh.g[e + i] : 0.0f; }
+    }
+
+    for (int row0 = r0 + warp * (kRows * kU); row0 < r1; row0 += kB_Warps * kRows * kU) {
+        float v[kU][G][4];
+        bool on[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = row0 + u * kRows + sub;
+            on[u] = r < r1 && counted(p, (int64_t)s * p.L + r);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int64_t at = (int64_t)s * p.stride_s + (int64_t)(row0 + u * kRows + sub) * p.ld + i4;
+#pragma unroll
+            for (int j = 0; j < G; ++j) load4<TYPE>(p.logits, at + 4 * LANES * j, on[u] ? there[j] : 0, p.vec, v[u][j]);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = row0 + u * kRows + sub;
+            float slope[G][4];   // sigmoid mode: 1 - sigmoid(l)
+            float mx = __uint_as_float(0xFF800000u);
+            bool nan = false;
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float& l = v[u][j][i];
+                    if (p.mode == CHIMERE_ROUTE_SIGMOID_NORM_SCALE) {
+                        const float t = expf(-fabsf(l));
+                        slope[j][i] = (l >= 0.0f ? t : 1.0f) / (1.0f + t);
+                        l = (l < 0.0f ? l : l >= 0.0f ? 0.0f : l) - log1pf(t);
+                    }
+                    nan |= l != l;
+                    mx = fmaxf(mx, l);
+                }
+            mx = lanes_max<LANES>(mx);
+            const bool none = mx == __uint_as_float(0xFF800000u);   // no finite logit: no probabilities
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float& l = v[u][j][i];
+                    l = none && !nan ? 0.0f : expf(l - mx);
+                    sum += l;
+                }
+            sum = lanes_sum<LANES>(sum);
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            float dot = 0.0f;
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float& l = v[u][j][i];
+                    l *= inv;
+                    if (on[u] && i < there[j]) acc[j][i] += l;
+                    dot = fmaf(l, g[j][i], dot);
+                }
+            if (!grad) continue;
+            dot = lanes_sum<LANES>(dot);
+            if (r >= r1) continue;
+            const int64_t at = (int64_t)s * p.stride_ds + (int64_t)r * p.ldd + i4;
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                float d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    d[i] = v[u][j][i] * (g[j][i] - dot);
+                    if (p.mode == CHIMERE_ROUTE_SIGMOID_NORM_SCALE) d[i] *= slope[j][i];
+                    if (!on[u]) d[i] = 0.0f;
+                }
+                store4<TYPE>(p.d_logits, at + 4 * LANES * j, there[j], p.vec, d);
+            }
+        }
+    }
+    griddep_launch();
+    if (!stats) return;
+
+    // the piece's sums: over the rows of a warp, then over the warps
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int d = LANES; d < 32; d <<= 1) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], d);
+            const int e = i4 + 4 * LANES * j + i;
+            if (sub == 0 && e < p.E) sh.part[warp][e] = acc[j][i];
+        }
+    __syncthreads();
+    auto of_piece = [&](int e) {
+        double v = 0.0;
+#pragma unroll
+        for (int w = 0; w < kB_Warps; ++w) v += (double)sh.part[w][e];
+        return v;
+    };
+    if (p.pieces == 1) {
+        finish_sequence(p, sh, s, of_piece);
+        return;
+    }
+    const int groups = groups_of(p.pieces), group = piece / kB_Group, in_group = min(kB_Group, p.pieces - group * kB_Group);
+    float* part = p.part + (int64_t)s * p.pieces * p.E;
+    for (int e = tid; e < p.E; e += kB_Threads) __stcg(part + (int64_t)piece * p.E + e, (float)of_piece(e));
+    __syncthreads();
+    if (tid == 0) sh.last = atom_add_acq_rel_gpu(p.counters + (int64_t)s * (groups + 1) + group, 1) == in_group - 1;
+    __syncthreads();
+    if (!sh.last) return;
+    auto of_group = [&](int e) {
+        double v = 0.0;
+#pragma unroll 8
+        for (int i = 0; i < in_group; ++i) v += (double)__ldcg(part + (int64_t)(group * kB_Group + i) * p.E + e);
+        return v;
+    };
+    if (groups == 1) {
+        finish_sequence(p, sh, s, of_group);
+        return;
+    }
+    double* gpart = p.group_part + (int64_t)s * groups * p.E;
+    for (int e = tid; e < p.E; e += kB_Threads) __stcg(gpart + (int64_t)group * p.E + e, of_group(e));
+    __syncthreads();
+    if (tid == 0) sh.last = atom_add_acq_rel_gpu(p.counters + (int64_t)s * (groups + 1) + groups, 1) == groups - 1;
+    __syncthreads();
+    if (!sh.last) return;
+    finish_sequence(p, sh, s, [&](int e) {
+        double v = 0.0;
+#pragma unroll 8
+        for (int i = 0; i < groups; ++i) v += __ldcg(gpart + (int64_t)i * p.E + e);
+        return v;
+    });
+}
+
+template <int TYPE>
+cudaError_t launch_balance_type(const BalanceParams& p, bool pdl, cudaStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)p.S * p.pieces));
+    auto go = [&](auto kernel) -> cudaError_t {
+        if (pdl) return launch_pdl(kernel, grid, kB_Threads, 0, stream, p);
+        kernel<<<grid, kB_Threads, 0, stream>>>(p);
+        return cudaGetLastError();
+    };
+    if (p.E <= 32) return go(balance_kernel<TYPE, 8, 1>);
+    if (p.E <= 64) return go(balance_kernel<TYPE, 16, 1>);
+    if (p.E <= 128) return go(balance_kernel<TYPE, 32, 1>);
+    return go(balance_kernel<TYPE, 32, 2>);
+}
+cudaError_t launch_balance(const BalanceParams& p, int type, bool pdl, cudaStream_t stream) {
+    return type == CHIMERE_TYPE_F32 ? launch_balance_type<CHIMERE_TYPE_F32>(p, pdl, stream)
+         : type == CHIMERE_TYPE_F16 ? launch_balance_type<CHIMERE_TYPE_F16>(p, pdl, stream) : launch_balance_type<CHIMERE_TYPE_BF16>(p, pdl, stream);
+}
+
+// Pieces of a sequence: as many CTAs as run at once, and at least kB_PieceRows rows in each; counting CTAs likewise.
+constexpr int kB_PieceRows = 64, kB_CtasPerSm = 3;
+struct Plan { int pieces, rows, count_pieces, count_rows; };
+Plan plan_of(int64_t S, int L, int k, bool stats) {
+    Plan r{};
+    int64_t n = ((int64_t)kB_CtasPerSm * 148 + S - 1) / S;      // (the scratch's size goes by it: a constant of the GPU this is written for)
+    const int64_t most = ((int64_t)L + kB_PieceRows - 1) / kB_PieceRows;
+    n = n > most ? most : n;
+    n = n > kB_MaxPieces ? kB_MaxPieces : n < 1 ? 1 : n;
+    r.rows = (int)((L + n - 1) / n);
+    r.pieces = r.rows > 0 ? (int)(((int64_t)L + r.rows - 1) / r.rows) : 1;
+    if (r.pieces < 1) r.pieces = 1;
+    if (stats && r.pieces > 1) {
+        int64_t c = ((int64_t)L * k + kB_CountIds - 1) / kB_CountIds;
+        c = c > kB_MaxCountPieces ? kB_MaxCountPieces : c;
+        r.count_rows = (int)((L + c - 1) / c);
+        r.count_pieces = (int)(((int64_t)L + r.count_rows - 1) / r.count_rows);
+    }
+    return r;
+}
+inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+struct Scratch { size_t count_part, part, group_part, counters, total; };
+Scratch scratch_of(const Plan& r, int64_t S, int E) {
+    Scratch a{};
+    if (r.pieces == 1) { a.total = 256; return a; }
+    size_t o = 0;
+    a.group_part = o; o += up256((size_t)S * groups_of(r.pieces) * E * 8);
+    a.part = o; o += up256((size_t)S * r.pieces * E * 4);
+    a.count_part = o; o += up256((size_t)S * r.count_pieces * (E + 1) * 4);
+    a.counters = o; o += up256((size_t)S * (groups_of(r.pieces) + 1) * 4);
+    a.total = o;
+    return a;
+}
+inline bool misaligned(const void* p, int to) { return ((uintptr_t)p & (uintptr_t)(to - 1)) != 0; }
+inline int rc_of(cudaError_t e) { return e == cudaSuccess ? 0 : -(100 + (int)e); }
+
+int check_dims(int64_t S, int64_t L, int E, int k, int mode, int type, int64_t ld, int64_t stride_s) {
+    if (S < 0 || L < 0 || S > 0x7FFFFFFF / kB_MaxPieces || L > 0x7FFFFF00 || E <= 0 || E > kMaxExperts || k <= 0 || k > kMaxExperts) return -2;
+    if (L > 0 && S > 0x7FFFFFFF / L) return -2;      // (counts and token numbers are 32-bit)
+    if (L > 0 && k > 0x7FFFFFFF / L) return -2;
+    if (mode != CHIMERE_ROUTE_SOFTMAX_RENORM && mode != CHIMERE_ROUTE_SIGMOID_NORM_SCALE) return -2;
+    if (ld < E || (S > 1 && stride_s < 0)) return -2;
+    if (type != CHIMERE_TYPE_F32 && type != CHIMERE_TYPE_F16 && type != CHIMERE_TYPE_BF16) return -3;
+    return 0;
+}
+int vectors(const void* p, int64_t ld, int64_t stride, int E, int type) {
+    const int size = type == CHIMERE_TYPE_F32 ? 4 : 2;
+    return E % 4 == 0 && !misaligned(p, 4 * size) && ld % 4 == 0 && stride % 4 == 0;
+}
+
+}  // namespace
+}  // namespace chimere
+
+using namespace chimere;
+
+extern "C" {
+
+size_t chimere_b200_balance_loss_bytes(int64_t S, int64_t L, int E, int top_k) {
+    if (check_dims(S, L, E, top_k, CHIMERE_ROUTE_SOFTMAX_RENORM, CHIMERE_TYPE_F32, E, 0)) return 0;
+    return S == 0 ? 256 : scratch_of(plan_of(S, (int)L, top_k, true), S, E).total;
+}
+
+int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_t stride_s, const int32_t* d_topk_idx, const uint8_t* d_mask, int64_t S, int64_t L, int E,
+                              int top_k, int route_mode, float coef, float* d_loss, int32_t* d_counts, float* d_prob, int32_t* d_tokens,
+                              const float* d_grad_loss, void* d_grad_logits, int64_t ld_grad, int64_t stride_grad_s, void* d_ws, size_t ws_bytes, cudaStream_t stream) {
+    const int rc = check_dims(S, L, E, top_k, route_mode, type, ld, stride_s);
+    if (rc) return rc;
+    if (d_grad_logits && (ld_grad < E || (S > 1 && stride_grad_s < (L > 0 ? (L - 1) * ld_grad + E : 0)))) return -2;
+    if (S == 0) return 0;
+    if (!d_loss || !d_counts || !d_prob || !d_tokens || !d_ws || (L > 0 && (!d_logits || !d_topk_idx))) return -1;
+    const int size = type == CHIMERE_TYPE_F32 ? 4 : 2;
+    if (misaligned(d_ws, 256) || misaligned(d_logits, size) || misaligned(d_grad_logits, size) || misaligned(d_topk_idx, 4) || misaligned(d_loss, 4) || misaligned(d_counts, 4) ||
+        misaligned(d_prob, 4) || misaligned(d_tokens, 4) || misaligned(d_grad_loss, 4)) return -5;
+    const Plan plan = plan_of(S, (int)L, top_k, true);
+    const Scratch a = scratch_of(plan, S, E);
+    if (ws_bytes < a.total) return -4;
+    uint8_t* ws = (uint8_t*)d_ws;
+    BalanceParams p{};
+    p.logits = d_logits; p.ld = ld; p.stride_s = stride_s; p.ids = d_topk_idx ? d_topk_idx : (const int32_t*)d_ws; p.mask = d_mask;
+    p.S = (int)S; p.L = (int)L; p.E = E; p.k = top_k; p.mode = route_mode; p.coef = coef;
+    p.loss = d_loss; p.counts = d_counts; p.prob = d_prob; p.tokens = d_tokens;
+    p.d_loss = d_grad_loss; p.d_logits = d_grad_logits; p.ldd = ld_grad; p.stride_ds = stride_grad_s;
+    p.vec = vectors(d_logits, ld, S > 1 ? stride_s : 0, E, type) && (!d_grad_logits || vectors(d_grad_logits, ld_grad, S > 1 ? stride_grad_s : 0, E, type));
+    p.pieces = plan.pieces; p.rows = plan.rows; p.count_pieces = plan.count_pieces; p.count_rows = plan.count_rows;
+    p.count_part = (int32_t*)(ws + a.count_part); p.part = (float*)(ws + a.part); p.group_part = (double*)(ws + a.group_part); p.counters = (int32_t*)(ws + a.counters);
+    if (p.count_pieces) {
+        count_kernel<<<(unsigned)(S * p.count_pieces), kB_Threads, 0, stream>>>(p);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return rc_of(e);
+    }
+    return rc_of(launch_balance(p, type, p.count_pieces > 0, stream));
+}
+
+int chimere_b200_balance_loss_backward(const void* d_logits, int type, int64_t ld, int64_t stride_s, const uint8_t* d_mask, const int32_t* d_counts, const int32_t* d_tokens,
+                                       int64_t S, int64_t L, int E, int top_k, int route_mode, float coef, const float* d_grad_loss, void* d_grad_logits, int64_t ld_grad,
+                                       int64_t stride_grad_s, cudaStream_t stream) {
+    const int rc = check_dims(S, L, E, top_k, route_mode, type, ld, stride_s);
+    if (rc) return rc;
+    if (ld_grad < E || (S > 1 && stride_grad_s < (L > 0 ? (L - 1) * ld_grad + E : 0))) return -2;
+    if (S == 0 || L == 0) return 0;
+    if (!d_logits || !d_counts || !d_tokens || !d_grad_logits) return -1;
+    const int size = type == CHIMERE_TYPE_F32 ? 4 : 2;
+    if (misaligned(d_logits, size) || misaligned(d_grad_logits, size) || misaligned(d_counts, 4) || misaligned(d_tokens, 4) || misaligned(d_grad_loss, 4)) return -5;
+    const Plan plan = plan_of(S, (int)L, top_k, false);
+    BalanceParams p{};
+    p.logits = d_logits; p.ld = ld; p.stride_s = stride_s; p.mask = d_mask;
+    p.S = (int)S; p.L = (int)L; p.E = E; p.k = top_k; p.mode = route_mode; p.coef = coef;
+    p.counts = const_cast<int32_t*>(d_counts); p.tokens = const_cast<int32_t*>(d_tokens);
+    p.d_loss = d_grad_loss; p.d_logits = d_grad_logits; p.ldd = ld_grad; p.stride_ds = stride_grad_s;
+    p.vec = vectors(d_logits, ld, S > 1 ? stride_s : 0, E, type) && vectors(d_grad_logits, ld_grad, S > 1 ? stride_grad_s : 0, E, type);
+    p.pieces = plan.pieces; p.rows = plan.rows;
+    return rc_of(launch_balance(p, type, false, stream));
+}
+
+}  // extern "C"

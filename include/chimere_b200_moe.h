@@ -406,6 +406,29 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
                               int H, int F, int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes,
                               int32_t* d_status, cudaStream_t stream);
 
+/* ------------------------------------------------------------ balance loss -------------- */
+/* What a router is trained and watched with: pairs per expert, mean probability per expert and the balance loss of each of S sequences of L tokens (S = 1: a batch),
+ * with the gradient of the logits.  No counterpart in the reference, which only logs the experts' load (moe_ffn.rs:120-131).
+ *   p = softmax(logits) (CHIMERE_ROUTE_SOFTMAX_RENORM) or sigmoid(logits) / their sum (CHIMERE_ROUTE_SIGMOID_NORM_SCALE), n = tokens that the mask leaves,
+ *   counts[e] = how often e stands in these tokens' ids (an id outside [0, E) counts nowhere), prob[e] = mean of p over them,
+ *   loss = coef * E / (top_k * n) * sum_e counts[e] * prob[e]     (an even load gives coef; n = 0 gives zeros),
+ *   grad_logits = grad_loss * d loss / d logits with the counts held constant; rows that the mask leaves out get zeros, whatever they hold.
+ * logits, grad_logits: row t of sequence s starts s * stride_s + t * ld elements behind the first, values side by side; topk_idx int32 [S][L][top_k], as the
+ * router leaves it, mask uint8 [S][L] or NULL, grad_loss f32 [S] or NULL (ones); loss f32 [S], counts int32 [S][E], prob f32 [S][E], tokens int32 [S] (n).
+ * E <= 256, top_k <= 256, S * L and L * top_k below 2^31.  A token whose logits are all -inf has no probabilities (it adds none and its gradient is
+ * zero; its pairs count); a NaN, or +inf under softmax, makes its sequence's loss and prob and its own gradient NaN.
+ * d_grad_logits NULL: no gradient.  d_ws: scratch of balance_loss_bytes, 256-byte aligned, used by no other call at the same time.  Sums are added in an order
+ * that depends on S, L, E and top_k alone: the same bits every time.  Errors as above. */
+size_t chimere_b200_balance_loss_bytes(int64_t S, int64_t L, int E, int top_k);
+int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_t stride_s, const int32_t* d_topk_idx, const uint8_t* d_mask,
+                              int64_t S, int64_t L, int E, int top_k, int route_mode, float coef, float* d_loss, int32_t* d_counts, float* d_prob,
+                              int32_t* d_tokens, const float* d_grad_loss, void* d_grad_logits, int64_t ld_grad, int64_t stride_grad_s,
+                              void* d_ws, size_t ws_bytes, cudaStream_t stream);
+/* The gradient alone, from the counts and tokens of the call above (or from those of several ranks, added up). */
+int chimere_b200_balance_loss_backward(const void* d_logits, int type, int64_t ld, int64_t stride_s, const uint8_t* d_mask, const int32_t* d_counts,
+                                       const int32_t* d_tokens, int64_t S, int64_t L, int E, int top_k, int route_mode, float coef,
+                                       const float* d_grad_loss, void* d_grad_logits, int64_t ld_grad, int64_t stride_grad_s, cudaStream_t stream);
+
 /* RMSNorm with unit weight over rows of length H: y = x / sqrt(mean(x^2) + eps). Used between
  * stacked layers. */
 int chimere_b200_rmsnorm(const float* d_x, float* d_y, int T, int H, float eps, cudaStream_t stream);
