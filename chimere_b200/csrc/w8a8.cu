@@ -171,17 +171,20 @@ cudaError_t launch_quantize(QuantParams p, int type, int64_t M, cudaStream_t str
 }
 
 // ------------------------------------------------------------------ product ----
-// tcgen05 kind::i8 with the weights as the MMA's 128 rows and the tokens as its columns, so that one kernel serves one token and
-// thousands: a tile is 128 weight rows (two such blocks, gate and up, where the activation joins them) x BN tokens, BN the narrowest of
-// 16 .. 256 that suits the batch.  Operands come by TMA as rows of 128 bytes (128-byte swizzle), zeros beyond K and beyond the last row.
-// Where a batch has fewer tiles than the GPU has SMs, a cluster of up to eight CTAs shares a tile, each with a part of K; their int32 sums
-// meet in shared memory over the cluster, exact in any order.
-//   warp 0     TMA            warp 1     MMA            warps 4..7   read the accumulators back, scale, store (thread = weight row)
+// tcgen05 kind::i8; operands by TMA as rows of 128 bytes (128-byte swizzle), zeros beyond K and beyond the last row.  Two kernels, which differ
+// in whose rows are the MMA's:
+//   few tokens (matmul_kernel)   128 weight rows (two such blocks, gate and up, where the activation joins them) x BN tokens, BN the narrowest of
+//       16 .. 256 that suits the batch.  Where there are fewer tiles than SMs a cluster of up to eight CTAs shares a tile, each with a
+//       part of K; their int32 sums meet in shared memory over the cluster, exact in any order.
+//   many tokens (wide_kernel)    256 tokens x 256 weight rows by a pair of CTAs (cta_group::2): each fetches its 128 tokens and 128 of the weight rows
+//       (with SwiGLU one the gate's, the other the up matrix'), half of what a CTA alone would need for the same MMAs.  A thread of the epilogue has
+//       one token's row: its scale and place are looked up once, its results go out 32 bytes at a time.
+// Rows of x that an index array picks (the dispatch's pairs) are fetched by tile::gather4, four rows an instruction, a lane's four rows each.
 // All waits are bounded: one that runs out makes the tile's outputs NaN and raises the status word.
-constexpr int kMM_Threads = 256;
 constexpr int kMM_KBytes = 128;          // of K per stage
 constexpr int kMM_ABytes = 128 * kMM_KBytes;
 constexpr int kMM_MaxStages = 12;
+constexpr int kMM_Threads = 384, kMM_FirstEpi = 4;   // warps 0 TMA, 1 MMA, 4 .. 11 epilogue (2 and 3 help to set up)
 
 struct MatmulParams {
     const float* sx;
@@ -190,27 +193,25 @@ struct MatmulParams {
     void* y;
     int64_t ldy, y_rows;
     const int32_t* offsets;    // grouped: [E + 1], else null
+    const int32_t* rows;       // rows of x by index (over rows_div), or null
     const int32_t* out_rows;   // or null
     int32_t* status;           // or null
     int M, N, K, E;
+    int rows_div, x_rows;
     int y_type, act;
-    int mt, nt;                // dense: token tiles; tiles of 128 outputs
+    int mt, nt;                // dense: token tiles; tiles of outputs
     int n_stages, split;
     int early;                 // the weights, scales and offsets do not come from the previous kernel
-};
-
-struct MatmulShared {
-    uint64_t full[kMM_MaxStages], empty[kMM_MaxStages];
-    uint64_t tfull[2], tempty[2];
-    uint64_t drain;
-    uint32_t tmem_base;
-    int failed;
-    float sx[2][256];
-    int row[2][256];
-    int scan[kMM_Threads / 32];
+    int vec;                   // wide: rows of y start on 32-byte boundaries
 };
 
 struct Tile { int expert, row0, ntok, n0; };
+
+// Token tiles per expert, summed over the experts in front, and where the experts' rows start.
+struct GroupTable {
+    int prefix[kMaxGroups + 1], start[kMaxGroups + 1];
+    int scan[kMM_Threads / 32];
+};
 
 __device__ __forceinline__ bool elect1() {
     uint32_t r;
@@ -219,33 +220,78 @@ __device__ __forceinline__ bool elect1() {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar) {   // ... to the barrier at this place in both CTAs of a pair
+    if (CTAS == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
+template <int CTAS>
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    if (CTAS == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __host__ constexpr uint32_t idesc_i8(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+template <int CTAS>
+__device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {
+    if (CTAS == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+    if (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 // rows of 128 bytes, 128-byte swizzle: groups of eight rows 1024 bytes apart; a step of 32 along K is 32 bytes of the start address
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+// CTAS 2: the copy lands in this CTA and is counted on the barrier at this place in the pair's first CTA
+template <int CTAS> __device__ __forceinline__ uint32_t bar_addr(uint64_t* bar) { return CTAS == 1 ? smem_u32(bar) : smem_u32(bar) & 0xFEFFFFFFu; }
+template <int CTAS>
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&r)[4], uint32_t bar) {
+    if (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar) : "memory");
 }
+template <int CTAS>
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    if (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+// TMEM -> registers, thread = lane, neighbouring columns (the wait in the same statement: no use of a value can move in front of it)
 __device__ __forceinline__ void ld16(uint32_t taddr, int* v) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
           "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -259,39 +305,127 @@ __device__ __forceinline__ int ld_cluster(uint32_t addr) {
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+
+// By all threads; returns the call's token tiles.
+template <int TOKENS>
+__device__ __forceinline__ int group_table(const MatmulParams& p, GroupTable& g) {
+    constexpr int kPer = (kMaxGroups + kMM_Threads - 1) / kMM_Threads;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int mine[kPer], start[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = tid * kPer + i;
+        mine[i] = start[i] = 0;
+        if (e < p.E) {
+            start[i] = min(max(p.offsets[e], 0), p.M);
+            mine[i] = (min(max(p.offsets[e + 1], start[i]), p.M) - start[i] + TOKENS - 1) / TOKENS;
+        }
+        sum += mine[i];
+    }
+    int scan = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += o;
+    }
+    if (lane == 31) g.scan[warp] = scan;
+    __syncthreads();
+    int before = scan - sum;
+    for (int w = 0; w < warp; ++w) before += g.scan[w];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = tid * kPer + i;
+        if (e <= p.E) { g.prefix[e] = before; g.start[e] = start[i]; }
+        before += mine[i];
+    }
+    __syncthreads();
+    return g.prefix[p.E];
+}
+static_assert((kMaxGroups + kMM_Threads - 1) / kMM_Threads * kMM_Threads > kMaxGroups, "a thread writes the table's end");
 
 // Tile `id` of the call: token tiles fastest, so that the CTAs at work at a time share weight rows.
-__device__ __forceinline__ Tile take_tile(const MatmulParams& p, const int* prefix, int id, int BN) {
+template <int TOKENS, int OUTS>
+__device__ __forceinline__ Tile take_tile(const MatmulParams& p, const GroupTable& g, int id) {
     Tile t;
     if (!p.offsets) {
         const int m = id % p.mt;
         t.expert = 0;
-        t.row0 = m * BN;
-        t.ntok = min(BN, p.M - t.row0);
-        t.n0 = id / p.mt * 128;
+        t.row0 = m * TOKENS;
+        t.ntok = min(TOKENS, p.M - t.row0);
+        t.n0 = id / p.mt * OUTS;
         return t;
     }
     // prefix[e]: token tiles of the experts in front of e; largest e with prefix[e] * nt <= id
+    const int tile = id / p.nt;
     int lo = 0, hi = p.E - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (prefix[mid] * p.nt <= id) lo = mid; else hi = mid - 1;
+        if (g.prefix[mid] <= tile) lo = mid; else hi = mid - 1;
     }
-    const int c = prefix[lo + 1] - prefix[lo], local = id - prefix[lo] * p.nt, m = local % c;
-    const int start = min(max(p.offsets[lo], 0), p.M), end = min(max(p.offsets[lo + 1], start), p.M);
+    const int c = g.prefix[lo + 1] - g.prefix[lo], local = id - g.prefix[lo] * p.nt, m = local % c, start = g.start[lo];
     t.expert = lo;
-    t.row0 = start + m * BN;
-    t.ntok = min(BN, end - t.row0);
-    t.n0 = local / c * 128;
+    t.row0 = start + m * TOKENS;
+    t.ntok = min(TOKENS, min(max(__ldg(p.offsets + lo + 1), start), p.M) - t.row0);
+    t.n0 = local / c * OUTS;
     return t;
 }
-
-__device__ __forceinline__ void put(const MatmulParams& p, int64_t row, int n, float v) {
-    const int64_t at = row * p.ldy + n;
-    if (p.y_type == kF32) reinterpret_cast<float*>(p.y)[at] = v;
-    else if (p.y_type == kBF16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
-    else reinterpret_cast<__half*>(p.y)[at] = __float2half_rn(v);
+// Row of x behind row `i` of the product, -1 if there is none.
+__device__ __forceinline__ int source_row(const MatmulParams& p, int i) {
+    if (!p.rows) return i;
+    const int r = __ldg(p.rows + i), s = r < 0 ? -1 : r / p.rows_div;
+    return s < p.x_rows ? s : -1;
 }
+// A warp's copies of `n` token rows (a stage's 128 bytes of each) from x: one box of BOX rows, or lane i rows 4 i .. 4 i + 3 (and so on, 128 further).
+template <int BOX> struct RowList { int r[(BOX + 127) / 128][4]; };
+template <int BOX>
+__device__ __forceinline__ void list_rows(const MatmulParams& p, RowList<BOX>& l, int row0, int n, int lane) {
+    if (!p.rows) return;
+#pragma unroll
+    for (int h = 0; h < (BOX + 127) / 128; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = 128 * h + 4 * lane + j;
+            l.r[h][j] = i < n ? max(source_row(p, row0 + i), 0) : 0;
+        }
+}
+template <int BOX> __device__ __forceinline__ uint32_t row_bytes_of(const MatmulParams& p, int n) { return n <= 0 ? 0u : (p.rows ? (uint32_t)(n + 3) / 4 * 4 : (uint32_t)BOX) * kMM_KBytes; }
+template <int CTAS, int BOX>
+__device__ __forceinline__ void load_rows(const MatmulParams& p, const CUtensorMap* map, const RowList<BOX>& l, uint32_t dst, int k0, int row0, int n, uint32_t bar, int lane) {
+    if (p.rows) {
+#pragma unroll
+        for (int h = 0; h < (BOX + 127) / 128; ++h)
+            if (128 * h + 4 * lane < n) tma_gather4<CTAS>(dst + (128 * h + 4 * lane) * kMM_KBytes, map, k0, l.r[h], bar);
+    } else if (n > 0 && elect1()) {
+        tma_2d<CTAS>(dst, map, k0, row0, bar);
+    }
+    __syncwarp();
+}
+
+template <int TYPE> struct Out;
+template <> struct Out<kF32> {
+    using T = float;
+    __device__ static __forceinline__ T of(float v) { return v; }
+};
+template <> struct Out<kF16> {
+    using T = __half;
+    __device__ static __forceinline__ T of(float v) { return __float2half_rn(v); }
+};
+template <> struct Out<kBF16> {
+    using T = __nv_bfloat16;
+    __device__ static __forceinline__ T of(float v) { return __float2bfloat16_rn(v); }
+};
+__device__ __forceinline__ void put(const MatmulParams& p, int64_t at, float v) {
+    if (p.y_type == kF32) reinterpret_cast<float*>(p.y)[at] = v;
+    else if (p.y_type == kBF16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = Out<kBF16>::of(v);
+    else reinterpret_cast<__half*>(p.y)[at] = Out<kF16>::of(v);
+}
+// (the channel's scale first: a token's may lie anywhere in fp32's range, and then only a result that does not fit overflows)
+__device__ __forceinline__ float scaled(int acc, float sw, float sx, float b) { return (float)acc * sw * sx + b; }
+__device__ __forceinline__ float relu2(float v) { v = v > 0.0f || v != v ? v : 0.0f; return v * v; }
+
 // what one thread needs of its weight row(s)
 struct Channel { float sw, sw_up, b, b_up; };
 __device__ __forceinline__ Channel channel(const MatmulParams& p, bool dual, int expert, int n) {
@@ -309,12 +443,20 @@ __device__ __forceinline__ Channel channel(const MatmulParams& p, bool dual, int
 }
 template <bool DUAL>
 __device__ __forceinline__ float finish(const MatmulParams& p, const Channel& c, float sx, int acc, int acc_up) {
-    // (the channel's scale first: a token's may lie anywhere in fp32's range, and then only a result that does not fit overflows)
-    float v = (float)acc * c.sw * sx + c.b;
-    if (DUAL) v = silu_mul_ref(v, (float)acc_up * c.sw_up * sx + c.b_up);
-    else if (p.act == CHIMERE_ACT_RELU2) { v = v > 0.0f || v != v ? v : 0.0f; v *= v; }
-    return v;
+    const float v = scaled(acc, c.sw, sx, c.b);
+    if (DUAL) return silu_mul_ref(v, scaled(acc_up, c.sw_up, sx, c.b_up));
+    return p.act == CHIMERE_ACT_RELU2 ? relu2(v) : v;
 }
+
+struct MatmulShared {
+    uint64_t full[kMM_MaxStages], empty[kMM_MaxStages];
+    uint64_t tfull[2], tempty[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int failed;
+    float sx[2][256];
+    int row[2][256];
+};
 
 template <int BN, bool DUAL>
 __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, MatmulParams p) {
@@ -324,46 +466,14 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
     static_assert(kTmemCols <= 512, "two accumulators fit");
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) MatmulShared sh;
-    __shared__ int prefix[kMaxGroups + 1];
+    __shared__ GroupTable table;
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int S = p.split, rank = S > 1 ? blockIdx.x % S : 0, first = blockIdx.x / S, step = gridDim.x / S;
     const uint32_t stages = smem_u32(smem);
 
     if (!p.early) griddep_wait();
-    int total = p.mt * p.nt;
-    if (p.offsets) {   // token tiles per expert, summed over the experts in front
-        int mine[kMaxGroups / kMM_Threads], sum = 0;
-#pragma unroll
-        for (int i = 0; i < kMaxGroups / kMM_Threads; ++i) {
-            const int e = tid * (kMaxGroups / kMM_Threads) + i;
-            mine[i] = 0;
-            if (e < p.E) {
-                const int start = min(max(p.offsets[e], 0), p.M), end = min(max(p.offsets[e + 1], start), p.M);
-                mine[i] = (end - start + BN - 1) / BN;
-            }
-            sum += mine[i];
-        }
-        int scan = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, scan, d);
-            if (lane >= d) scan += o;
-        }
-        if (lane == 31) sh.scan[warp] = scan;
-        __syncthreads();
-        int before = scan - sum;
-        for (int w = 0; w < warp; ++w) before += sh.scan[w];
-#pragma unroll
-        for (int i = 0; i < kMaxGroups / kMM_Threads; ++i) {
-            const int e = tid * (kMaxGroups / kMM_Threads) + i;
-            if (e <= p.E) prefix[e] = before;
-            before += mine[i];
-        }
-        if (tid == kMM_Threads - 1 && p.E == kMaxGroups) prefix[kMaxGroups] = before;
-        __syncthreads();
-        total = prefix[p.E] * p.nt;
-    }
+    const int total = (p.offsets ? group_table<BN>(p, table) : p.mt) * p.nt;
     if (first >= total) {   // (the whole cluster; nothing has been allocated)
         griddep_launch();
         return;
@@ -376,10 +486,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
         sh.failed = 0;
         mbar_fence_init();
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(kTmemCols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<1>(&sh.tmem_base, kTmemCols);
     fence_before();
     __syncthreads();
     fence_after();
@@ -394,19 +501,20 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
         uint32_t ph = 0, used = 0;
         bool ok = true, waited = !p.early;
         for (int id = first; ok && id < total; id += step) {
-            const Tile t = take_tile(p, prefix, id, BN);
+            const Tile t = take_tile<BN, 128>(p, table, id);
+            RowList<BN> rows;
+            list_rows<BN>(p, rows, t.row0, t.ntok, lane);
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!mbar_wait(&sh.empty[st], ph ^ 1u)) { ok = false; break; }
-                const uint32_t dst = stages + st * kStage;
+                const uint32_t dst = stages + st * kStage, bar = smem_u32(&sh.full[st]);
                 if (elect1()) {
-                    mbar_expect_tx(&sh.full[st], kStage);
-                    tma_3d(dst, &map_w, kb * kMM_KBytes, t.n0, t.expert, &sh.full[st]);
-                    if (DUAL) tma_3d(dst + kMM_ABytes, &map_w, kb * kMM_KBytes, p.N + t.n0, t.expert, &sh.full[st]);
+                    mbar_expect_tx(&sh.full[st], kMM_ABytes * (DUAL ? 2 : 1) + row_bytes_of<BN>(p, t.ntok));
+                    tma_3d<1>(dst, &map_w, kb * kMM_KBytes, t.n0, t.expert, bar);
+                    if (DUAL) tma_3d<1>(dst + kMM_ABytes, &map_w, kb * kMM_KBytes, p.N + t.n0, t.expert, bar);
                 }
                 __syncwarp();
                 if (!waited) { griddep_wait(); waited = true; }
-                if (elect1()) tma_2d(dst + kMM_ABytes * (DUAL ? 2 : 1), &map_x, kb * kMM_KBytes, t.row0, &sh.full[st]);
-                __syncwarp();
+                load_rows<1, BN>(p, &map_x, rows, dst + kMM_ABytes * (DUAL ? 2 : 1), kb * kMM_KBytes, t.row0, t.ntok, bar, lane);
                 used |= 1u << st;
                 if (++st == p.n_stages) { st = 0; ph ^= 1u; }
             }
@@ -417,7 +525,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
                 if (used >> i & 1u) mbar_wait(&sh.full[i], (i < st ? ph : ph ^ 1u));
         }
     } else if (warp == 1) {
-        constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t idesc = idesc_i8(128, BN);
         int st = 0, n = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -434,41 +542,43 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
 #pragma unroll
                     for (int k = 0; k < kMM_KBytes / 32; ++k) {
                         const uint32_t acc = kb > kb0 || k > 0;
-                        mma_i8(d, desc_sw128(a + 32 * k), desc_sw128(b + 32 * k), idesc, acc);
-                        if (DUAL) mma_i8(d + BN, desc_sw128(a + kMM_ABytes + 32 * k), desc_sw128(b + 32 * k), idesc, acc);
+                        mma_i8<1>(d, desc_sw128(a + 32 * k), desc_sw128(b + 32 * k), idesc, acc);
+                        if (DUAL) mma_i8<1>(d + BN, desc_sw128(a + kMM_ABytes + 32 * k), desc_sw128(b + 32 * k), idesc, acc);
                     }
-                    commit(&sh.empty[st]);
+                    commit<1>(&sh.empty[st]);
                 }
                 __syncwarp();
                 if (++st == p.n_stages) { st = 0; ph ^= 1u; }
             }
-            if (ok && elect1()) commit(&sh.tfull[buf]);
+            if (ok && elect1()) commit<1>(&sh.tfull[buf]);
             __syncwarp();
         }
         if (!ok) {
             sh.failed = 1;
-            if (elect1()) commit(&sh.drain);   // (the MMAs under way)
+            if (elect1()) commit<1>(&sh.drain);   // (the MMAs under way)
             __syncwarp();
             mbar_wait(&sh.drain, 0);
         }
-    } else if (warp >= 4) {
-        const int q = warp & 3, row = q * 32 + lane, et = tid - 128;
-        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+    } else if (warp >= kMM_FirstEpi) {
+        // four warps take every other tile: what a tile's scales and places cost to look up passes behind the other four's tile
+        const int q = warp & 3, buf = (warp - kMM_FirstEpi) >> 2, row = q * 32 + lane;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + buf * kAccCols;
         bool ok = true;
         griddep_wait();   // (the tokens' scales; and nothing of y is written before what used its memory has ended)
-        int n = 0;
-        for (int id = first; id < total; id += step, ++n) {
-            const Tile t = take_tile(p, prefix, id, BN);
-            const int buf = n & 1;
+        uint32_t ph = 0;
+        for (int id = first + buf * step; id < total; id += 2 * step, ph ^= 1u) {
+            const Tile t = take_tile<BN, 128>(p, table, id);
             const Channel ch = channel(p, DUAL, t.expert, t.n0 + row);
             if (S == 1) {
-                for (int i = et; i < t.ntok; i += 128) {
-                    sh.sx[buf][i] = p.sx[t.row0 + i];
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");   // (the tile before has been read)
+                for (int i = row; i < t.ntok; i += 128) {
+                    const int r = source_row(p, t.row0 + i);
+                    sh.sx[buf][i] = r < 0 ? 0.0f : p.sx[r];
                     sh.row[buf][i] = p.out_rows ? p.out_rows[t.row0 + i] : t.row0 + i;
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");
             }
-            if (ok && !mbar_wait(&sh.tfull[buf], (n >> 1) & 1)) { ok = false; sh.failed = 1; }
+            if (ok && !mbar_wait(&sh.tfull[buf], ph)) { ok = false; sh.failed = 1; }
             fence_after();
             if (S > 1) {   // this CTA's part of the sums, over the operands' buffers: [gate / up][token][128]
                 int* part = reinterpret_cast<int*>(smem);
@@ -476,8 +586,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
 #pragma unroll
                     for (int h = 0; h < (DUAL ? 2 : 1); ++h) {
                         int v[16];
-                        ld16(taddr + buf * kAccCols + h * BN + c0, v);
-                        wait_ld();
+                        ld16(taddr + h * BN + c0, v);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) part[(h * BN + c0 + j) * 128 + row] = v[j];
                     }
@@ -486,9 +595,8 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
             }
             for (int c0 = 0; c0 < t.ntok; c0 += 16) {
                 int v[16], u[16];
-                ld16(taddr + buf * kAccCols + c0, v);
-                if (DUAL) ld16(taddr + buf * kAccCols + BN + c0, u);
-                wait_ld();
+                ld16(taddr + c0, v);
+                if (DUAL) ld16(taddr + BN + c0, u);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int m = c0 + j;
@@ -496,7 +604,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
                         const int64_t r = sh.row[buf][m];
                         float o = finish<DUAL>(p, ch, sh.sx[buf][m], v[j], DUAL ? u[j] : 0);
                         if (!ok) o = __uint_as_float(0x7FC00000u);
-                        if (r >= 0 && r < p.y_rows) put(p, r, t.n0 + row, o);
+                        if (r >= 0 && r < p.y_rows) put(p, r * p.ldy + t.n0 + row, o);
                     }
                 }
             }
@@ -508,9 +616,9 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    if (warp == 1) tmem_free<1>(tmem, kTmemCols);   // (in front of the cluster's barrier: who waits for a neighbour holds none)
     if (S > 1) {
-        const Tile t = take_tile(p, prefix, first, BN);
+        const Tile t = take_tile<BN, 128>(p, table, first);
         griddep_wait();
         cluster_sync();   // every part is there
         bool bad = false;
@@ -524,12 +632,261 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
                 if (DUAL) up += ld_cluster(cluster_addr(stages + 4 * (i + BN * 128), s));
             }
             const int64_t r = p.out_rows ? p.out_rows[t.row0 + m] : t.row0 + m;
-            float o = finish<DUAL>(p, channel(p, DUAL, t.expert, n), p.sx[t.row0 + m], acc, up);
+            const int src = source_row(p, t.row0 + m);
+            float o = finish<DUAL>(p, channel(p, DUAL, t.expert, n), src < 0 ? 0.0f : p.sx[src], acc, up);
             if (bad) o = __uint_as_float(0x7FC00000u);
-            if (r >= 0 && r < p.y_rows) put(p, r, n, o);
+            if (r >= 0 && r < p.y_rows) put(p, r * p.ldy + n, o);
         }
         cluster_sync();   // ... and has been read
     }
+    if (tid == 0 && sh.failed && p.status) atomicOr(p.status, kStatusWaitTimeout);
+}
+
+// ---- many tokens ----
+constexpr int kW_Tokens = 256, kW_Cols = 256;                 // of a pair's tile: tokens, weight rows (SwiGLU: 128 gate, 128 up)
+constexpr int kW_Stage = 2 * kMM_ABytes, kW_Stages = 6, kW_StagesTurned = 5;
+constexpr int kW_EpiWarps = 8;
+constexpr int kW_TurnFloats = 32 * 33;                        // a warp's 32 x 32 results on their way to rows that are not aligned
+constexpr int kW_Smem = 1024 + kW_Stages * kW_Stage, kW_SmemTurned = 1024 + kW_StagesTurned * kW_Stage + kW_EpiWarps * kW_TurnFloats * 4;
+
+struct WideShared {
+    uint64_t full[kW_Stages], empty[kW_Stages];
+    uint64_t tfull[2], tempty[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int failed;
+    float sw[2][kW_Cols], bias[2][kW_Cols];
+};
+
+__device__ __forceinline__ void ld32(uint32_t taddr, int (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void stg256(void* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+// 32 results of one row, all of them inside it and 32-byte aligned
+template <int TYPE>
+__device__ __forceinline__ void store_row32(typename Out<TYPE>::T* y, const float (&o)[32]) {
+    if (TYPE == kF32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) stg256(y + 8 * i, reinterpret_cast<const uint32_t*>(o) + 8 * i);
+    } else {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (TYPE == kF16) {
+                const __half2 h = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        stg256(y, w);
+        stg256(y + 16, w + 8);
+    }
+}
+// A warp's 32 rows x 32 results from column n on.  r: this lane's row of y, -1 if it has none.
+template <int TYPE>
+__device__ __forceinline__ void store_block(const MatmulParams& p, float* turn, int64_t r, int n, const float (&o)[32], int lane) {
+    using T = typename Out<TYPE>::T;
+    T* y = reinterpret_cast<T*>(p.y);
+    if (p.vec) {
+        if (r >= 0) {
+            if (n + 32 <= p.N) store_row32<TYPE>(y + r * p.ldy + n, o);
+            else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) if (n + j < p.N) y[r * p.ldy + n + j] = Out<TYPE>::of(o[j]);
+            }
+        }
+        return;
+    }
+    // a lane per column: 32 neighbours of a row at a time
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = o[j];
+    __syncwarp();
+    const bool in = n + lane < p.N;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+        const int64_t ri = __shfl_sync(0xffffffffu, r, i);
+        if (ri >= 0 && in) y[ri * p.ldy + n + lane] = Out<TYPE>::of(turn[i * 33 + lane]);
+    }
+}
+
+template <int TYPE, bool DUAL>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, MatmulParams p) {
+    constexpr int kOuts = DUAL ? 128 : 256;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) WideShared sh;
+    __shared__ GroupTable table;
+    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int rank = blockIdx.x & 1, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const uint32_t stages = smem_u32(smem);
+
+    if (!p.early) griddep_wait();
+    const int total = (p.offsets ? group_table<kW_Tokens>(p, table) : p.mt) * p.nt;
+    if (first >= total) {   // (both CTAs; nothing has been allocated)
+        griddep_launch();
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < p.n_stages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.tfull[i], 1); mbar_init(&sh.tempty[i], 2 * kW_EpiWarps); }
+        mbar_init(&sh.drain, 1);
+        sh.failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc<2>(&sh.tmem_base, 512);
+    fence_before();
+    __syncthreads();
+    cluster_sync();   // the pair's barriers stand before a copy or an MMA reaches over
+    fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    if (tid == 0) griddep_launch();
+    const int nkb = (p.K + kMM_KBytes - 1) / kMM_KBytes;
+
+    if (warp == 0) {
+        int st = 0;
+        uint32_t ph = 0, used = 0;
+        bool ok = true, waited = !p.early;
+        for (int id = first; ok && id < total; id += step) {
+            const Tile t = take_tile<kW_Tokens, kOuts>(p, table, id);
+            const int row0 = t.row0 + 128 * rank, n = max(0, min(128, t.ntok - 128 * rank));
+            const uint32_t bytes = 2 * kMM_ABytes + row_bytes_of<128>(p, min(128, t.ntok)) + row_bytes_of<128>(p, max(0, t.ntok - 128));
+            const int wrow = DUAL ? rank * p.N + t.n0 : t.n0 + 128 * rank;
+            RowList<128> rows;
+            list_rows<128>(p, rows, row0, n, lane);
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (!mbar_wait(&sh.empty[st], ph ^ 1u)) { ok = false; break; }
+                const uint32_t dst = stages + st * kW_Stage, bar = bar_addr<2>(&sh.full[st]);
+                if (elect1()) {
+                    if (rank == 0) mbar_expect_tx(&sh.full[st], bytes);   // (both CTAs' copies)
+                    tma_3d<2>(dst + kMM_ABytes, &map_w, kb * kMM_KBytes, wrow, t.expert, bar);
+                }
+                __syncwarp();
+                if (!waited) { griddep_wait(); waited = true; }
+                load_rows<2, 128>(p, &map_x, rows, dst, kb * kMM_KBytes, row0, n, bar, lane);
+                used |= 1u << st;
+                if (++st == p.n_stages) { st = 0; ph ^= 1u; }
+            }
+        }
+        if (!ok) {   // the copies under way, which the first CTA's barriers count, land before the pair goes
+            sh.failed = 1;
+            if (rank == 0)
+                for (int i = 0; i < p.n_stages; ++i)
+                    if (used >> i & 1u) mbar_wait(&sh.full[i], (i < st ? ph : ph ^ 1u));
+        }
+    } else if (warp == 1 && rank == 0) {
+        constexpr uint32_t idesc = idesc_i8(2 * 128, kW_Cols);
+        int st = 0, n = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int id = first; ok && id < total; id += step, ++n) {
+            const int buf = n & 1;
+            if (!mbar_wait(&sh.tempty[buf], ((n >> 1) & 1) ^ 1u)) { ok = false; break; }
+            fence_after();
+            const uint32_t d = tmem + buf * kW_Cols;
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (!mbar_wait(&sh.full[st], ph)) { ok = false; break; }
+                fence_after();
+                if (elect1()) {
+                    const uint32_t a = stages + st * kW_Stage, b = a + kMM_ABytes;
+#pragma unroll
+                    for (int k = 0; k < kMM_KBytes / 32; ++k) mma_i8<2>(d, desc_sw128(a + 32 * k), desc_sw128(b + 32 * k), idesc, kb > 0 || k > 0);
+                    commit<2>(&sh.empty[st]);
+                }
+                __syncwarp();
+                if (++st == p.n_stages) { st = 0; ph ^= 1u; }
+            }
+            if (ok && elect1()) commit<2>(&sh.tfull[buf]);
+            __syncwarp();
+        }
+        if (!ok) {
+            sh.failed = 1;
+            if (elect1()) commit<2>(&sh.drain);   // (the MMAs under way)
+            __syncwarp();
+            mbar_wait(&sh.drain, 0);
+        }
+    } else if (warp >= kMM_FirstEpi) {
+        const int q = warp & 3, half = (warp - kMM_FirstEpi) >> 2, row = q * 32 + lane, et = tid - 32 * kMM_FirstEpi;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+        float* turn = reinterpret_cast<float*>(smem + kW_StagesTurned * kW_Stage) + (warp - kMM_FirstEpi) * kW_TurnFloats;   // (where rows are not aligned)
+        bool ok = true;
+        griddep_wait();   // (the tokens' scales; and nothing of y is written before what used its memory has ended)
+        int n = 0;
+        for (int id = first; id < total; id += step, ++n) {
+            const Tile t = take_tile<kW_Tokens, kOuts>(p, table, id);
+            const int buf = n & 1;
+            {   // scale and bias of accumulator column `et`
+                const int c = DUAL ? t.n0 + (et & 127) : t.n0 + et;
+                const int64_t at = ((int64_t)t.expert * (DUAL ? 2 : 1) + (DUAL ? et >> 7 : 0)) * p.N + c;
+                sh.sw[buf][et] = c < p.N ? p.sw[at] : 0.0f;
+                sh.bias[buf][et] = c < p.N && p.bias ? p.bias[at] : 0.0f;
+            }
+            const int i = 128 * rank + row;   // this thread's token of the tile
+            int64_t r = -1;
+            float sx = 0.0f;
+            if (i < t.ntok) {
+                const int src = source_row(p, t.row0 + i);
+                if (src >= 0) sx = p.sx[src];
+                r = p.out_rows ? p.out_rows[t.row0 + i] : t.row0 + i;
+                if (r < 0 || r >= p.y_rows) r = -1;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (ok && !mbar_wait(&sh.tfull[buf], (n >> 1) & 1)) { ok = false; sh.failed = 1; }
+            fence_after();
+            if (!ok) sx = __uint_as_float(0x7FC00000u);
+            if (128 * rank + q * 32 < t.ntok) {
+#pragma unroll 1
+                for (int c0 = half * (kOuts / 2); c0 < (half + 1) * (kOuts / 2); c0 += 32) {
+                    if (t.n0 + c0 >= p.N) break;
+                    int v[32];
+                    float o[32];
+                    ld32(taddr + buf * kW_Cols + c0, v);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 s = *reinterpret_cast<const float4*>(&sh.sw[buf][c0 + j]), b = *reinterpret_cast<const float4*>(&sh.bias[buf][c0 + j]);
+                        o[j] = scaled(v[j], s.x, sx, b.x); o[j + 1] = scaled(v[j + 1], s.y, sx, b.y);
+                        o[j + 2] = scaled(v[j + 2], s.z, sx, b.z); o[j + 3] = scaled(v[j + 3], s.w, sx, b.w);
+                    }
+                    if (DUAL) {
+                        ld32(taddr + buf * kW_Cols + 128 + c0, v);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 s = *reinterpret_cast<const float4*>(&sh.sw[buf][128 + c0 + j]), b = *reinterpret_cast<const float4*>(&sh.bias[buf][128 + c0 + j]);
+                            o[j] = silu_mul_ref(o[j], scaled(v[j], s.x, sx, b.x));
+                            o[j + 1] = silu_mul_ref(o[j + 1], scaled(v[j + 1], s.y, sx, b.y));
+                            o[j + 2] = silu_mul_ref(o[j + 2], scaled(v[j + 2], s.z, sx, b.z));
+                            o[j + 3] = silu_mul_ref(o[j + 3], scaled(v[j + 3], s.w, sx, b.w));
+                        }
+                    } else if (p.act == CHIMERE_ACT_RELU2) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = relu2(o[j]);
+                    }
+                    store_block<TYPE>(p, turn, r, t.n0 + c0, o, lane);
+                }
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(cluster_addr(smem_u32(&sh.tempty[buf]), 0));
+        }
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();   // nothing of the other CTA's reaches over any more
+    fence_after();
+    if (warp == 1) tmem_free<2>(tmem, 512);
     if (tid == 0 && sh.failed && p.status) atomicOr(p.status, kStatusWaitTimeout);
 }
 
@@ -564,19 +921,33 @@ struct MatmulCall {
     bool dual;
 };
 
+cudaLaunchConfig_t launch_config(int grid, size_t smem, int cluster, bool pdl, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kMM_Threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    int n = 0;
+    if (pdl) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
+    if (cluster > 1) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = cluster; attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1; ++n; }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cfg;
+}
+
 template <int BN, bool DUAL>
 int launch_tile(const MatmulCall& c, int tiles, int split, bool pdl, cudaStream_t stream) {
     constexpr int kStage = kMM_ABytes * (DUAL ? 2 : 1) + BN * kMM_KBytes;
     static bool done[64];
     CUtensorMap mx, mw;
     MatmulParams p = c.p;
-    if (!make_map(&mx, c.x, p.K, p.M, 1, c.ldx, 0, BN, 2)) return -5;
+    if (!make_map(&mx, c.x, p.K, p.x_rows, 1, c.ldx, 0, p.rows ? 1 : BN, 2)) return -5;
     if (!make_map(&mw, c.w, p.K, (DUAL ? 2 : 1) * (int64_t)p.N, p.E, c.ldw, c.w_plane, 128, 3)) return -5;
     const int nkb = (p.K + kMM_KBytes - 1) / kMM_KBytes, most = (200 * 1024) / kStage;
     int stages = (nkb + split - 1) / split;
     const int parts = split > 1 ? (BN * (DUAL ? 2 : 1) * 512 + kStage - 1) / kStage : 1;   // room for the sums
     stages = stages < parts ? parts : stages;
-    if (split == 1 && stages < 2) stages = 2;
+    if (split == 1 && stages < most) stages = most;
     stages = stages > most ? most : stages;
     stages = stages > kMM_MaxStages ? kMM_MaxStages : stages;
     p.n_stages = stages;
@@ -584,21 +955,35 @@ int launch_tile(const MatmulCall& c, int tiles, int split, bool pdl, cudaStream_
     p.mt = (p.M + BN - 1) / BN;
     p.nt = (p.N + 127) / 128;
     auto kernel = matmul_kernel<BN, DUAL>;
-    constexpr int kMostSmem = 1024 + 200 * 1024;
-    cudaError_t e = max_smem_once(kernel, kMostSmem, done);
+    cudaError_t e = max_smem_once(kernel, 1024 + 200 * 1024, done);
     if (e != cudaSuccess) return -(100 + (int)e);
     const int grid = split > 1 ? tiles * split : tiles < sm_count() ? tiles : sm_count();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kMM_Threads);
-    cfg.dynamicSmemBytes = 1024 + (size_t)stages * kStage;
-    cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (pdl) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
-    if (split > 1) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = split; attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1; ++n; }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
+    const cudaLaunchConfig_t cfg = launch_config(grid, 1024 + (size_t)stages * kStage, split, pdl, stream, attr);
+    e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, p);
+    return e == cudaSuccess ? 0 : -(100 + (int)e);
+}
+
+template <int TYPE, bool DUAL>
+int launch_wide(const MatmulCall& c, int64_t tiles, bool pdl, cudaStream_t stream) {
+    static bool done[64];
+    CUtensorMap mx, mw;
+    MatmulParams p = c.p;
+    if (!make_map(&mx, c.x, p.K, p.x_rows, 1, c.ldx, 0, p.rows ? 1 : 128, 2)) return -5;
+    if (!make_map(&mw, c.w, p.K, (DUAL ? 2 : 1) * (int64_t)p.N, p.E, c.ldw, c.w_plane, 128, 3)) return -5;
+    constexpr int kOuts = DUAL ? 128 : 256, kSize = TYPE == kF32 ? 4 : 2;
+    p.mt = (p.M + kW_Tokens - 1) / kW_Tokens;
+    p.nt = (p.N + kOuts - 1) / kOuts;
+    p.split = 1;
+    p.vec = ((uintptr_t)p.y & 31) == 0 && p.ldy * kSize % 32 == 0;
+    p.n_stages = p.vec ? kW_Stages : kW_StagesTurned;
+    auto kernel = wide_kernel<TYPE, DUAL>;
+    constexpr int kMost = kW_Smem > kW_SmemTurned ? kW_Smem : kW_SmemTurned;
+    cudaError_t e = max_smem_once(kernel, kMost, done);
+    if (e != cudaSuccess) return -(100 + (int)e);
+    const int pairs = sm_count() / 2;
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg = launch_config(2 * (int)(tiles < pairs ? tiles : pairs), p.vec ? kW_Smem : kW_SmemTurned, 1, pdl, stream, attr);
     e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, p);
     return e == cudaSuccess ? 0 : -(100 + (int)e);
 }
@@ -617,15 +1002,28 @@ int launch_matmul(const MatmulCall& c, bool pdl, cudaStream_t stream) {
     const int widest = c.dual ? 128 : 256;
     int bn = 16;
     double best = 1e30;
-    const int64_t per = c.p.offsets ? (c.p.M + c.p.E - 1) / c.p.E : c.p.M;   // (grouped: of an even load)
+    const int64_t per = c.p.offsets ? (c.p.M + c.p.E - 1) / c.p.E : c.p.M, of = c.p.offsets ? c.p.E : 1;   // (grouped: of an even load)
     for (int b = 16; b <= widest; b *= 2) {
         const double mma = 2.1 * b * (c.dual ? 2 : 1), load = (16384.0 * (c.dual ? 2 : 1) + 128.0 * b) / 50.0;
-        const int64_t tiles = (c.p.offsets ? c.p.E * ((per + b - 1) / b) : (per + b - 1) / b) * nt;
+        const int64_t tiles = of * ((per + b - 1) / b) * nt;
         const double cost = (double)((tiles + sms - 1) / sms) * (mma > load ? mma : load);
         if (cost < best) { best = cost; bn = b; }
     }
+    {   // a pair's tile: 256 x 256 in the time of its MMAs
+        const int outs = c.dual ? 128 : 256;
+        const int64_t wide = of * ((per + kW_Tokens - 1) / kW_Tokens) * ((c.p.N + outs - 1) / outs);
+        if (per > 64 && (double)((wide + sms / 2 - 1) / (sms / 2)) * 2.1 * 256 * 1.2 < best) {
+            const int64_t tiles = token_tiles(c, kW_Tokens) * ((c.p.N + outs - 1) / outs);
+            if (tiles > 0x3FFFFFFF) return -2;
+            switch (c.p.y_type) {
+                case kF32: return c.dual ? launch_wide<kF32, true>(c, tiles, pdl, stream) : launch_wide<kF32, false>(c, tiles, pdl, stream);
+                case kF16: return c.dual ? launch_wide<kF16, true>(c, tiles, pdl, stream) : launch_wide<kF16, false>(c, tiles, pdl, stream);
+                default: return c.dual ? launch_wide<kBF16, true>(c, tiles, pdl, stream) : launch_wide<kBF16, false>(c, tiles, pdl, stream);
+            }
+        }
+    }
     const int64_t tiles = token_tiles(c, bn) * nt;
-    if (tiles > 0x7FFFFFFF) return -2;
+    if (tiles > 0x3FFFFFFF) return -2;
     int split = 1;
     const int nkb = (c.p.K + kMM_KBytes - 1) / kMM_KBytes;
     if (bn <= 64)
@@ -658,7 +1056,7 @@ int check_quantize(const void* x, int type, int64_t ldx, int64_t x_rows, const i
     return 0;
 }
 int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, int E, int64_t M, int N, int K,
-                 int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows) {
+                 int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* rows, int rows_div, int64_t x_rows, const int32_t* out_rows) {
     const int64_t R = (act == CHIMERE_ACT_SWIGLU ? 2 : 1) * (int64_t)N;
     if (M < 0 || M > 0x7FFFFFFF || N <= 0 || R > 0x7FFFFF00 || K <= 0 || K > kMaxK || E <= 0 || E > kMaxGroups) return -2;
     if (ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldy < N || y_rows < 0) return -2;
@@ -666,24 +1064,27 @@ int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w,
     if (act != CHIMERE_ACT_NONE && act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
     if (!float_type(y_type)) return -3;
     if (!out_rows && y_rows < M) return -2;
+    if (x_rows < 0 || x_rows > 0x7FFFFFFF || rows_div <= 0 || (rows ? M > 0 && x_rows == 0 : x_rows < M)) return -2;
     if (M == 0) return 0;
     if (!x || !sx || !w || !sw || (!y && y_rows > 0)) return -1;
-    if (misaligned(x, 16) || misaligned(w, 16) || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4) || misaligned(y, type_size(y_type)) || misaligned(out_rows, 4)) return -5;
+    if (misaligned(x, 16) || misaligned(w, 16) || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4) || misaligned(y, type_size(y_type)) || misaligned(rows, 4) ||
+        misaligned(out_rows, 4)) return -5;
     return 0;
 }
 MatmulCall matmul_call(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, const int32_t* offsets, int E,
-                       int64_t M, int N, int K, int act, void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows, int32_t* status, bool early) {
+                       int64_t M, int N, int K, int act, void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* rows, int rows_div, int64_t x_rows, const int32_t* out_rows,
+                       int32_t* status, bool early) {
     MatmulCall c{};
     c.x = x; c.ldx = ldx; c.w = w; c.ldw = ldw;
     c.dual = act == CHIMERE_ACT_SWIGLU;
     c.w_plane = E > 1 ? w_plane : (c.dual ? 2 : 1) * (int64_t)N * ldw;
     MatmulParams& p = c.p;
-    p.sx = sx; p.sw = sw; p.bias = bias; p.y = y; p.ldy = ldy; p.y_rows = y_rows; p.offsets = offsets; p.out_rows = out_rows; p.status = status;
+    p.sx = sx; p.sw = sw; p.bias = bias; p.y = y; p.ldy = ldy; p.y_rows = y_rows; p.offsets = offsets; p.rows = rows; p.rows_div = rows_div; p.x_rows = (int)x_rows; p.out_rows = out_rows; p.status = status;
     p.M = (int)M; p.N = N; p.K = K; p.E = E; p.y_type = y_type; p.act = act; p.early = early;
     return c;
 }
 inline int up16(int k) { return (k + 15) & ~15; }
-inline int up4(int k) { return (k + 3) & ~3; }
+inline int up8(int k) { return (k + 7) & ~7; }
 inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 inline size_t rows_bytes(int64_t M, int K) { return up256((size_t)M * up16(K)) + up256((size_t)M * 4); }   // int8 rows and their scales
 struct Carver {
@@ -709,19 +1110,20 @@ int chimere_b200_quantize_i8(const void* d_x, int x_type, int64_t ldx, int64_t x
 
 int chimere_b200_matmul_w8a8(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,
                              int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy, int32_t* d_status, cudaStream_t stream) {
-    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
+    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr);
     if (rc || M == 0) return rc;
-    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, false), false, stream);
+    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr, d_status, false), false, stream);
 }
 
 int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, int64_t stride_w, const float* d_w_scale,
                                      const float* d_bias, const int32_t* d_offsets, int E, int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy,
-                                     int64_t y_rows, const int32_t* d_out_rows, int32_t* d_status, cudaStream_t stream) {
-    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_out_rows);
+                                     int64_t y_rows, const int32_t* d_rows, int rows_div, int64_t x_rows, const int32_t* d_out_rows, int32_t* d_status, cudaStream_t stream) {
+    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_rows, rows_div, x_rows, d_out_rows);
     if (rc || M == 0) return rc;
     if (!d_offsets) return -1;
     if (misaligned(d_offsets, 4)) return -5;
-    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, d_offsets, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_out_rows, d_status, false), false, stream);
+    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, d_offsets, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_rows, rows_div,
+                                     x_rows, d_out_rows, d_status, false), false, stream);
 }
 
 size_t chimere_b200_linear_w8a8_bytes(int64_t M, int K) {
@@ -738,18 +1140,18 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
     if (misaligned(d_ws, 256)) return -5;
     int rc = check_quantize(d_x, x_type, ldx, M, nullptr, 1, M, K, q, up16(K), scale);
     if (rc) return rc;
-    rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
+    rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr);
     if (rc || M == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     if (!encoder()) return -6;
     rc = rc_of(launch_quantize(QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, 0}, x_type, M, stream, false));
     if (rc) return rc;
-    return launch_matmul(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, true), true, stream);
+    return launch_matmul(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr, d_status, true), true, stream);
 }
 
 size_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F) {
     if (pairs < 0 || pairs > 0x7FFFFFFF || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return 0;
-    return rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up4(F) * 4) + 256;
+    return rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up8(F) * 4) + 256;
 }
 
 int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
@@ -761,29 +1163,30 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
     if (act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
     const int64_t P = T * top_k;
     Carver ws{(uint8_t*)d_ws, 0};
-    int8_t* q = (int8_t*)ws.take((size_t)P * up16(H));
-    float* scale = (float*)ws.take((size_t)P * 4);
+    int8_t* q = (int8_t*)ws.take((size_t)T * up16(H));
+    float* scale = (float*)ws.take((size_t)T * 4);
     int8_t* hq = (int8_t*)ws.take((size_t)P * up16(F));
     float* h_scale = (float*)ws.take((size_t)P * 4);
-    float* h = (float*)ws.take((size_t)P * up4(F) * 4);
+    float* h = (float*)ws.take((size_t)P * up8(F) * 4);
     if (P > 0 && (!d_ws || !d_perm || !d_offsets)) return -1;
     if (misaligned(d_ws, 256) || misaligned(d_offsets, 4)) return -5;
-    int rc = check_quantize(d_x, x_type, ldx, T, d_perm, top_k, P, H, q, up16(H), scale);
+    int rc = check_quantize(d_x, x_type, ldx, T, nullptr, 1, T, H, q, up16(H), scale);
     if (rc) return rc;
-    rc = check_matmul(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, E, P, F, H, act, h, kF32, up4(F), P, nullptr);
+    rc = check_matmul(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, E, P, F, H, act, h, kF32, up8(F), P, d_perm, top_k, T, nullptr);
     if (rc) return rc;
-    rc = check_matmul(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm);
+    rc = check_matmul(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, nullptr, 1, P, d_perm);
     if (rc || P == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     if (!encoder()) return -6;
-    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, d_perm, top_k, H, q, up16(H), scale, 0}, x_type, P, stream, false));
+    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, nullptr, 1, H, q, up16(H), scale, 0}, x_type, T, stream, false));
     if (rc) return rc;
-    rc = launch_matmul(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up4(F), P, nullptr, d_status, true), true, stream);
+    rc = launch_matmul(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up8(F), P, d_perm, top_k, T, nullptr, d_status, true),
+                       true, stream);
     if (rc) return rc;
-    rc = rc_of(launch_quantize(QuantParams{h, up4(F), P, nullptr, 1, F, hq, up16(F), h_scale, 0}, kF32, P, stream, true));
+    rc = rc_of(launch_quantize(QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, 0}, kF32, P, stream, true));
     if (rc) return rc;
-    return launch_matmul(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm,
-                                     d_status, true), true, stream);
+    return launch_matmul(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, nullptr, 1, P,
+                                     d_perm, d_status, true), true, stream);
 }
 
 }  // extern "C"

@@ -133,7 +133,7 @@ def test_quantize_rows_of_a_wider_matrix_and_gathered(dtype):
 
 # ---- dense ----
 SHAPES = [(1, 1, 1), (1, 2048, 4096), (2, 128, 128), (3, 129, 5), (7, 2688, 3712), (16, 512, 100), (17, 100, 130), (33, 2005, 257), (61, 4096, 2048), (64, 64, 64),
-          (65, 300, 700), (129, 1000, 513), (300, 640, 1000), (777, 2005, 1031), (1500, 384, 2500), (5000, 130, 260), (4000, 2048, 2048)]
+          (65, 300, 700), (129, 1000, 513), (300, 640, 1000), (777, 2005, 1031), (1500, 384, 2500), (5000, 130, 260), (4000, 2048, 2048), (2300, 1000, 1024), (1111, 640, 4099), (20000, 64, 320)]
 
 
 @pytest.mark.parametrize("act", [abi.ACT_NONE, abi.ACT_SWIGLU, abi.ACT_RELU2])
@@ -244,6 +244,25 @@ def test_grouped_rows_to_other_places(M):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("act", [abi.ACT_NONE, abi.ACT_SWIGLU])
+@pytest.mark.parametrize("M,K,N,counts", [(11, 100, 70, [4, 0, 7]), (70, 512, 130, [1, 33, 36]), (900, 700, 300, [500, 3, 397]), (1500, 256, 512, [129, 771, 600])])
+def test_grouped_rows_from_other_places(M, K, N, counts, act):
+    g = gen(M + K)
+    n, E, R = M // 2, len(counts), 2 * N if act == abi.ACT_SWIGLU else N
+    q, w, sx, sw = i8(g, n, K), i8(g, E, R, K), scales(g, n) / K ** 0.5, scales(g, E, R)
+    rows = torch.randint(0, 3 * n, (M,), generator=g, device="cuda", dtype=torch.int32)
+    rows[0], rows[1], rows[2], rows[M - 1] = -1, 3 * n, 2 ** 31 - 1, -2 ** 31       # no such rows
+    off = groups(counts)
+    y = w8a8.matmul_w8a8_grouped(q, sx, w, sw, off, act=act, rows=rows, rows_div=3, out_dtype=torch.bfloat16)
+    there = (rows >= 0) & (rows < 3 * n)
+    src = torch.where(there, rows // 3, 0).long()
+    fq, fs = torch.where(there[:, None], q[src], 0), torch.where(there, sx[src], 0.0)
+    for e in range(E):
+        a, b = int(off[e]), int(off[e + 1])
+        if b > a:
+            check(y[a:b], *product(fq[a:b], fs[a:b], w[e], sw[e], None, act, torch.bfloat16))
+
+
 def test_offsets_that_fall_are_empty_groups():
     g = gen(3)
     q, w, sx, sw = i8(g, 30, 64), i8(g, 4, 48, 64), scales(g, 30), scales(g, 4, 48)
@@ -299,6 +318,8 @@ def test_experts_behind_the_router(cfg, T):
     # the four steps one by one
     q, s = w8a8.quantize_i8(x, perm, k)
     h = w8a8.matmul_w8a8_grouped(q, s, w_up, s_up, off, act=cfg.act)
+    q, s = w8a8.quantize_i8(x)
+    assert torch.equal(h, w8a8.matmul_w8a8_grouped(q, s, w_up, s_up, off, act=cfg.act, rows=perm, rows_div=k))
     hq, hs = w8a8.quantize_i8(h)
     steps = w8a8.matmul_w8a8_grouped(hq, hs, w_dn, s_dn, off, out_rows=perm, out=torch.empty_like(y))
     assert torch.equal(y, steps)
