@@ -20,10 +20,11 @@ namespace chimere {
 namespace {
 
 constexpr int kB_Threads = 256, kB_Warps = kB_Threads / 32;
+constexpr int kB_CtasPerSm = 3;
 constexpr int kB_Group = 32;          // pieces that are added up together, and groups of them
 constexpr int kB_MaxPieces = kB_Group * kB_Group;
-constexpr int kB_MaxCountPieces = 128;
-constexpr int kB_CountIds = 8192;     // ids of a counting CTA, where that gives few enough of them
+constexpr int kB_CountCluster = 8, kB_MaxCountPieces = 16;
+constexpr int kB_CountIds = 4096;     // ids of a counting CTA, where that gives few enough of them
 
 struct BalanceParams {
     const void* logits;
@@ -41,7 +42,7 @@ struct BalanceParams {
     int64_t ldd, stride_ds;
     int vec;                          // rows of logits and gradient can be read and written four values at a time
     int pieces, rows;                 // of a sequence; rows of a piece
-    int count_pieces, count_rows;     // (0: counted here)
+    int count_pieces, count_rows;     // of a sequence, by a cluster each (0: counted here); rows of a CTA
     int32_t* count_part;              // [S][count_pieces][E + 1]
     float* part;                      // [S][pieces][E]
     double* group_part;               // [S][groups][E]
@@ -51,63 +52,98 @@ __host__ __device__ inline int groups_of(int pieces) { return (pieces + kB_Group
 
 __device__ __forceinline__ bool counted(const BalanceParams& p, int64_t row) { return !p.mask || p.mask[row] != 0; }
 
-// Pairs and tokens of rows [r0, r1) of sequence s, added to hist[E] and *n (shared memory).
-__device__ __forceinline__ void count_rows(const BalanceParams& p, int s, int r0, int r1, int* hist, int* n) {
+// Pairs and tokens of rows [r0, r1) of sequence s, added to hist[E] and hist[E + 1] (shared memory).
+__device__ __forceinline__ void count_rows(const BalanceParams& p, int s, int r0, int r1, int* hist) {
     const int64_t base = (int64_t)s * p.L;
-    int mine = 0;
-    if (!p.mask) mine = threadIdx.x == 0 ? r1 - r0 : 0;
-    else for (int r = r0 + threadIdx.x; r < r1; r += kB_Threads) mine += p.mask[base + r] != 0;
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if ((threadIdx.x & 31) == 0 && mine) atomicAdd(n, mine);
-    const int64_t total = (int64_t)(r1 - r0) * p.k;
     const int32_t* ids = p.ids + (base + r0) * p.k;
-    for (int64_t i = threadIdx.x; i < total; i += kB_Threads) {
-        const int e = ids[i];
-        if (e >= 0 && e < p.E && (!p.mask || p.mask[base + r0 + i / p.k])) atomicAdd(hist + e, 1);
+    auto add = [&](int e) { if ((uint32_t)e < (uint32_t)p.E) atomicAdd(hist + e, 1); };
+    if (!p.mask) {
+        if (threadIdx.x == 0) atomicAdd(hist + p.E, r1 - r0);
+        const int total = (r1 - r0) * p.k, head = min(total, (int)(-((uintptr_t)ids >> 2) & 3)), quads = (total - head) >> 2;   // (16-byte boundaries)
+        const int4* ids4 = reinterpret_cast<const int4*>(ids + head);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < quads; i += kB_Threads) {
+            const int4 v = __ldg(ids4 + i);
+            add(v.x); add(v.y); add(v.z); add(v.w);
+        }
+        const int rest = total - 4 * quads;   // in front and behind
+        if ((int)threadIdx.x < rest) add(ids[(int)threadIdx.x < head ? threadIdx.x : threadIdx.x + 4 * quads]);
+    } else {
+        int mine = 0;
+        const int rows = r1 - r0, per = kB_Threads / min(p.k, 8), sub = threadIdx.x / per;   // up to eight threads per row, neighbours on neighbouring rows
+#pragma unroll 2
+        for (int r = threadIdx.x % per; r < rows && sub < min(p.k, 8); r += per) {
+            if (!p.mask[base + r0 + r]) continue;
+            mine += sub == 0;
+            for (int j = sub; j < p.k; j += 8) add(__ldg(ids + (int64_t)r * p.k + j));
+        }
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        if ((threadIdx.x & 31) == 0 && mine) atomicAdd(hist + p.E, mine);
     }
 }
 
-__global__ void __launch_bounds__(kB_Threads) count_kernel(BalanceParams p) {
+// A cluster of eight CTAs counts a piece of a sequence; its counts meet in shared memory.
+__global__ void __cluster_dims__(kB_CountCluster, 1, 1) __launch_bounds__(kB_Threads) count_kernel(BalanceParams p) {
     __shared__ int hist[kMaxExperts + 1];
     griddep_launch();
-    const int s = blockIdx.x / p.count_pieces, c = blockIdx.x % p.count_pieces;
+    const int rank = blockIdx.x % kB_CountCluster, s = blockIdx.x / kB_CountCluster / p.count_pieces, c = blockIdx.x / kB_CountCluster % p.count_pieces;
     for (int e = threadIdx.x; e <= p.E; e += kB_Threads) hist[e] = 0;
-    if (c == 0) {
+    if (c == 0 && rank == 0) {
         const int n = groups_of(p.pieces) + 1;
         for (int i = threadIdx.x; i < n; i += kB_Threads) p.counters[(int64_t)s * n + i] = 0;
     }
     __syncthreads();
-    const int r0 = (int)min((int64_t)c * p.count_rows, (int64_t)p.L), r1 = (int)min((int64_t)r0 + p.count_rows, (int64_t)p.L);
-    count_rows(p, s, r0, r1, hist, hist + p.E);
-    __syncthreads();
-    int32_t* out = p.count_part + (int64_t)blockIdx.x * (p.E + 1);
-    for (int e = threadIdx.x; e <= p.E; e += kB_Threads) out[e] = hist[e];
+    const int64_t at = ((int64_t)c * kB_CountCluster + rank) * p.count_rows;
+    const int r0 = (int)min(at, (int64_t)p.L), r1 = (int)min(at + p.count_rows, (int64_t)p.L);
+    count_rows(p, s, r0, r1, hist);
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    int32_t* out = p.count_part + ((int64_t)s * p.count_pieces + c) * (p.E + 1);
+    for (int e = (int)threadIdx.x * kB_CountCluster + rank; e <= p.E; e += kB_CountCluster * kB_Threads) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kB_CountCluster; ++i) {
+            uint32_t a;
+            int v;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(hist + e)), "r"(i));
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+            n += v;
+        }
+        out[e] = n;
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // (a CTA's counts stay until all have read them)
 }
 
 template <int TYPE> __device__ __forceinline__ float to_float(uint32_t bits) { return TYPE == CHIMERE_TYPE_F16 ? h2f(bits) : __uint_as_float(bits << 16); }
-template <int TYPE>
-__device__ __forceinline__ void load4(const void* base, int64_t at, int n, bool vec, float (&v)[4]) {   // n: values there are (0 .. 4)
-    if (TYPE == CHIMERE_TYPE_F32) {
-        const float* q = reinterpret_cast<const float*>(base) + at;
-        if (vec && n == 4) {
-            const float4 a = __ldcs(reinterpret_cast<const float4*>(q));
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        } else {
+// Four neighbouring logits as they lie in memory; those that are not there are -infinity.
+template <int TYPE> struct Four {
+    uint32_t w[TYPE == CHIMERE_TYPE_F32 ? 4 : 2];
+    __device__ __forceinline__ void load(const void* base, int64_t at, int n, bool vec) {   // n: values there are (0 .. 4)
+        if constexpr (TYPE == CHIMERE_TYPE_F32) {
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(base) + at;
+            if (vec && n == 4) {
+                const uint4 a = __ldcs(reinterpret_cast<const uint4*>(q));
+                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = i < n ? q[i] : __uint_as_float(0xFF800000u);
-        }
-    } else {
-        const uint16_t* q = reinterpret_cast<const uint16_t*>(base) + at;
-        if (vec && n == 4) {
-            const uint2 a = __ldcs(reinterpret_cast<const uint2*>(q));
-            v[0] = to_float<TYPE>(a.x & 0xFFFFu); v[1] = to_float<TYPE>(a.x >> 16);
-            v[2] = to_float<TYPE>(a.y & 0xFFFFu); v[3] = to_float<TYPE>(a.y >> 16);
+                for (int i = 0; i < 4; ++i) w[i] = i < n ? q[i] : 0xFF800000u;
+            }
         } else {
+            constexpr uint32_t kNone = TYPE == CHIMERE_TYPE_F16 ? 0xFC00u : 0xFF80u;
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(base) + at;
+            if (vec && n == 4) {
+                const uint2 a = __ldcs(reinterpret_cast<const uint2*>(q));
+                w[0] = a.x; w[1] = a.y;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = i < n ? to_float<TYPE>(q[i]) : __uint_as_float(0xFF800000u);
+                for (int i = 0; i < 2; ++i) w[i] = (2 * i < n ? q[2 * i] : kNone) | ((2 * i + 1 < n ? q[2 * i + 1] : kNone) << 16);
+            }
         }
     }
-}
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (TYPE == CHIMERE_TYPE_F32) return __uint_as_float(w[i]);
+        else return to_float<TYPE>((w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
+    }
+};
 template <int TYPE> __device__ __forceinline__ uint32_t from_float(float v) {
     return TYPE == CHIMERE_TYPE_F16 ? (uint32_t)__half_as_ushort(__float2half_rn(v)) : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
@@ -173,13 +209,35 @@ __device__ __forceinline__ void finish_sequence(const BalanceParams& p, BalanceS
 
 // A row by LANES lanes, G groups of four values each: lane i owns values 4 (i + LANES g) .. + 3.
 template <int TYPE, int LANES, int G>
-__global__ void __launch_bounds__(kB_Threads) balance_kernel(BalanceParams p) {
+__global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(BalanceParams p) {
     constexpr int kRows = 32 / LANES, kU = G == 2 ? 2 : 4;   // rows of a warp at a time: kRows * kU
     __shared__ BalanceShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / LANES, i4 = 4 * (lane % LANES);
     const int s = blockIdx.x / p.pieces, piece = blockIdx.x % p.pieces;
     const int r0 = (int)min((int64_t)piece * p.rows, (int64_t)p.L), r1 = (int)min((int64_t)r0 + p.rows, (int64_t)p.L);
     const bool stats = p.loss != nullptr, grad = p.d_logits != nullptr;
+
+    // this warp's first rows
+    const int row_first = r0 + warp * (kRows * kU);
+    int there[G];
+#pragma unroll
+    for (int j = 0; j < G; ++j) there[j] = max(0, min(4, p.E - (i4 + 4 * LANES * j)));
+    Four<TYPE> next[kU][G];
+    bool next_on[kU];
+    auto fetch = [&](int row0) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = row0 + u * kRows + sub;
+            next_on[u] = r < r1 && counted(p, (int64_t)s * p.L + r);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int64_t at = (int64_t)s * p.stride_s + (int64_t)(row0 + u * kRows + sub) * p.ld + i4;
+#pragma unroll
+            for (int j = 0; j < G; ++j) next[u][j].load(p.logits, at + 4 * LANES * j, next_on[u] ? there[j] : 0, p.vec);
+        }
+    };
+    fetch(row_first);
 
     // the pairs of the whole sequence
     for (int e = tid; e <= p.E; e += kB_Threads) sh.hist[e] = 0;
@@ -188,13 +246,13 @@ __global__ void __launch_bounds__(kB_Threads) balance_kernel(BalanceParams p) {
         for (int e = tid; e < p.E; e += kB_Threads) sh.hist[e] = p.counts[(int64_t)s * p.E + e];
         if (tid == 0) sh.hist[p.E] = p.tokens[s];
     } else if (p.count_pieces == 0) {
-        count_rows(p, s, 0, p.L, sh.hist, sh.hist + p.E);
+        count_rows(p, s, 0, p.L, sh.hist);
     } else {
         griddep_wait();
         const int32_t* part = p.count_part + (int64_t)s * p.count_pieces * (p.E + 1);
         for (int e = tid; e <= p.E; e += kB_Threads) {
             int c = 0;
-#pragma unroll 8
+#pragma unroll 4
             for (int i = 0; i < p.count_pieces; ++i) c += __ldcg(part + (int64_t)i * (p.E + 1) + e);
             sh.hist[e] = c;
         }
@@ -209,29 +267,25 @@ __global__ void __launch_bounds__(kB_Threads) balance_kernel(BalanceParams p) {
         __syncthreads();
     }
     float g[G][4], acc[G][4];
-    int there[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
         const int e = i4 + 4 * LANES * j;
-        there[j] = max(0, min(4, p.E - e));
 #pragma unroll
         for (int i = 0; i < 4; ++i) { acc[j][i] = 0.0f; g[j][i] = grad && e + i < p.E ? sh.g[e + i] : 0.0f; }
     }
 
-    for (int row0 = r0 + warp * (kRows * kU); row0 < r1; row0 += kB_Warps * kRows * kU) {
+    for (int row0 = row_first; row0 < r1; row0 += kB_Warps * kRows * kU) {
         float v[kU][G][4];
         bool on[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int r = row0 + u * kRows + sub;
-            on[u] = r < r1 && counted(p, (int64_t)s * p.L + r);
-        }
+            on[u] = next_on[u];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int64_t at = (int64_t)s * p.stride_s + (int64_t)(row0 + u * kRows + sub) * p.ld + i4;
+            for (int j = 0; j < G; ++j)
 #pragma unroll
-            for (int j = 0; j < G; ++j) load4<TYPE>(p.logits, at + 4 * LANES * j, on[u] ? there[j] : 0, p.vec, v[u][j]);
+                for (int i = 0; i < 4; ++i) v[u][j][i] = next[u][j].value(i);
         }
+        fetch(row0 + kB_Warps * kRows * kU);   // (the rows after these are on their way while these are worked on)
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int r = row0 + u * kRows + sub;
@@ -365,7 +419,7 @@ cudaError_t launch_balance(const BalanceParams& p, int type, bool pdl, cudaStrea
 }
 
 // Pieces of a sequence: as many CTAs as run at once, and at least kB_PieceRows rows in each; counting CTAs likewise.
-constexpr int kB_PieceRows = 64, kB_CtasPerSm = 3;
+constexpr int kB_PieceRows = 32;
 struct Plan { int pieces, rows, count_pieces, count_rows; };
 Plan plan_of(int64_t S, int L, int k, bool stats) {
     Plan r{};
@@ -377,10 +431,10 @@ Plan plan_of(int64_t S, int L, int k, bool stats) {
     r.pieces = r.rows > 0 ? (int)(((int64_t)L + r.rows - 1) / r.rows) : 1;
     if (r.pieces < 1) r.pieces = 1;
     if (stats && r.pieces > 1) {
-        int64_t c = ((int64_t)L * k + kB_CountIds - 1) / kB_CountIds;
+        int64_t c = ((int64_t)L * k + kB_CountCluster * kB_CountIds - 1) / (kB_CountCluster * kB_CountIds);
         c = c > kB_MaxCountPieces ? kB_MaxCountPieces : c;
-        r.count_rows = (int)((L + c - 1) / c);
-        r.count_pieces = (int)(((int64_t)L + r.count_rows - 1) / r.count_rows);
+        r.count_pieces = (int)c;
+        r.count_rows = (int)((L + c * kB_CountCluster - 1) / (c * kB_CountCluster));
     }
     return r;
 }
@@ -401,7 +455,7 @@ inline bool misaligned(const void* p, int to) { return ((uintptr_t)p & (uintptr_
 inline int rc_of(cudaError_t e) { return e == cudaSuccess ? 0 : -(100 + (int)e); }
 
 int check_dims(int64_t S, int64_t L, int E, int k, int mode, int type, int64_t ld, int64_t stride_s) {
-    if (S < 0 || L < 0 || S > 0x7FFFFFFF / kB_MaxPieces || L > 0x7FFFFF00 || E <= 0 || E > kMaxExperts || k <= 0 || k > kMaxExperts) return -2;
+    if (S < 0 || L < 0 || S > 0x7FFFFFFF / (kB_MaxPieces * kB_CountCluster) || L > 0x7FFFFF00 || E <= 0 || E > kMaxExperts || k <= 0 || k > kMaxExperts) return -2;
     if (L > 0 && S > 0x7FFFFFFF / L) return -2;      // (counts and token numbers are 32-bit)
     if (L > 0 && k > 0x7FFFFFFF / L) return -2;
     if (mode != CHIMERE_ROUTE_SOFTMAX_RENORM && mode != CHIMERE_ROUTE_SIGMOID_NORM_SCALE) return -2;
@@ -450,7 +504,7 @@ int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_
     p.pieces = plan.pieces; p.rows = plan.rows; p.count_pieces = plan.count_pieces; p.count_rows = plan.count_rows;
     p.count_part = (int32_t*)(ws + a.count_part); p.part = (float*)(ws + a.part); p.group_part = (double*)(ws + a.group_part); p.counters = (int32_t*)(ws + a.counters);
     if (p.count_pieces) {
-        count_kernel<<<(unsigned)(S * p.count_pieces), kB_Threads, 0, stream>>>(p);
+        count_kernel<<<(unsigned)(S * p.count_pieces * kB_CountCluster), kB_Threads, 0, stream>>>(p);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return rc_of(e);
     }

@@ -8,6 +8,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -19,10 +21,9 @@ constexpr int kMaxGroups = 1024;
 constexpr int kMaxK = 131071;
 
 // ------------------------------------------------------------------ rows -> int8 ----
-// One CTA per row: a thread holds up to kQ_Vecs pieces of eight values in registers between the maximum and the division, so a row of up
-// to blockDim * 32 values is read once; what lies behind is read again (from L2).  Bound: memory.
-constexpr int kQ_Vecs = 4;
-
+// A row by GROUP threads, which keep it as it came (16 bytes of kQ_Vecs pieces each) between the maximum and the division, so that it is read
+// once; what a row has beyond that is read again, from L2.  Bound: memory, so what counts is how many rows are on their way at a time: one warp
+// per row where rows are short and many (no barrier, nothing waits for another row), a CTA per row else.
 struct QuantParams {
     const void* x;
     int64_t ldx;
@@ -33,65 +34,65 @@ struct QuantParams {
     int8_t* q;
     int64_t ldq;
     float* scale;
+    int64_t M;
     int vec;               // x rows start on 16-byte boundaries
 };
 
-template <int TYPE> struct Elem;
-template <> struct Elem<kF32> {
-    using T = float;
-    __device__ static __forceinline__ float f(T v) { return v; }
-    __device__ static __forceinline__ void load8(const T* p, float (&v)[8]) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    }
-};
-template <> struct Elem<kF16> {
-    using T = __half;
-    __device__ static __forceinline__ float f(T v) { return __half2float(v); }
-    __device__ static __forceinline__ void load8(const T* p, float (&v)[8]) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+template <int TYPE> struct Elem {   // eight values as they lie in memory
+    static constexpr int kWords = TYPE == kF32 ? 8 : 4;
+    using T = typename std::conditional<TYPE == kF32, float, uint16_t>::type;
+    struct Raw { uint32_t w[kWords]; };
+    __device__ static __forceinline__ Raw load8(const T* p) {
+        Raw r;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { v[2 * i] = h2f(w[i] & 0xFFFFu); v[2 * i + 1] = h2f(w[i] >> 16); }
+        for (int i = 0; i < kWords / 4; ++i) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            r.w[4 * i] = a.x; r.w[4 * i + 1] = a.y; r.w[4 * i + 2] = a.z; r.w[4 * i + 3] = a.w;
+        }
+        return r;
     }
-};
-template <> struct Elem<kBF16> {
-    using T = __nv_bfloat16;
-    __device__ static __forceinline__ float f(T v) { return __bfloat162float(v); }
-    __device__ static __forceinline__ void load8(const T* p, float (&v)[8]) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    __device__ static __forceinline__ float of(uint32_t bits) { return TYPE == kF16 ? h2f(bits) : __uint_as_float(bits << 16); }
+    __device__ static __forceinline__ float value(const Raw& r, int i) {
+        if (TYPE == kF32) return __uint_as_float(r.w[i % kWords]);
+        if (TYPE == kBF16 && (i & 1)) return __uint_as_float(r.w[i / 2] & 0xFFFF0000u);
+        return of((r.w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
+    }
+    __device__ static __forceinline__ float one(const T* p) {
+        if constexpr (TYPE == kF32) return *p;
+        else return of(*p);
+    }
+    // bits of the largest magnitude: patterns of non-negative floats order like the values, with the NaNs above infinity
+    __device__ static __forceinline__ uint32_t top(const Raw& r, uint32_t m) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(value(r, i)) & 0x7FFFFFFFu);
+        return m;
     }
 };
 
-// The two quotients.  In the wide range of magnitudes both come correctly rounded from a reciprocal (div_by_recip), elsewhere from the
+// The two quotients.  In the wide range of magnitudes both come correctly rounded from a reciprocal (div_by_recip), in rows outside it from the
 // division operator; a scale below the normal numbers would make the quotients coarse, so it stays at 2^-126.
+// Nearest integer, ties to even: the sum with 1.5 * 2^23 holds it in its low byte (|x / scale| <= 127.5).
 struct RowScale {
     float scale, recip;
-    bool plain;
+    __device__ __forceinline__ static bool wide(float amax) { return amax > 1e-25f && amax < 1e25f; }
     __device__ __forceinline__ explicit RowScale(float amax) {
-        plain = !(amax > 1e-25f && amax < 1e25f);
-        scale = amax == 0.0f ? 0.0f : fmaxf(plain ? amax / 127.0f : div_by_recip(amax, 127.0f, 1.0f / 127.0f), 1.17549435e-38f);
+        scale = div_by_recip(amax, 127.0f, 1.0f / 127.0f);
         recip = __frcp_rn(scale);
     }
-    // nearest integer, ties to even: the sum with 1.5 * 2^23 holds it in its low byte (|x / scale| <= 127.5)
-    __device__ __forceinline__ uint32_t q(float x) const {
-        const float v = plain ? (scale == 0.0f ? 0.0f : x / scale) : div_by_recip(x, scale, recip);
-        return __float_as_uint(__fadd_rn(v, 12582912.0f)) & 0xFFu;
-    }
+    __device__ __forceinline__ uint32_t q(float x) const { return __float_as_uint(__fadd_rn(div_by_recip(x, scale, recip), 12582912.0f)); }
+    __device__ __forceinline__ uint32_t q4(float a, float b, float c, float d) const { return prmt(prmt(q(a), q(b), 0x0040u), prmt(q(c), q(d), 0x0040u), 0x5410u); }
 };
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a | (b << 8) | (c << 16) | (d << 24); }
 
-template <int TYPE>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(QuantParams p) {
+// GROUP 32: a warp per row, eight rows per CTA; GROUP 0: a CTA per row
+template <int TYPE, int GROUP, int VECS>
+__global__ void __launch_bounds__(GROUP ? 256 : 1024) quantize_rows_kernel(QuantParams p) {
     using E = Elem<TYPE>;
     __shared__ uint32_t s_max[32];
-    const int tid = threadIdx.x, nt = blockDim.x;
+    const int tid = GROUP ? threadIdx.x % 32 : threadIdx.x, nt = GROUP ? 32 : blockDim.x;
     griddep_wait();          // (in front of the next kernel's start: what lies before this kernel is then complete for that one too)
     griddep_launch();
-    const int64_t row = blockIdx.x;
+    const int64_t row = GROUP ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
+    if (GROUP && row >= p.M) return;
     int64_t src = row;
     if (p.rows) {
         const int32_t r = p.rows[row];
@@ -105,28 +106,18 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(QuantParams p) {
     }
     const typename E::T* x = reinterpret_cast<const typename E::T*>(p.x) + src * p.ldx;
     const int nv = p.vec ? p.K >> 3 : 0;
-    float v[kQ_Vecs][8];
+    typename E::Raw v[VECS];
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < kQ_Vecs; ++i)
-        if (tid + i * nt < nv) {
-            E::load8(x + 8 * (tid + i * nt), v[i]);
-        }
+    for (int i = 0; i < VECS; ++i)
+        if (tid + i * nt < nv) v[i] = E::load8(x + 8 * (tid + i * nt));
 #pragma unroll
-    for (int i = 0; i < kQ_Vecs; ++i)
-        if (tid + i * nt < nv) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(v[i][j])));   // (a NaN's bits lie above infinity's)
-        }
-    for (int i = tid + kQ_Vecs * nt; i < nv; i += nt) {
-        float w[8];
-        E::load8(x + 8 * i, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(w[j])));
-    }
-    for (int i = 8 * nv + tid; i < p.K; i += nt) m = max(m, __float_as_uint(fabsf(E::f(x[i]))));
+    for (int i = 0; i < VECS; ++i)
+        if (tid + i * nt < nv) m = E::top(v[i], m);
+    for (int i = tid + VECS * nt; i < nv; i += nt) m = E::top(E::load8(x + 8 * i), m);
+    for (int i = 8 * nv + tid; i < p.K; i += nt) m = max(m, __float_as_uint(E::one(x + i)) & 0x7FFFFFFFu);
     m = __reduce_max_sync(0xffffffffu, m);
-    if (nt > 32) {
+    if (!GROUP && nt > 32) {
         if ((tid & 31) == 0) s_max[tid >> 5] = m;
         __syncthreads();
         m = __reduce_max_sync(0xffffffffu, (tid & 31) < (nt >> 5) ? s_max[tid & 31] : 0u);
@@ -136,38 +127,53 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(QuantParams p) {
         if (tid == 0) p.scale[row] = __uint_as_float(0x7FC00000u);
         return;
     }
-    const RowScale s(__uint_as_float(m));
+    const float amax = __uint_as_float(m);
+    if (!RowScale::wide(amax)) {
+        const float scale = amax == 0.0f ? 0.0f : fmaxf(amax / 127.0f, 1.17549435e-38f);
+#pragma unroll 1
+        for (int i = tid; i < p.K; i += nt) q[i] = (int8_t)(scale == 0.0f ? 0 : __float2int_rn(E::one(x + i) / scale));
+        if (tid == 0) p.scale[row] = scale;
+        return;
+    }
+    const RowScale s(amax);
     if (tid == 0) p.scale[row] = s.scale;
-    auto put = [&](int i, const float (&w)[8]) {
+    auto put = [&](int i, const typename E::Raw& w) {
         uint2 o;
-        o.x = pack4(s.q(w[0]), s.q(w[1]), s.q(w[2]), s.q(w[3]));
-        o.y = pack4(s.q(w[4]), s.q(w[5]), s.q(w[6]), s.q(w[7]));
+        o.x = s.q4(E::value(w, 0), E::value(w, 1), E::value(w, 2), E::value(w, 3));
+        o.y = s.q4(E::value(w, 4), E::value(w, 5), E::value(w, 6), E::value(w, 7));
         *reinterpret_cast<uint2*>(q + 8 * i) = o;
     };
 #pragma unroll
-    for (int i = 0; i < kQ_Vecs; ++i)
+    for (int i = 0; i < VECS; ++i)
         if (tid + i * nt < nv) put(tid + i * nt, v[i]);
-    for (int i = tid + kQ_Vecs * nt; i < nv; i += nt) {
-        float w[8];
-        E::load8(x + 8 * i, w);
-        put(i, w);
-    }
-    for (int i = 8 * nv + tid; i < p.K; i += nt) q[i] = (int8_t)s.q(E::f(x[i]));
+    for (int i = tid + VECS * nt; i < nv; i += nt) put(i, E::load8(x + 8 * i));
+    for (int i = 8 * nv + tid; i < p.K; i += nt) q[i] = (int8_t)s.q(E::one(x + i));
 }
 
-cudaError_t launch_quantize(QuantParams p, int type, int64_t M, cudaStream_t stream, bool pdl) {
-    const int size = type == kF32 ? 4 : 2;
-    p.vec = ((uintptr_t)p.x & 15) == 0 && (p.ldx * size) % 16 == 0;
+template <int TYPE>
+cudaError_t launch_quantize_type(const QuantParams& p, cudaStream_t stream, bool pdl) {
+    auto go = [&](auto kernel, int64_t grid, int nt) -> cudaError_t {
+        if (pdl) return launch_pdl(kernel, dim3((unsigned)grid), nt, 0, stream, p);
+        kernel<<<(unsigned)grid, nt, 0, stream>>>(p);
+        return cudaGetLastError();
+    };
+    // A warp holds 512 bytes of a row per register piece (four registers); sixteen of them at most, and enough rows for every SM's warps.
+    const int pieces = (p.K / 8 * (TYPE == kF32 ? 2 : 1) + 31) / 32;
+    if (p.vec && pieces <= 16 && p.M >= 148 * 8) {
+        constexpr int k = TYPE == kF32 ? 2 : 1;
+        const int64_t grid = (p.M + 7) / 8;
+        if (pieces <= 4) return go(quantize_rows_kernel<TYPE, 32, 4 / k>, grid, 256);
+        if (pieces <= 8) return go(quantize_rows_kernel<TYPE, 32, 8 / k>, grid, 256);
+        return go(quantize_rows_kernel<TYPE, 32, 16 / k>, grid, 256);
+    }
     // two pieces of eight values per thread, at least a warp
     int nt = (p.K + 15) / 16;
     nt = nt > 1024 ? 1024 : (nt + 31) / 32 * 32;
-    const dim3 grid((unsigned)M);
-    auto go = [&](auto kernel) -> cudaError_t {
-        if (pdl) return launch_pdl(kernel, grid, nt, 0, stream, p);
-        kernel<<<grid, nt, 0, stream>>>(p);
-        return cudaGetLastError();
-    };
-    return type == kF32 ? go(quantize_rows_kernel<kF32>) : type == kF16 ? go(quantize_rows_kernel<kF16>) : go(quantize_rows_kernel<kBF16>);
+    return go(quantize_rows_kernel<TYPE, 0, 2>, p.M, nt);
+}
+cudaError_t launch_quantize(QuantParams p, int type, cudaStream_t stream, bool pdl) {
+    p.vec = ((uintptr_t)p.x & 15) == 0 && (p.ldx * (type == kF32 ? 4 : 2)) % 16 == 0;
+    return type == kF32 ? launch_quantize_type<kF32>(p, stream, pdl) : type == kF16 ? launch_quantize_type<kF16>(p, stream, pdl) : launch_quantize_type<kBF16>(p, stream, pdl);
 }
 
 // ------------------------------------------------------------------ product ----
@@ -1105,7 +1111,7 @@ int chimere_b200_quantize_i8(const void* d_x, int x_type, int64_t ldx, int64_t x
                              int8_t* d_q, int64_t ldq, float* d_scale, cudaStream_t stream) {
     const int rc = check_quantize(d_x, x_type, ldx, x_rows, d_rows, rows_div, M, K, d_q, ldq, d_scale);
     if (rc || M == 0) return rc;
-    return rc_of(launch_quantize(QuantParams{d_x, ldx, x_rows, d_rows, rows_div, K, d_q, ldq, d_scale, 0}, x_type, M, stream, false));
+    return rc_of(launch_quantize(QuantParams{d_x, ldx, x_rows, d_rows, rows_div, K, d_q, ldq, d_scale, M, 0}, x_type, stream, false));
 }
 
 int chimere_b200_matmul_w8a8(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,
@@ -1144,7 +1150,7 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
     if (rc || M == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     if (!encoder()) return -6;
-    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, 0}, x_type, M, stream, false));
+    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, stream, false));
     if (rc) return rc;
     return launch_matmul(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr, d_status, true), true, stream);
 }
@@ -1178,12 +1184,12 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
     if (rc || P == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     if (!encoder()) return -6;
-    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, nullptr, 1, H, q, up16(H), scale, 0}, x_type, T, stream, false));
+    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, nullptr, 1, H, q, up16(H), scale, T, 0}, x_type, stream, false));
     if (rc) return rc;
     rc = launch_matmul(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up8(F), P, d_perm, top_k, T, nullptr, d_status, true),
                        true, stream);
     if (rc) return rc;
-    rc = rc_of(launch_quantize(QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, 0}, kF32, P, stream, true));
+    rc = rc_of(launch_quantize(QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, P, 0}, kF32, stream, true));
     if (rc) return rc;
     return launch_matmul(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, nullptr, 1, P,
                                      d_perm, d_status, true), true, stream);

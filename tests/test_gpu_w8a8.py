@@ -72,7 +72,8 @@ def check(y, ref, bound):
 
 # ---- rows ----
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,K", [(1, 1), (3, 7), (2, 8), (5, 2005), (4, 2048), (33, 96), (2, 40000), (1, 131071)])
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 7), (2, 8), (5, 2005), (4, 2048), (33, 96), (2, 40000), (1, 131071), (1200, 512), (1201, 1000), (1500, 2048), (1300, 4096), (1184, 2056),
+                                 (1190, 5), (1190, 4100)])
 def test_quantize_rows(M, K, dtype):
     x = (torch.randn(M, K, generator=gen(M * K), device="cuda") * 3).to(dtype)
     q, s = w8a8.quantize_i8(x)
