@@ -5,10 +5,11 @@
 //   f_e = number of ids equal to e,  P_e = sum of p_te,   loss = coef * E / (k n^2) * sum_e f_e P_e      (even load: coef)
 //   d l_te = d_loss * coef * E / (k n^2) * p_te * (f_e - sum_j f_j p_tj)  [ * (1 - sigmoid(l_te)) ]
 // The counts need the ids alone, which are a few percent of the bytes; with them known one pass over the logits gives both the sums
-// and the gradient, so every logit is read once and every gradient written once.  Bound: memory.
-//   count_kernel   pairs per expert of a piece of a sequence (integers; any order gives the same)
-//   balance_kernel a piece of a sequence per CTA, a row by 8, 16 or 32 lanes; sums of a piece in fp32, of the pieces in fp64 and always in
-//                  the same order, by the CTAs that finish last.  A sequence in one piece counts its pairs here as well: one launch.
+// and the gradient, so every logit is read once and every gradient written once.  Bound: memory in large batches, launches and latency in small ones.
+//   balance_kernel a piece of a sequence per CTA, a row by 8, 16 or 32 lanes; sums of a piece in fp32, of the pieces in fp64 and always in the same
+//                  order.  Short sequences, and many of them: the pieces of a sequence are a cluster of up to eight CTAs, which count its pairs and add up its sums over
+//                  shared memory, one launch in all.  A few long sequences: dozens of pieces each, whose sums the CTAs that finish last add up, behind
+//   count_kernel   pairs per expert of a piece of a sequence.
 // In the gradient f_e is replaced by f_e - (sum_j f_j) / E, a constant less: it drops out (the p of a row add up to 1), and the difference
 // that remains does not lose the digits of the load all experts share.
 #include <cuda_bf16.h>
@@ -22,7 +23,6 @@ namespace {
 constexpr int kB_Threads = 256, kB_Warps = kB_Threads / 32;
 constexpr int kB_CtasPerSm = 3;
 constexpr int kB_Group = 32;          // pieces that are added up together, and groups of them
-constexpr int kB_MaxPieces = kB_Group * kB_Group;
 constexpr int kB_CountCluster = 8, kB_MaxCountPieces = 16;
 constexpr int kB_CountIds = 4096;     // ids of a counting CTA, where that gives few enough of them
 
@@ -41,7 +41,7 @@ struct BalanceParams {
     void* d_logits;                   // or null
     int64_t ldd, stride_ds;
     int vec;                          // rows of logits and gradient can be read and written four values at a time
-    int pieces, rows;                 // of a sequence; rows of a piece
+    int pieces, rows;                 // of a sequence (count_pieces = 0: the CTAs of a cluster); rows of a piece
     int count_pieces, count_rows;     // of a sequence, by a cluster each (0: counted here); rows of a CTA
     int32_t* count_part;              // [S][count_pieces][E + 1]
     float* part;                      // [S][pieces][E]
@@ -73,13 +73,27 @@ __device__ __forceinline__ void count_rows(const BalanceParams& p, int s, int r0
         const int rows = r1 - r0, per = kB_Threads / min(p.k, 8), sub = threadIdx.x / per;   // up to eight threads per row, neighbours on neighbouring rows
 #pragma unroll 2
         for (int r = threadIdx.x % per; r < rows && sub < min(p.k, 8); r += per) {
-            if (!p.mask[base + r0 + r]) continue;
-            mine += sub == 0;
-            for (int j = sub; j < p.k; j += 8) add(__ldg(ids + (int64_t)r * p.k + j));
+            const bool on = p.mask[base + r0 + r] != 0;
+            mine += on && sub == 0;
+            for (int j = sub; j < p.k; j += 8) {
+                const int e = __ldg(ids + (int64_t)r * p.k + j);   // (on its way together with the mask)
+                if (on) add(e);
+            }
         }
         mine = __reduce_add_sync(0xffffffffu, mine);
         if ((threadIdx.x & 31) == 0 && mine) atomicAdd(hist + p.E, mine);
     }
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int ld_peer(const int* mine, int rank) {   // the value at this place in another CTA of the cluster
+    uint32_t a;
+    int v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
 }
 
 // A cluster of eight CTAs counts a piece of a sequence; its counts meet in shared memory.
@@ -96,88 +110,132 @@ __global__ void __cluster_dims__(kB_CountCluster, 1, 1) __launch_bounds__(kB_Thr
     const int64_t at = ((int64_t)c * kB_CountCluster + rank) * p.count_rows;
     const int r0 = (int)min(at, (int64_t)p.L), r1 = (int)min(at + p.count_rows, (int64_t)p.L);
     count_rows(p, s, r0, r1, hist);
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_barrier();
     int32_t* out = p.count_part + ((int64_t)s * p.count_pieces + c) * (p.E + 1);
     for (int e = (int)threadIdx.x * kB_CountCluster + rank; e <= p.E; e += kB_CountCluster * kB_Threads) {
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < kB_CountCluster; ++i) {
-            uint32_t a;
-            int v;
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(hist + e)), "r"(i));
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-            n += v;
-        }
+        for (int i = 0; i < kB_CountCluster; ++i) n += ld_peer(hist + e, i);
         out[e] = n;
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // (a CTA's counts stay until all have read them)
+    cluster_barrier();   // (a CTA's counts stay until all have read them)
 }
 
 template <int TYPE> __device__ __forceinline__ float to_float(uint32_t bits) { return TYPE == CHIMERE_TYPE_F16 ? h2f(bits) : __uint_as_float(bits << 16); }
-// Four neighbouring logits as they lie in memory; those that are not there are -infinity.
+// Four neighbouring logits as they lie in memory; those that are not there are -infinity.  n: values there are (FULL: 0 or 4, else 0 .. 4).
 template <int TYPE> struct Four {
-    uint32_t w[TYPE == CHIMERE_TYPE_F32 ? 4 : 2];
-    __device__ __forceinline__ void load(const void* base, int64_t at, int n, bool vec) {   // n: values there are (0 .. 4)
-        if constexpr (TYPE == CHIMERE_TYPE_F32) {
-            const uint32_t* q = reinterpret_cast<const uint32_t*>(base) + at;
-            if (vec && n == 4) {
-                const uint4 a = __ldcs(reinterpret_cast<const uint4*>(q));
-                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-            } else {
+    static constexpr int kWords = TYPE == CHIMERE_TYPE_F32 ? 4 : 2;
+    static constexpr uint32_t kNone = TYPE == CHIMERE_TYPE_F32 ? 0xFF800000u : TYPE == CHIMERE_TYPE_F16 ? 0xFC00FC00u : 0xFF80FF80u;
+    uint32_t w[kWords];
+    template <bool FULL>
+    __device__ __forceinline__ void load(const void* base, int64_t at, int n, bool vec) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(base) + at * kWords);
+        if (FULL || (vec && n == 4)) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = i < n ? q[i] : 0xFF800000u;
+            for (int i = 0; i < kWords; ++i) w[i] = kNone;
+            if (n) {
+                if constexpr (TYPE == CHIMERE_TYPE_F32) {
+                    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(q));
+                    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+                } else {
+                    const uint2 a = __ldcs(reinterpret_cast<const uint2*>(q));
+                    w[0] = a.x; w[1] = a.y;
+                }
             }
+        } else if constexpr (TYPE == CHIMERE_TYPE_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = i < n ? q[i] : kNone;
         } else {
-            constexpr uint32_t kNone = TYPE == CHIMERE_TYPE_F16 ? 0xFC00u : 0xFF80u;
-            const uint16_t* q = reinterpret_cast<const uint16_t*>(base) + at;
-            if (vec && n == 4) {
-                const uint2 a = __ldcs(reinterpret_cast<const uint2*>(q));
-                w[0] = a.x; w[1] = a.y;
-            } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(q);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) w[i] = (2 * i < n ? q[2 * i] : kNone) | ((2 * i + 1 < n ? q[2 * i + 1] : kNone) << 16);
-            }
+            for (int i = 0; i < 2; ++i) w[i] = (2 * i < n ? h[2 * i] : kNone & 0xFFFFu) | ((2 * i + 1 < n ? h[2 * i + 1] : kNone & 0xFFFFu) << 16);
         }
     }
     __device__ __forceinline__ float value(int i) const {
         if constexpr (TYPE == CHIMERE_TYPE_F32) return __uint_as_float(w[i]);
+        else if (TYPE == CHIMERE_TYPE_BF16 && (i & 1)) return __uint_as_float(w[i / 2] & 0xFFFF0000u);
         else return to_float<TYPE>((w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
     }
 };
-template <int TYPE> __device__ __forceinline__ uint32_t from_float(float v) {
-    return TYPE == CHIMERE_TYPE_F16 ? (uint32_t)__half_as_ushort(__float2half_rn(v)) : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v));
+template <int TYPE> __device__ __forceinline__ uint32_t two(float a, float b) {
+    if (TYPE == CHIMERE_TYPE_F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <int TYPE>
+template <int TYPE, bool FULL>
 __device__ __forceinline__ void store4(void* base, int64_t at, int n, bool vec, const float (&v)[4]) {
-    if (TYPE == CHIMERE_TYPE_F32) {
+    if constexpr (TYPE == CHIMERE_TYPE_F32) {
         float* q = reinterpret_cast<float*>(base) + at;
-        if (vec && n == 4) __stcs(reinterpret_cast<float4*>(q), make_float4(v[0], v[1], v[2], v[3]));
-        else {
+        if (FULL || (vec && n == 4)) {
+            if (n) __stcs(reinterpret_cast<float4*>(q), make_float4(v[0], v[1], v[2], v[3]));
+        } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) if (i < n) q[i] = v[i];
         }
     } else {
         uint16_t* q = reinterpret_cast<uint16_t*>(base) + at;
-        if (vec && n == 4) __stcs(reinterpret_cast<uint2*>(q), make_uint2(from_float<TYPE>(v[0]) | (from_float<TYPE>(v[1]) << 16), from_float<TYPE>(v[2]) | (from_float<TYPE>(v[3]) << 16)));
-        else {
+        const uint2 w = make_uint2(two<TYPE>(v[0], v[1]), two<TYPE>(v[2], v[3]));
+        if (FULL || (vec && n == 4)) {
+            if (n) __stcs(reinterpret_cast<uint2*>(q), w);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) if (i < n) q[i] = (uint16_t)from_float<TYPE>(v[i]);
+            for (int i = 0; i < 4; ++i) if (i < n) q[i] = (uint16_t)((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
         }
     }
 }
-template <int LANES> __device__ __forceinline__ float lanes_max(float v) {
+// over the LANES lanes of a row, several rows at a time
+template <int LANES, int N> __device__ __forceinline__ void lanes_max(float (&v)[N]) {
+    if constexpr (LANES == 32) {
 #pragma unroll
-    for (int d = LANES / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-    return v;
+        for (int u = 0; u < N; ++u) asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v[u]));   // (passes over NaNs, as fmaxf does)
+    } else {
+#pragma unroll
+        for (int d = LANES / 2; d > 0; d >>= 1)
+#pragma unroll
+            for (int u = 0; u < N; ++u) v[u] = fmaxf(v[u], __shfl_xor_sync(0xffffffffu, v[u], d));
+    }
 }
-template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
+template <int LANES, int N> __device__ __forceinline__ void lanes_sum(float (&v)[N]) {
 #pragma unroll
-    for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
+    for (int d = LANES / 2; d > 0; d >>= 1) {
+        float o[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) o[u] = __shfl_xor_sync(0xffffffffu, v[u], d);
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] += o[u];
+    }
+}
+__device__ __forceinline__ float rcp(float v) {   // (off by one step at most)
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// exp of two values that are not positive: 2^h times 1 + r with h = x log2(e) rounded and r = x - h ln(2) what the rounding left out (ln(2) in two
+// parts).  Below -150 it is 0 (a NaN stays one); off by the two steps of ex2 and half a step of the last product.
+__device__ __forceinline__ uint64_t exp_pair(uint64_t x) {
+    float a, b;
+    unpack2(x, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-150.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-150.0f));
+    x = pack2f(a, b);
+    const uint64_t h = mul2(x, pack2f(1.44269504f, 1.44269504f));
+    uint64_t r = fma2(h, pack2f(-0.693147182f, -0.693147182f), x);
+    r = fma2(h, pack2f(1.90465421e-9f, 1.90465421e-9f), r);
+    unpack2(h, a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    const uint64_t e = pack2f(a, b);
+    return fma2(e, r, e);
 }
 
 struct BalanceShared {
-    int hist[kMaxExperts + 1];        // [E]: tokens
+    int hist[kMaxExperts + 1];        // of the whole sequence; [E]: tokens
+    int mine[kMaxExperts + 1];        // of this CTA's rows (cluster)
+    float sums[kMaxExperts];          // ... and their probabilities
     float g[kMaxExperts];
     float part[kB_Warps][kMaxExperts];
     double sum[kB_Warps];
@@ -208,7 +266,8 @@ __device__ __forceinline__ void finish_sequence(const BalanceParams& p, BalanceS
 }
 
 // A row by LANES lanes, G groups of four values each: lane i owns values 4 (i + LANES g) .. + 3.
-template <int TYPE, int LANES, int G>
+// FULL: as many logits as the lanes hold, rows that are read and written four values at a time: no lane looks at what it has.
+template <int TYPE, int LANES, int G, bool SIGMOID, bool FULL>
 __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(BalanceParams p) {
     constexpr int kRows = 32 / LANES, kU = G == 2 ? 2 : 4;   // rows of a warp at a time: kRows * kU
     __shared__ BalanceShared sh;
@@ -221,32 +280,38 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
     const int row_first = r0 + warp * (kRows * kU);
     int there[G];
 #pragma unroll
-    for (int j = 0; j < G; ++j) there[j] = max(0, min(4, p.E - (i4 + 4 * LANES * j)));
+    for (int j = 0; j < G; ++j) there[j] = FULL ? 4 : max(0, min(4, p.E - (i4 + 4 * LANES * j)));
     Four<TYPE> next[kU][G];
-    bool next_on[kU];
+    // (a row that is not there, or that the mask leaves out, is one of -infinities: no probabilities, no gradient)
     auto fetch = [&](int row0) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int r = row0 + u * kRows + sub;
-            next_on[u] = r < r1 && counted(p, (int64_t)s * p.L + r);
-        }
+            const bool on = r < r1 && counted(p, (int64_t)s * p.L + r);
+            const int64_t at = (int64_t)s * p.stride_s + (int64_t)r * p.ld + i4;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int64_t at = (int64_t)s * p.stride_s + (int64_t)(row0 + u * kRows + sub) * p.ld + i4;
-#pragma unroll
-            for (int j = 0; j < G; ++j) next[u][j].load(p.logits, at + 4 * LANES * j, next_on[u] ? there[j] : 0, p.vec);
+            for (int j = 0; j < G; ++j) next[u][j].template load<FULL>(p.logits, at + 4 * LANES * j, on ? there[j] : 0, p.vec);
         }
     };
     fetch(row_first);
 
     // the pairs of the whole sequence
-    for (int e = tid; e <= p.E; e += kB_Threads) sh.hist[e] = 0;
-    __syncthreads();
     if (!p.ids) {
         for (int e = tid; e < p.E; e += kB_Threads) sh.hist[e] = p.counts[(int64_t)s * p.E + e];
         if (tid == 0) sh.hist[p.E] = p.tokens[s];
     } else if (p.count_pieces == 0) {
-        count_rows(p, s, 0, p.L, sh.hist);
+        int* mine = p.pieces == 1 ? sh.hist : sh.mine;
+        for (int e = tid; e <= p.E; e += kB_Threads) mine[e] = 0;
+        __syncthreads();
+        count_rows(p, s, r0, r1, mine);
+        if (p.pieces > 1) {
+            cluster_barrier();
+            for (int e = tid; e <= p.E; e += kB_Threads) {
+                int n = 0;
+                for (int i = 0; i < p.pieces; ++i) n += ld_peer(sh.mine + e, i);
+                sh.hist[e] = n;
+            }
+        }
     } else {
         griddep_wait();
         const int32_t* part = p.count_part + (int64_t)s * p.count_pieces * (p.E + 1);
@@ -266,82 +331,108 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
         for (int e = tid; e < p.E; e += kB_Threads) sh.g[e] = (float)(c * (sh.hist[e] - (double)all / p.E));
         __syncthreads();
     }
-    float g[G][4], acc[G][4];
+    uint64_t g[G][2], acc[G][2];
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-        const int e = i4 + 4 * LANES * j;
+    for (int j = 0; j < G; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { acc[j][i] = 0.0f; g[j][i] = grad && e + i < p.E ? sh.g[e + i] : 0.0f; }
-    }
+        for (int i = 0; i < 2; ++i) {
+            const int e = i4 + 4 * LANES * j + 2 * i;
+            acc[j][i] = 0;
+            g[j][i] = pack2f(grad && e < p.E ? sh.g[e] : 0.0f, grad && e + 1 < p.E ? sh.g[e + 1] : 0.0f);
+        }
 
+#pragma unroll 1
     for (int row0 = row_first; row0 < r1; row0 += kB_Warps * kRows * kU) {
-        float v[kU][G][4];
-        bool on[kU];
+        uint64_t v[kU][G][2];   // two values each
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            on[u] = next_on[u];
+        for (int u = 0; u < kU; ++u)
 #pragma unroll
             for (int j = 0; j < G; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[u][j][i] = next[u][j].value(i);
+                for (int i = 0; i < 2; ++i) v[u][j][i] = pack2f(next[u][j].value(2 * i), next[u][j].value(2 * i + 1));
+        // step by step for all of the warp's rows, so that one row's exchanges between lanes pass behind the others'
+        float mx[kU], sum[kU], dot[kU];
+        uint64_t slope[SIGMOID ? kU : 1][G][2];   // 1 - sigmoid(l)
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            mx[u] = next[u][0].value(0);
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx[u] = fmaxf(mx[u], next[u][j].value(i));
         }
         fetch(row0 + kB_Warps * kRows * kU);   // (the rows after these are on their way while these are worked on)
+        lanes_max<LANES>(mx);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            if (mx[u] == __uint_as_float(0xFF800000u)) mx[u] = 0.0f;   // (-infinities stay zeros, a NaN among them stays one)
+            // l becomes its part of the sum: exp(l - max), or sigmoid(l) -- in rows whose sigmoids are all below 1e-26, where they are exp(l) to
+            // fp32's last digit and could leave its range, the same exp(l - max)
+            const bool low = SIGMOID && mx[u] < -60.0f;
+            const float shift = !SIGMOID || low ? -mx[u] : 0.0f, one = low ? 0.0f : 1.0f;
+            const uint64_t shift2 = pack2f(shift, shift), one2 = pack2f(one, one);
+            uint64_t sum2 = 0, dot2 = 0;
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint64_t& l = v[u][j][i];
+                    if (SIGMOID) {
+                        float a, b;
+                        unpack2(l, a, b);
+                        const uint64_t t = exp_pair(add2(pack2f(-fabsf(a), -fabsf(b)), shift2));
+                        float d0, d1;
+                        unpack2(fma2(t, one2, pack2f(1.0f, 1.0f)), d0, d1);
+                        const uint64_t q = pack2f(rcp(d0), rcp(d1));
+                        float q0, q1, t0, t1;
+                        unpack2(q, q0, q1);
+                        unpack2(mul2(t, q), t0, t1);
+                        const bool up0 = a >= 0.0f, up1 = b >= 0.0f;
+                        slope[u][j][i] = pack2f(up0 ? t0 : q0, up1 ? t1 : q1);
+                        l = pack2f(up0 ? q0 : t0, up1 ? q1 : t1);
+                    } else {
+                        l = exp_pair(add2(l, shift2));
+                    }
+                    sum2 = add2(sum2, l);
+                    dot2 = fma2(l, g[j][i], dot2);
+                }
+            float a, b;
+            unpack2(sum2, a, b);
+            sum[u] = a + b;
+            unpack2(dot2, a, b);
+            dot[u] = a + b;
+        }
+        lanes_sum<LANES>(sum);
+        if (grad) lanes_sum<LANES>(dot);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const float inv = sum[u] == 0.0f ? 0.0f : __frcp_rn(sum[u]);
+            const uint64_t inv2 = pack2f(inv, inv);
+            dot[u] *= inv;
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    v[u][j][i] = mul2(v[u][j][i], inv2);
+                    acc[j][i] = add2(acc[j][i], v[u][j][i]);
+                }
+        }
+        if (!grad) continue;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int r = row0 + u * kRows + sub;
-            float slope[G][4];   // sigmoid mode: 1 - sigmoid(l)
-            float mx = __uint_as_float(0xFF800000u);
-            bool nan = false;
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float& l = v[u][j][i];
-                    if (p.mode == CHIMERE_ROUTE_SIGMOID_NORM_SCALE) {
-                        const float t = expf(-fabsf(l));
-                        slope[j][i] = (l >= 0.0f ? t : 1.0f) / (1.0f + t);
-                        l = (l < 0.0f ? l : l >= 0.0f ? 0.0f : l) - log1pf(t);
-                    }
-                    nan |= l != l;
-                    mx = fmaxf(mx, l);
-                }
-            mx = lanes_max<LANES>(mx);
-            const bool none = mx == __uint_as_float(0xFF800000u);   // no finite logit: no probabilities
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float& l = v[u][j][i];
-                    l = none && !nan ? 0.0f : expf(l - mx);
-                    sum += l;
-                }
-            sum = lanes_sum<LANES>(sum);
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            float dot = 0.0f;
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float& l = v[u][j][i];
-                    l *= inv;
-                    if (on[u] && i < there[j]) acc[j][i] += l;
-                    dot = fmaf(l, g[j][i], dot);
-                }
-            if (!grad) continue;
-            dot = lanes_sum<LANES>(dot);
-            if (r >= r1) continue;
             const int64_t at = (int64_t)s * p.stride_ds + (int64_t)r * p.ldd + i4;
+            const uint64_t less = pack2f(-dot[u], -dot[u]);
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 float d[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    d[i] = v[u][j][i] * (g[j][i] - dot);
-                    if (p.mode == CHIMERE_ROUTE_SIGMOID_NORM_SCALE) d[i] *= slope[j][i];
-                    if (!on[u]) d[i] = 0.0f;
+                for (int i = 0; i < 2; ++i) {
+                    uint64_t w = mul2(v[u][j][i], add2(g[j][i], less));
+                    if (SIGMOID) w = mul2(w, slope[u][j][i]);
+                    unpack2(w, d[2 * i], d[2 * i + 1]);
                 }
-                store4<TYPE>(p.d_logits, at + 4 * LANES * j, there[j], p.vec, d);
+                store4<TYPE, FULL>(p.d_logits, at + 4 * LANES * j, r < r1 ? there[j] : 0, p.vec, d);
             }
         }
     }
@@ -353,10 +444,13 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
     for (int j = 0; j < G; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            float a, b;
+            unpack2(acc[j][i / 2], a, b);
+            float v = i & 1 ? b : a;
 #pragma unroll
-            for (int d = LANES; d < 32; d <<= 1) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], d);
+            for (int d = LANES; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
             const int e = i4 + 4 * LANES * j + i;
-            if (sub == 0 && e < p.E) sh.part[warp][e] = acc[j][i];
+            if (sub == 0 && e < p.E) sh.part[warp][e] = v;
         }
     __syncthreads();
     auto of_piece = [&](int e) {
@@ -365,8 +459,19 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
         for (int w = 0; w < kB_Warps; ++w) v += (double)sh.part[w][e];
         return v;
     };
-    if (p.pieces == 1) {
-        finish_sequence(p, sh, s, of_piece);
+    if (p.count_pieces == 0) {
+        if (p.pieces > 1) {
+            for (int e = tid; e < p.E; e += kB_Threads) sh.sums[e] = (float)of_piece(e);
+            cluster_barrier();
+            if (piece == 0) finish_sequence(p, sh, s, [&](int e) {
+                double v = 0.0;
+                for (int i = 0; i < p.pieces; ++i) v += (double)__int_as_float(ld_peer(reinterpret_cast<int*>(sh.sums) + e, i));
+                return v;
+            });
+            cluster_barrier();   // (a CTA's sums stay until they have been read)
+        } else {
+            finish_sequence(p, sh, s, of_piece);
+        }
         return;
     }
     const int groups = groups_of(p.pieces), group = piece / kB_Group, in_group = min(kB_Group, p.pieces - group * kB_Group);
@@ -400,49 +505,66 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
     });
 }
 
-template <int TYPE>
-cudaError_t launch_balance_type(const BalanceParams& p, bool pdl, cudaStream_t stream) {
-    const dim3 grid((unsigned)((int64_t)p.S * p.pieces));
-    auto go = [&](auto kernel) -> cudaError_t {
-        if (pdl) return launch_pdl(kernel, grid, kB_Threads, 0, stream, p);
-        kernel<<<grid, kB_Threads, 0, stream>>>(p);
-        return cudaGetLastError();
-    };
-    if (p.E <= 32) return go(balance_kernel<TYPE, 8, 1>);
-    if (p.E <= 64) return go(balance_kernel<TYPE, 16, 1>);
-    if (p.E <= 128) return go(balance_kernel<TYPE, 32, 1>);
-    return go(balance_kernel<TYPE, 32, 2>);
+template <int TYPE, bool SIGMOID>
+cudaError_t launch_balance_type(const BalanceParams& p, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((int64_t)p.S * p.pieces));
+    cfg.blockDim = dim3(kB_Threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    cfg.attrs = attr;
+    if (p.count_pieces) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+    } else if (p.pieces > 1 && p.ids) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)p.pieces;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+    }
+    auto go = [&](auto full, auto any, int logits) { return cudaLaunchKernelEx(&cfg, p.vec && p.E == logits ? full : any, p); };
+    if (p.E <= 32) return go(balance_kernel<TYPE, 8, 1, SIGMOID, true>, balance_kernel<TYPE, 8, 1, SIGMOID, false>, 32);
+    if (p.E <= 64) return go(balance_kernel<TYPE, 16, 1, SIGMOID, true>, balance_kernel<TYPE, 16, 1, SIGMOID, false>, 64);
+    if (p.E <= 128) return go(balance_kernel<TYPE, 32, 1, SIGMOID, true>, balance_kernel<TYPE, 32, 1, SIGMOID, false>, 128);
+    return go(balance_kernel<TYPE, 32, 2, SIGMOID, true>, balance_kernel<TYPE, 32, 2, SIGMOID, false>, 256);
 }
-cudaError_t launch_balance(const BalanceParams& p, int type, bool pdl, cudaStream_t stream) {
-    return type == CHIMERE_TYPE_F32 ? launch_balance_type<CHIMERE_TYPE_F32>(p, pdl, stream)
-         : type == CHIMERE_TYPE_F16 ? launch_balance_type<CHIMERE_TYPE_F16>(p, pdl, stream) : launch_balance_type<CHIMERE_TYPE_BF16>(p, pdl, stream);
+template <int TYPE> cudaError_t launch_balance_mode(const BalanceParams& p, cudaStream_t stream) {
+    return p.mode == CHIMERE_ROUTE_SIGMOID_NORM_SCALE ? launch_balance_type<TYPE, true>(p, stream) : launch_balance_type<TYPE, false>(p, stream);
+}
+cudaError_t launch_balance(const BalanceParams& p, int type, cudaStream_t stream) {
+    return type == CHIMERE_TYPE_F32 ? launch_balance_mode<CHIMERE_TYPE_F32>(p, stream)
+         : type == CHIMERE_TYPE_F16 ? launch_balance_mode<CHIMERE_TYPE_F16>(p, stream) : launch_balance_mode<CHIMERE_TYPE_BF16>(p, stream);
 }
 
-// Pieces of a sequence: as many CTAs as run at once, and at least kB_PieceRows rows in each; counting CTAs likewise.
-constexpr int kB_PieceRows = 32;
+// Pieces of a sequence.  With the counting in front: as many CTAs as run at once.  In clusters: two to eight, at least kB_PieceRows rows in each; taken
+// for short sequences, and for so many of them that eight pieces of each fill the GPU.
+constexpr int kB_PieceRows = 32, kB_Cluster = 8, kB_ClusterRows = 512, kB_Sms = 148;   // (the scratch's size goes by these: constants)
 struct Plan { int pieces, rows, count_pieces, count_rows; };
-Plan plan_of(int64_t S, int L, int k, bool stats) {
+Plan plan_of(int64_t S, int L, int k) {
     Plan r{};
-    int64_t n = ((int64_t)kB_CtasPerSm * 148 + S - 1) / S;      // (the scratch's size goes by it: a constant of the GPU this is written for)
-    const int64_t most = ((int64_t)L + kB_PieceRows - 1) / kB_PieceRows;
-    n = n > most ? most : n;
-    n = n > kB_MaxPieces ? kB_MaxPieces : n < 1 ? 1 : n;
-    r.rows = (int)((L + n - 1) / n);
-    r.pieces = r.rows > 0 ? (int)(((int64_t)L + r.rows - 1) / r.rows) : 1;
-    if (r.pieces < 1) r.pieces = 1;
-    if (stats && r.pieces > 1) {
-        int64_t c = ((int64_t)L * k + kB_CountCluster * kB_CountIds - 1) / (kB_CountCluster * kB_CountIds);
-        c = c > kB_MaxCountPieces ? kB_MaxCountPieces : c;
-        r.count_pieces = (int)c;
-        r.count_rows = (int)((L + c * kB_CountCluster - 1) / (c * kB_CountCluster));
+    if (L <= kB_ClusterRows || S * kB_Cluster >= kB_CtasPerSm * kB_Sms) {
+        r.pieces = 1;
+        while (r.pieces < kB_Cluster && L > r.pieces * kB_PieceRows) r.pieces *= 2;
+        r.rows = (int)(((int64_t)L + r.pieces - 1) / r.pieces);
+        return r;
     }
+    const int64_t n = kB_CtasPerSm * kB_Sms / S;      // (rounded down: one more wave for a few pieces would double the time)
+    r.rows = (int)((L + n - 1) / n);
+    r.rows = r.rows < kB_PieceRows ? kB_PieceRows : r.rows;
+    r.pieces = (int)(((int64_t)L + r.rows - 1) / r.rows);
+    int64_t c = ((int64_t)L * k + kB_CountCluster * kB_CountIds - 1) / (kB_CountCluster * kB_CountIds);
+    c = c > kB_MaxCountPieces ? kB_MaxCountPieces : c;
+    r.count_pieces = (int)c;
+    r.count_rows = (int)((L + c * kB_CountCluster - 1) / (c * kB_CountCluster));
     return r;
 }
+static_assert(kB_CtasPerSm * kB_Sms <= kB_Group * kB_Group, "two levels of sums");
 inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 struct Scratch { size_t count_part, part, group_part, counters, total; };
 Scratch scratch_of(const Plan& r, int64_t S, int E) {
     Scratch a{};
-    if (r.pieces == 1) { a.total = 256; return a; }
+    if (r.count_pieces == 0) { a.total = 256; return a; }
     size_t o = 0;
     a.group_part = o; o += up256((size_t)S * groups_of(r.pieces) * E * 8);
     a.part = o; o += up256((size_t)S * r.pieces * E * 4);
@@ -455,7 +577,7 @@ inline bool misaligned(const void* p, int to) { return ((uintptr_t)p & (uintptr_
 inline int rc_of(cudaError_t e) { return e == cudaSuccess ? 0 : -(100 + (int)e); }
 
 int check_dims(int64_t S, int64_t L, int E, int k, int mode, int type, int64_t ld, int64_t stride_s) {
-    if (S < 0 || L < 0 || S > 0x7FFFFFFF / (kB_MaxPieces * kB_CountCluster) || L > 0x7FFFFF00 || E <= 0 || E > kMaxExperts || k <= 0 || k > kMaxExperts) return -2;
+    if (S < 0 || L < 0 || S > 0x7FFFFFFF / 1024 || L > 0x7FFFFF00 || E <= 0 || E > kMaxExperts || k <= 0 || k > kMaxExperts) return -2;
     if (L > 0 && S > 0x7FFFFFFF / L) return -2;      // (counts and token numbers are 32-bit)
     if (L > 0 && k > 0x7FFFFFFF / L) return -2;
     if (mode != CHIMERE_ROUTE_SOFTMAX_RENORM && mode != CHIMERE_ROUTE_SIGMOID_NORM_SCALE) return -2;
@@ -477,7 +599,7 @@ extern "C" {
 
 size_t chimere_b200_balance_loss_bytes(int64_t S, int64_t L, int E, int top_k) {
     if (check_dims(S, L, E, top_k, CHIMERE_ROUTE_SOFTMAX_RENORM, CHIMERE_TYPE_F32, E, 0)) return 0;
-    return S == 0 ? 256 : scratch_of(plan_of(S, (int)L, top_k, true), S, E).total;
+    return S == 0 ? 256 : scratch_of(plan_of(S, (int)L, top_k), S, E).total;
 }
 
 int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_t stride_s, const int32_t* d_topk_idx, const uint8_t* d_mask, int64_t S, int64_t L, int E,
@@ -491,7 +613,7 @@ int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_
     const int size = type == CHIMERE_TYPE_F32 ? 4 : 2;
     if (misaligned(d_ws, 256) || misaligned(d_logits, size) || misaligned(d_grad_logits, size) || misaligned(d_topk_idx, 4) || misaligned(d_loss, 4) || misaligned(d_counts, 4) ||
         misaligned(d_prob, 4) || misaligned(d_tokens, 4) || misaligned(d_grad_loss, 4)) return -5;
-    const Plan plan = plan_of(S, (int)L, top_k, true);
+    const Plan plan = plan_of(S, (int)L, top_k);
     const Scratch a = scratch_of(plan, S, E);
     if (ws_bytes < a.total) return -4;
     uint8_t* ws = (uint8_t*)d_ws;
@@ -508,7 +630,7 @@ int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return rc_of(e);
     }
-    return rc_of(launch_balance(p, type, p.count_pieces > 0, stream));
+    return rc_of(launch_balance(p, type, stream));
 }
 
 int chimere_b200_balance_loss_backward(const void* d_logits, int type, int64_t ld, int64_t stride_s, const uint8_t* d_mask, const int32_t* d_counts, const int32_t* d_tokens,
@@ -521,7 +643,7 @@ int chimere_b200_balance_loss_backward(const void* d_logits, int type, int64_t l
     if (!d_logits || !d_counts || !d_tokens || !d_grad_logits) return -1;
     const int size = type == CHIMERE_TYPE_F32 ? 4 : 2;
     if (misaligned(d_logits, size) || misaligned(d_grad_logits, size) || misaligned(d_counts, 4) || misaligned(d_tokens, 4) || misaligned(d_grad_loss, 4)) return -5;
-    const Plan plan = plan_of(S, (int)L, top_k, false);
+    const Plan plan = plan_of(S, (int)L, top_k);
     BalanceParams p{};
     p.logits = d_logits; p.ld = ld; p.stride_s = stride_s; p.mask = d_mask;
     p.S = (int)S; p.L = (int)L; p.E = E; p.k = top_k; p.mode = route_mode; p.coef = coef;
@@ -529,7 +651,7 @@ int chimere_b200_balance_loss_backward(const void* d_logits, int type, int64_t l
     p.d_loss = d_grad_loss; p.d_logits = d_grad_logits; p.ldd = ld_grad; p.stride_ds = stride_grad_s;
     p.vec = vectors(d_logits, ld, S > 1 ? stride_s : 0, E, type) && vectors(d_grad_logits, ld_grad, S > 1 ? stride_grad_s : 0, E, type);
     p.pieces = plan.pieces; p.rows = plan.rows;
-    return rc_of(launch_balance(p, type, false, stream));
+    return rc_of(launch_balance(p, type, stream));
 }
 
 }  // extern "C"
