@@ -185,7 +185,6 @@ cudaError_t launch_quantize(QuantParams p, int type, cudaStream_t stream, bool p
 //   many tokens (wide_kernel)    256 tokens x 256 weight rows by a pair of CTAs (cta_group::2): each fetches its 128 tokens and 128 of the weight rows
 //       (with SwiGLU one the gate's, the other the up matrix'), half of what a CTA alone would need for the same MMAs.  A thread of the epilogue has
 //       one token's row: its scale and place are looked up once, its results go out 32 bytes at a time.
-// Rows of x that an index array picks (the dispatch's pairs) are fetched by tile::gather4, four rows an instruction, a lane's four rows each.
 // All waits are bounded: one that runs out makes the tile's outputs NaN and raises the status word.
 constexpr int kMM_KBytes = 128;          // of K per stage
 constexpr int kMM_ABytes = 128 * kMM_KBytes;
@@ -199,11 +198,9 @@ struct MatmulParams {
     void* y;
     int64_t ldy, y_rows;
     const int32_t* offsets;    // grouped: [E + 1], else null
-    const int32_t* rows;       // rows of x by index (over rows_div), or null
     const int32_t* out_rows;   // or null
     int32_t* status;           // or null
     int M, N, K, E;
-    int rows_div, x_rows;
     int y_type, act;
     int mt, nt;                // dense: token tiles; tiles of outputs
     int n_stages, split;
@@ -270,15 +267,6 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
     else
         asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
-template <int CTAS>
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&r)[4], uint32_t bar) {
-    if (CTAS == 1)
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar) : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar) : "memory");
 }
 template <int CTAS>
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -378,38 +366,6 @@ __device__ __forceinline__ Tile take_tile(const MatmulParams& p, const GroupTabl
     t.n0 = local / c * OUTS;
     return t;
 }
-// Row of x behind row `i` of the product, -1 if there is none.
-__device__ __forceinline__ int source_row(const MatmulParams& p, int i) {
-    if (!p.rows) return i;
-    const int r = __ldg(p.rows + i), s = r < 0 ? -1 : r / p.rows_div;
-    return s < p.x_rows ? s : -1;
-}
-// A warp's copies of `n` token rows (a stage's 128 bytes of each) from x: one box of BOX rows, or lane i rows 4 i .. 4 i + 3 (and so on, 128 further).
-template <int BOX> struct RowList { int r[(BOX + 127) / 128][4]; };
-template <int BOX>
-__device__ __forceinline__ void list_rows(const MatmulParams& p, RowList<BOX>& l, int row0, int n, int lane) {
-    if (!p.rows) return;
-#pragma unroll
-    for (int h = 0; h < (BOX + 127) / 128; ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = 128 * h + 4 * lane + j;
-            l.r[h][j] = i < n ? max(source_row(p, row0 + i), 0) : 0;
-        }
-}
-template <int BOX> __device__ __forceinline__ uint32_t row_bytes_of(const MatmulParams& p, int n) { return n <= 0 ? 0u : (p.rows ? (uint32_t)(n + 3) / 4 * 4 : (uint32_t)BOX) * kMM_KBytes; }
-template <int CTAS, int BOX>
-__device__ __forceinline__ void load_rows(const MatmulParams& p, const CUtensorMap* map, const RowList<BOX>& l, uint32_t dst, int k0, int row0, int n, uint32_t bar, int lane) {
-    if (p.rows) {
-#pragma unroll
-        for (int h = 0; h < (BOX + 127) / 128; ++h)
-            if (128 * h + 4 * lane < n) tma_gather4<CTAS>(dst + (128 * h + 4 * lane) * kMM_KBytes, map, k0, l.r[h], bar);
-    } else if (n > 0 && elect1()) {
-        tma_2d<CTAS>(dst, map, k0, row0, bar);
-    }
-    __syncwarp();
-}
-
 template <int TYPE> struct Out;
 template <> struct Out<kF32> {
     using T = float;
@@ -447,11 +403,32 @@ __device__ __forceinline__ Channel channel(const MatmulParams& p, bool dual, int
     }
     return c;
 }
+// silu(g) * u for two pairs: g / (1 + exp(-g)), exp as 2^h times 1 + r with h = -g log2(e) rounded and r what the rounding left out (ln(2) in two parts), the
+// quotient with the hardware's reciprocal.  silu is off by ten half-steps of fp32 at most: ex2 four, 1 + r and its product two, 1 + exp one, the
+// reciprocal two, the last product one.  (Through expf and the division operator the epilogue took longer than the MMAs: 32768 tokens x 512 of
+// 2048 122 us, plain results of the same sums 59.)
+__device__ __forceinline__ void silu_mul2(float g0, float g1, float u0, float u1, float (&y)[2]) {
+    float a = -g0, b = -g1;
+    asm("min.NaN.f32 %0, %0, %1;\n\tmax.NaN.f32 %0, %0, %2;" : "+f"(a) : "f"(200.0f), "f"(-200.0f));   // (beyond, exp is infinite or 0 as it is there)
+    asm("min.NaN.f32 %0, %0, %1;\n\tmax.NaN.f32 %0, %0, %2;" : "+f"(b) : "f"(200.0f), "f"(-200.0f));
+    const uint64_t x = pack2f(a, b), h = mul2(x, pack2f(1.44269504f, 1.44269504f)), one = pack2f(1.0f, 1.0f);
+    uint64_t r = fma2(h, pack2f(-0.693147182f, -0.693147182f), x);
+    r = fma2(h, pack2f(1.90465421e-9f, 1.90465421e-9f), r);
+    unpack2(h, a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    unpack2(add2(mul2(pack2f(a, b), add2(r, one)), one), a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+    unpack2(mul2(mul2(pack2f(g0, g1), pack2f(a, b)), pack2f(u0, u1)), y[0], y[1]);
+}
+// two tokens of one channel
 template <bool DUAL>
-__device__ __forceinline__ float finish(const MatmulParams& p, const Channel& c, float sx, int acc, int acc_up) {
-    const float v = scaled(acc, c.sw, sx, c.b);
-    if (DUAL) return silu_mul_ref(v, scaled(acc_up, c.sw_up, sx, c.b_up));
-    return p.act == CHIMERE_ACT_RELU2 ? relu2(v) : v;
+__device__ __forceinline__ void finish2(const MatmulParams& p, const Channel& c, float sx0, float sx1, int a0, int a1, int up0, int up1, float (&o)[2]) {
+    o[0] = scaled(a0, c.sw, sx0, c.b);
+    o[1] = scaled(a1, c.sw, sx1, c.b);
+    if (DUAL) silu_mul2(o[0], o[1], scaled(up0, c.sw_up, sx0, c.b_up), scaled(up1, c.sw_up, sx1, c.b_up), o);
+    else if (p.act == CHIMERE_ACT_RELU2) { o[0] = relu2(o[0]); o[1] = relu2(o[1]); }
 }
 
 struct MatmulShared {
@@ -508,19 +485,18 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
         bool ok = true, waited = !p.early;
         for (int id = first; ok && id < total; id += step) {
             const Tile t = take_tile<BN, 128>(p, table, id);
-            RowList<BN> rows;
-            list_rows<BN>(p, rows, t.row0, t.ntok, lane);
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!mbar_wait(&sh.empty[st], ph ^ 1u)) { ok = false; break; }
                 const uint32_t dst = stages + st * kStage, bar = smem_u32(&sh.full[st]);
                 if (elect1()) {
-                    mbar_expect_tx(&sh.full[st], kMM_ABytes * (DUAL ? 2 : 1) + row_bytes_of<BN>(p, t.ntok));
+                    mbar_expect_tx(&sh.full[st], kStage);
                     tma_3d<1>(dst, &map_w, kb * kMM_KBytes, t.n0, t.expert, bar);
                     if (DUAL) tma_3d<1>(dst + kMM_ABytes, &map_w, kb * kMM_KBytes, p.N + t.n0, t.expert, bar);
                 }
                 __syncwarp();
                 if (!waited) { griddep_wait(); waited = true; }
-                load_rows<1, BN>(p, &map_x, rows, dst + kMM_ABytes * (DUAL ? 2 : 1), kb * kMM_KBytes, t.row0, t.ntok, bar, lane);
+                if (elect1()) tma_2d<1>(dst + kMM_ABytes * (DUAL ? 2 : 1), &map_x, kb * kMM_KBytes, t.row0, bar);
+                __syncwarp();
                 used |= 1u << st;
                 if (++st == p.n_stages) { st = 0; ph ^= 1u; }
             }
@@ -566,27 +542,34 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
             mbar_wait(&sh.drain, 0);
         }
     } else if (warp >= kMM_FirstEpi) {
-        // four warps take every other tile: what a tile's scales and places cost to look up passes behind the other four's tile
+        // four warps take every other tile, and look up a tile's scales and places while the one before is on its way
         const int q = warp & 3, buf = (warp - kMM_FirstEpi) >> 2, row = q * 32 + lane;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + buf * kAccCols;
+        constexpr int kPer = (BN + 127) / 128;
         bool ok = true;
         griddep_wait();   // (the tokens' scales; and nothing of y is written before what used its memory has ended)
-        uint32_t ph = 0;
-        for (int id = first + buf * step; id < total; id += 2 * step, ph ^= 1u) {
-            const Tile t = take_tile<BN, 128>(p, table, id);
-            const Channel ch = channel(p, DUAL, t.expert, t.n0 + row);
-            if (S == 1) {
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");   // (the tile before has been read)
-                for (int i = row; i < t.ntok; i += 128) {
-                    const int r = source_row(p, t.row0 + i);
-                    sh.sx[buf][i] = r < 0 ? 0.0f : p.sx[r];
-                    sh.row[buf][i] = p.out_rows ? p.out_rows[t.row0 + i] : t.row0 + i;
+        Tile t;
+        Channel ch;
+        float sx[kPer];
+        int to[kPer];
+        auto look_up = [&](int id) {
+            t = take_tile<BN, 128>(p, table, id);
+            ch = channel(p, DUAL, t.expert, t.n0 + row);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (row + 128 * i < t.ntok) {
+                    sx[i] = p.sx[t.row0 + row + 128 * i];
+                    to[i] = p.out_rows ? p.out_rows[t.row0 + row + 128 * i] : t.row0 + row + 128 * i;
                 }
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");
-            }
-            if (ok && !mbar_wait(&sh.tfull[buf], ph)) { ok = false; sh.failed = 1; }
-            fence_after();
+        };
+        int id = first + buf * step;
+        if (id < total && S == 1) look_up(id);
+        uint32_t ph = 0;
+        for (; id < total; id += 2 * step, ph ^= 1u) {
             if (S > 1) {   // this CTA's part of the sums, over the operands' buffers: [gate / up][token][128]
+                t = take_tile<BN, 128>(p, table, id);
+                if (!mbar_wait(&sh.tfull[buf], ph)) sh.failed = 1;
+                fence_after();
                 int* part = reinterpret_cast<int*>(smem);
                 for (int c0 = 0; c0 < t.ntok; c0 += 16)
 #pragma unroll
@@ -599,19 +582,31 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
                 fence_before();
                 break;
             }
-            for (int c0 = 0; c0 < t.ntok; c0 += 16) {
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");   // (the tile before has been read)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (row + 128 * i < t.ntok) { sh.sx[buf][row + 128 * i] = sx[i]; sh.row[buf][row + 128 * i] = to[i]; }
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");
+            const Channel c = ch;
+            const int ntok = t.ntok, n = t.n0 + row;
+            if (id + 2 * step < total) look_up(id + 2 * step);
+            if (ok && !mbar_wait(&sh.tfull[buf], ph)) { ok = false; sh.failed = 1; }
+            fence_after();
+            for (int c0 = 0; c0 < ntok; c0 += 16) {
                 int v[16], u[16];
                 ld16(taddr + c0, v);
                 if (DUAL) ld16(taddr + BN + c0, u);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < 16; j += 2) {
+                    float o[2];
                     const int m = c0 + j;
-                    if (m < t.ntok && t.n0 + row < p.N) {
-                        const int64_t r = sh.row[buf][m];
-                        float o = finish<DUAL>(p, ch, sh.sx[buf][m], v[j], DUAL ? u[j] : 0);
-                        if (!ok) o = __uint_as_float(0x7FC00000u);
-                        if (r >= 0 && r < p.y_rows) put(p, r * p.ldy + t.n0 + row, o);
-                    }
+                    finish2<DUAL>(p, c, sh.sx[buf][m], sh.sx[buf][m + 1], v[j], v[j + 1], DUAL ? u[j] : 0, DUAL ? u[j + 1] : 0, o);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (m + i < ntok && n < p.N) {
+                            const int64_t r = sh.row[buf][m + i];
+                            if (r >= 0 && r < p.y_rows) put(p, r * p.ldy + n, ok ? o[i] : __uint_as_float(0x7FC00000u));
+                        }
                 }
             }
             fence_before();
@@ -638,10 +633,9 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
                 if (DUAL) up += ld_cluster(cluster_addr(stages + 4 * (i + BN * 128), s));
             }
             const int64_t r = p.out_rows ? p.out_rows[t.row0 + m] : t.row0 + m;
-            const int src = source_row(p, t.row0 + m);
-            float o = finish<DUAL>(p, channel(p, DUAL, t.expert, n), src < 0 ? 0.0f : p.sx[src], acc, up);
-            if (bad) o = __uint_as_float(0x7FC00000u);
-            if (r >= 0 && r < p.y_rows) put(p, r * p.ldy + n, o);
+            float o[2];
+            finish2<DUAL>(p, channel(p, DUAL, t.expert, n), p.sx[t.row0 + m], 0.0f, acc, 0, up, 0, o);
+            if (r >= 0 && r < p.y_rows) put(p, r * p.ldy + n, bad ? __uint_as_float(0x7FC00000u) : o[0]);
         }
         cluster_sync();   // ... and has been read
     }
@@ -768,11 +762,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
         bool ok = true, waited = !p.early;
         for (int id = first; ok && id < total; id += step) {
             const Tile t = take_tile<kW_Tokens, kOuts>(p, table, id);
-            const int row0 = t.row0 + 128 * rank, n = max(0, min(128, t.ntok - 128 * rank));
-            const uint32_t bytes = 2 * kMM_ABytes + row_bytes_of<128>(p, min(128, t.ntok)) + row_bytes_of<128>(p, max(0, t.ntok - 128));
+            const bool mine = t.ntok > 128 * rank;   // (a tile of up to 128 tokens is the first CTA's)
+            const uint32_t bytes = (t.ntok > 128 ? 4 : 3) * kMM_ABytes;
             const int wrow = DUAL ? rank * p.N + t.n0 : t.n0 + 128 * rank;
-            RowList<128> rows;
-            list_rows<128>(p, rows, row0, n, lane);
             for (int kb = 0; kb < nkb; ++kb) {
                 if (!mbar_wait(&sh.empty[st], ph ^ 1u)) { ok = false; break; }
                 const uint32_t dst = stages + st * kW_Stage, bar = bar_addr<2>(&sh.full[st]);
@@ -782,7 +774,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
                 }
                 __syncwarp();
                 if (!waited) { griddep_wait(); waited = true; }
-                load_rows<2, 128>(p, &map_x, rows, dst, kb * kMM_KBytes, row0, n, bar, lane);
+                if (mine && elect1()) tma_2d<2>(dst, &map_x, kb * kMM_KBytes, t.row0 + 128 * rank, bar);
+                __syncwarp();
                 used |= 1u << st;
                 if (++st == p.n_stages) { st = 0; ph ^= 1u; }
             }
@@ -830,33 +823,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
         float* turn = reinterpret_cast<float*>(smem + kW_StagesTurned * kW_Stage) + (warp - kMM_FirstEpi) * kW_TurnFloats;   // (where rows are not aligned)
         bool ok = true;
         griddep_wait();   // (the tokens' scales; and nothing of y is written before what used its memory has ended)
+        // a tile's scales and places are looked up while the one before is on its way
+        Tile t;
+        float sw_next, bias_next, sx_next;
+        int64_t r_next;
+        auto look_up = [&](int id) {
+            t = take_tile<kW_Tokens, kOuts>(p, table, id);
+            const int c = DUAL ? t.n0 + (et & 127) : t.n0 + et;   // accumulator column `et`
+            const int64_t at = ((int64_t)t.expert * (DUAL ? 2 : 1) + (DUAL ? et >> 7 : 0)) * p.N + c;
+            sw_next = c < p.N ? p.sw[at] : 0.0f;
+            bias_next = c < p.N && p.bias ? p.bias[at] : 0.0f;
+            const int i = 128 * rank + row;   // this thread's token of the tile
+            r_next = -1;
+            sx_next = 0.0f;
+            if (i < t.ntok) {
+                sx_next = p.sx[t.row0 + i];
+                r_next = p.out_rows ? p.out_rows[t.row0 + i] : t.row0 + i;
+            }
+        };
+        look_up(first);
         int n = 0;
         for (int id = first; id < total; id += step, ++n) {
-            const Tile t = take_tile<kW_Tokens, kOuts>(p, table, id);
-            const int buf = n & 1;
-            {   // scale and bias of accumulator column `et`
-                const int c = DUAL ? t.n0 + (et & 127) : t.n0 + et;
-                const int64_t at = ((int64_t)t.expert * (DUAL ? 2 : 1) + (DUAL ? et >> 7 : 0)) * p.N + c;
-                sh.sw[buf][et] = c < p.N ? p.sw[at] : 0.0f;
-                sh.bias[buf][et] = c < p.N && p.bias ? p.bias[at] : 0.0f;
-            }
-            const int i = 128 * rank + row;   // this thread's token of the tile
-            int64_t r = -1;
-            float sx = 0.0f;
-            if (i < t.ntok) {
-                const int src = source_row(p, t.row0 + i);
-                if (src >= 0) sx = p.sx[src];
-                r = p.out_rows ? p.out_rows[t.row0 + i] : t.row0 + i;
-                if (r < 0 || r >= p.y_rows) r = -1;
-            }
+            const int buf = n & 1, ntok = t.ntok, n0 = t.n0;
+            sh.sw[buf][et] = sw_next;
+            sh.bias[buf][et] = bias_next;
+            const int64_t r = r_next >= 0 && r_next < p.y_rows ? r_next : -1;
+            float sx = sx_next;
             asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (id + step < total) look_up(id + step);
             if (ok && !mbar_wait(&sh.tfull[buf], (n >> 1) & 1)) { ok = false; sh.failed = 1; }
             fence_after();
             if (!ok) sx = __uint_as_float(0x7FC00000u);
-            if (128 * rank + q * 32 < t.ntok) {
+            if (128 * rank + q * 32 < ntok) {
 #pragma unroll 1
                 for (int c0 = half * (kOuts / 2); c0 < (half + 1) * (kOuts / 2); c0 += 32) {
-                    if (t.n0 + c0 >= p.N) break;
+                    if (n0 + c0 >= p.N) break;
                     int v[32];
                     float o[32];
                     ld32(taddr + buf * kW_Cols + c0, v);
@@ -871,16 +872,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const float4 s = *reinterpret_cast<const float4*>(&sh.sw[buf][128 + c0 + j]), b = *reinterpret_cast<const float4*>(&sh.bias[buf][128 + c0 + j]);
-                            o[j] = silu_mul_ref(o[j], scaled(v[j], s.x, sx, b.x));
-                            o[j + 1] = silu_mul_ref(o[j + 1], scaled(v[j + 1], s.y, sx, b.y));
-                            o[j + 2] = silu_mul_ref(o[j + 2], scaled(v[j + 2], s.z, sx, b.z));
-                            o[j + 3] = silu_mul_ref(o[j + 3], scaled(v[j + 3], s.w, sx, b.w));
+                            float y[2];
+                            silu_mul2(o[j], o[j + 1], scaled(v[j], s.x, sx, b.x), scaled(v[j + 1], s.y, sx, b.y), y);
+                            o[j] = y[0]; o[j + 1] = y[1];
+                            silu_mul2(o[j + 2], o[j + 3], scaled(v[j + 2], s.z, sx, b.z), scaled(v[j + 3], s.w, sx, b.w), y);
+                            o[j + 2] = y[0]; o[j + 3] = y[1];
                         }
                     } else if (p.act == CHIMERE_ACT_RELU2) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) o[j] = relu2(o[j]);
                     }
-                    store_block<TYPE>(p, turn, r, t.n0 + c0, o, lane);
+                    store_block<TYPE>(p, turn, r, n0 + c0, o, lane);
                 }
             }
             fence_before();
@@ -947,7 +949,7 @@ int launch_tile(const MatmulCall& c, int tiles, int split, bool pdl, cudaStream_
     static bool done[64];
     CUtensorMap mx, mw;
     MatmulParams p = c.p;
-    if (!make_map(&mx, c.x, p.K, p.x_rows, 1, c.ldx, 0, p.rows ? 1 : BN, 2)) return -5;
+    if (!make_map(&mx, c.x, p.K, p.M, 1, c.ldx, 0, BN, 2)) return -5;
     if (!make_map(&mw, c.w, p.K, (DUAL ? 2 : 1) * (int64_t)p.N, p.E, c.ldw, c.w_plane, 128, 3)) return -5;
     const int nkb = (p.K + kMM_KBytes - 1) / kMM_KBytes, most = (200 * 1024) / kStage;
     int stages = (nkb + split - 1) / split;
@@ -975,7 +977,7 @@ int launch_wide(const MatmulCall& c, int64_t tiles, bool pdl, cudaStream_t strea
     static bool done[64];
     CUtensorMap mx, mw;
     MatmulParams p = c.p;
-    if (!make_map(&mx, c.x, p.K, p.x_rows, 1, c.ldx, 0, p.rows ? 1 : 128, 2)) return -5;
+    if (!make_map(&mx, c.x, p.K, p.M, 1, c.ldx, 0, 128, 2)) return -5;
     if (!make_map(&mw, c.w, p.K, (DUAL ? 2 : 1) * (int64_t)p.N, p.E, c.ldw, c.w_plane, 128, 3)) return -5;
     constexpr int kOuts = DUAL ? 128 : 256, kSize = TYPE == kF32 ? 4 : 2;
     p.mt = (p.M + kW_Tokens - 1) / kW_Tokens;
@@ -1062,7 +1064,7 @@ int check_quantize(const void* x, int type, int64_t ldx, int64_t x_rows, const i
     return 0;
 }
 int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, int E, int64_t M, int N, int K,
-                 int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* rows, int rows_div, int64_t x_rows, const int32_t* out_rows) {
+                 int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows) {
     const int64_t R = (act == CHIMERE_ACT_SWIGLU ? 2 : 1) * (int64_t)N;
     if (M < 0 || M > 0x7FFFFFFF || N <= 0 || R > 0x7FFFFF00 || K <= 0 || K > kMaxK || E <= 0 || E > kMaxGroups) return -2;
     if (ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldy < N || y_rows < 0) return -2;
@@ -1070,22 +1072,19 @@ int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w,
     if (act != CHIMERE_ACT_NONE && act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
     if (!float_type(y_type)) return -3;
     if (!out_rows && y_rows < M) return -2;
-    if (x_rows < 0 || x_rows > 0x7FFFFFFF || rows_div <= 0 || (rows ? M > 0 && x_rows == 0 : x_rows < M)) return -2;
     if (M == 0) return 0;
     if (!x || !sx || !w || !sw || (!y && y_rows > 0)) return -1;
-    if (misaligned(x, 16) || misaligned(w, 16) || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4) || misaligned(y, type_size(y_type)) || misaligned(rows, 4) ||
-        misaligned(out_rows, 4)) return -5;
+    if (misaligned(x, 16) || misaligned(w, 16) || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4) || misaligned(y, type_size(y_type)) || misaligned(out_rows, 4)) return -5;
     return 0;
 }
 MatmulCall matmul_call(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, const int32_t* offsets, int E,
-                       int64_t M, int N, int K, int act, void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* rows, int rows_div, int64_t x_rows, const int32_t* out_rows,
-                       int32_t* status, bool early) {
+                       int64_t M, int N, int K, int act, void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows, int32_t* status, bool early) {
     MatmulCall c{};
     c.x = x; c.ldx = ldx; c.w = w; c.ldw = ldw;
     c.dual = act == CHIMERE_ACT_SWIGLU;
     c.w_plane = E > 1 ? w_plane : (c.dual ? 2 : 1) * (int64_t)N * ldw;
     MatmulParams& p = c.p;
-    p.sx = sx; p.sw = sw; p.bias = bias; p.y = y; p.ldy = ldy; p.y_rows = y_rows; p.offsets = offsets; p.rows = rows; p.rows_div = rows_div; p.x_rows = (int)x_rows; p.out_rows = out_rows; p.status = status;
+    p.sx = sx; p.sw = sw; p.bias = bias; p.y = y; p.ldy = ldy; p.y_rows = y_rows; p.offsets = offsets; p.out_rows = out_rows; p.status = status;
     p.M = (int)M; p.N = N; p.K = K; p.E = E; p.y_type = y_type; p.act = act; p.early = early;
     return c;
 }
@@ -1116,20 +1115,19 @@ int chimere_b200_quantize_i8(const void* d_x, int x_type, int64_t ldx, int64_t x
 
 int chimere_b200_matmul_w8a8(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,
                              int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy, int32_t* d_status, cudaStream_t stream) {
-    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr);
+    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
     if (rc || M == 0) return rc;
-    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr, d_status, false), false, stream);
+    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, false), false, stream);
 }
 
 int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, int64_t stride_w, const float* d_w_scale,
                                      const float* d_bias, const int32_t* d_offsets, int E, int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy,
-                                     int64_t y_rows, const int32_t* d_rows, int rows_div, int64_t x_rows, const int32_t* d_out_rows, int32_t* d_status, cudaStream_t stream) {
-    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_rows, rows_div, x_rows, d_out_rows);
+                                     int64_t y_rows, const int32_t* d_out_rows, int32_t* d_status, cudaStream_t stream) {
+    const int rc = check_matmul(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_out_rows);
     if (rc || M == 0) return rc;
     if (!d_offsets) return -1;
     if (misaligned(d_offsets, 4)) return -5;
-    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, d_offsets, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_rows, rows_div,
-                                     x_rows, d_out_rows, d_status, false), false, stream);
+    return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, d_offsets, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_out_rows, d_status, false), false, stream);
 }
 
 size_t chimere_b200_linear_w8a8_bytes(int64_t M, int K) {
@@ -1146,13 +1144,13 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
     if (misaligned(d_ws, 256)) return -5;
     int rc = check_quantize(d_x, x_type, ldx, M, nullptr, 1, M, K, q, up16(K), scale);
     if (rc) return rc;
-    rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr);
+    rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
     if (rc || M == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     if (!encoder()) return -6;
     rc = rc_of(launch_quantize(QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, stream, false));
     if (rc) return rc;
-    return launch_matmul(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, 1, M, nullptr, d_status, true), true, stream);
+    return launch_matmul(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, true), true, stream);
 }
 
 size_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F) {
@@ -1169,30 +1167,29 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
     if (act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
     const int64_t P = T * top_k;
     Carver ws{(uint8_t*)d_ws, 0};
-    int8_t* q = (int8_t*)ws.take((size_t)T * up16(H));
-    float* scale = (float*)ws.take((size_t)T * 4);
+    int8_t* q = (int8_t*)ws.take((size_t)P * up16(H));
+    float* scale = (float*)ws.take((size_t)P * 4);
     int8_t* hq = (int8_t*)ws.take((size_t)P * up16(F));
     float* h_scale = (float*)ws.take((size_t)P * 4);
     float* h = (float*)ws.take((size_t)P * up8(F) * 4);
     if (P > 0 && (!d_ws || !d_perm || !d_offsets)) return -1;
     if (misaligned(d_ws, 256) || misaligned(d_offsets, 4)) return -5;
-    int rc = check_quantize(d_x, x_type, ldx, T, nullptr, 1, T, H, q, up16(H), scale);
+    int rc = check_quantize(d_x, x_type, ldx, T, d_perm, top_k, P, H, q, up16(H), scale);
     if (rc) return rc;
-    rc = check_matmul(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, E, P, F, H, act, h, kF32, up8(F), P, d_perm, top_k, T, nullptr);
+    rc = check_matmul(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, E, P, F, H, act, h, kF32, up8(F), P, nullptr);
     if (rc) return rc;
-    rc = check_matmul(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, nullptr, 1, P, d_perm);
+    rc = check_matmul(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm);
     if (rc || P == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     if (!encoder()) return -6;
-    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, nullptr, 1, H, q, up16(H), scale, T, 0}, x_type, stream, false));
+    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, d_perm, top_k, H, q, up16(H), scale, P, 0}, x_type, stream, false));
     if (rc) return rc;
-    rc = launch_matmul(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up8(F), P, d_perm, top_k, T, nullptr, d_status, true),
-                       true, stream);
+    rc = launch_matmul(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up8(F), P, nullptr, d_status, true), true, stream);
     if (rc) return rc;
     rc = rc_of(launch_quantize(QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, P, 0}, kF32, stream, true));
     if (rc) return rc;
-    return launch_matmul(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, nullptr, 1, P,
-                                     d_perm, d_status, true), true, stream);
+    return launch_matmul(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm,
+                                     d_status, true), true, stream);
 }
 
 }  // extern "C"

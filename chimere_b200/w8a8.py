@@ -125,25 +125,23 @@ def _stack(w: torch.Tensor, name: str, device: torch.device) -> Tuple[int, int, 
 
 
 def matmul_w8a8_grouped(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
-                        act: int = abi.ACT_NONE, rows: Optional[torch.Tensor] = None, rows_div: int = 1, out_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                        act: int = abi.ACT_NONE, out_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                         out_dtype: Optional[torch.dtype] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same with a matrix per group of rows: rows offsets[e] .. offsets[e + 1] of q (int32 [E + 1], as the router's dispatch leaves them) by w[e];
-    w int8 [E, N or 2 N, K], w_scale and bias f32 [E, N or 2 N].  With `rows` (int32 [M]) row i of the product is row rows[i] // rows_div of q -- the dispatch
-    permutation and top_k, say; zeros where q has none -- with its scale.  With out_rows (int32 [M]) row i goes to row out_rows[i] of `out`.  Rows that belong to no
+    w int8 [E, N or 2 N, K], w_scale and bias f32 [E, N or 2 N].  With out_rows (int32 [M]) row i goes to row out_rows[i] of `out`.  Rows that belong to no
     group, and rows with an index outside `out`, are not written: `out` keeps what it held there (without `out` those rows are not initialised)."""
     _need(q.is_cuda and q.dim() == 2 and w.dim() == 3 and q.shape[1] == w.shape[2], "q [M, K] and w [E, N, K] on a CUDA device")
-    dev, (n, K), (E, R) = q.device, q.shape, w.shape[:2]
-    M = n if rows is None else rows.shape[0]
+    dev, (M, K), (E, R) = q.device, q.shape, w.shape[:2]
     _need(act != abi.ACT_SWIGLU or R % 2 == 0, "w: gate and up rows in equal number")
     N = R // 2 if act == abi.ACT_SWIGLU else R
     y_rows = M if out is None or out_rows is None else out.shape[0]
     out = _output(out, y_rows, N, out_dtype or (None if out is not None else torch.float32), dev)
     xp, ldx = _weight(q, "q", dev)
     wp, ldw, plane = _stack(w, "w", dev)
-    _call("chimere_b200_matmul_w8a8_grouped", dev, xp, ldx, _vector(q_scale, "q_scale", (n,), torch.float32, dev), wp, ldw, plane,
+    _call("chimere_b200_matmul_w8a8_grouped", dev, xp, ldx, _vector(q_scale, "q_scale", (M,), torch.float32, dev), wp, ldw, plane,
           _vector(w_scale, "w_scale", (E, R), torch.float32, dev), _vector(bias, "bias", (E, R), torch.float32, dev),
           _vector(offsets, "offsets", (E + 1,), torch.int32, dev), E, M, N, K, act, out.data_ptr(), _TYPES[out.dtype], _ld_out(out), y_rows,
-          _vector(rows, "rows", (M,), torch.int32, dev), rows_div, n, _vector(out_rows, "out_rows", (M,), torch.int32, dev), _vector(status, "status", (1,), torch.int32, dev))
+          _vector(out_rows, "out_rows", (M,), torch.int32, dev), _vector(status, "status", (1,), torch.int32, dev))
     return out
 
 

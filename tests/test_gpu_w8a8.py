@@ -1,8 +1,9 @@
 """W8A8 products and their quantised rows against their definition in 64 bits.
 
 Bounds, relative to 2^-24 (half a step of f32, u below): a sum converted to f32, its two scales and the bias are four roundings; an output of
-fewer bits adds half a step of its own type.  silu(g) = g / (1 + exp(-g)): exp two steps (4 u), the sum and the quotient one rounding each, so
-6 u, and its slope is at most 1.1; the product with u one more rounding."""
+fewer bits adds half a step of its own type.  silu(g) = g / (1 + exp(-g)): exp as 2^h (1 + r), ex2 off by 2^-22 (4 u), the sum 1 + r and the product one rounding
+each; 1 + exp one, the reciprocal one step (2 u), the product with g one: 10 u, and silu's slope is at most 1.1; the product with u one more rounding.
+Below -87, where the reciprocal is subnormal, it is 0: off by less than 88 * 2^-126."""
 import numpy as np
 import pytest
 import torch
@@ -53,7 +54,7 @@ def product(q, sx, w, sw, bias, act, dtype):
         n = v.shape[1] // 2
         g, u, eg, eu = v[:, :n], v[:, n:], e[:, :n], e[:, n:]
         s = g * torch.sigmoid(g)
-        es = 1.1 * eg + 6 * U * s.abs() + 2.0 ** -126
+        es = 1.1 * eg + 10 * U * s.abs() + 2.0 ** -119
         y, e = s * u, es * (u.abs() + eu) + s.abs() * eu + U * (s * u).abs()
     elif act == abi.ACT_RELU2:
         r = v.clamp_min(0)
@@ -245,25 +246,6 @@ def test_grouped_rows_to_other_places(M):
     assert torch.equal(out, want)
 
 
-@pytest.mark.parametrize("act", [abi.ACT_NONE, abi.ACT_SWIGLU])
-@pytest.mark.parametrize("M,K,N,counts", [(11, 100, 70, [4, 0, 7]), (70, 512, 130, [1, 33, 36]), (900, 700, 300, [500, 3, 397]), (1500, 256, 512, [129, 771, 600])])
-def test_grouped_rows_from_other_places(M, K, N, counts, act):
-    g = gen(M + K)
-    n, E, R = M // 2, len(counts), 2 * N if act == abi.ACT_SWIGLU else N
-    q, w, sx, sw = i8(g, n, K), i8(g, E, R, K), scales(g, n) / K ** 0.5, scales(g, E, R)
-    rows = torch.randint(0, 3 * n, (M,), generator=g, device="cuda", dtype=torch.int32)
-    rows[0], rows[1], rows[2], rows[M - 1] = -1, 3 * n, 2 ** 31 - 1, -2 ** 31       # no such rows
-    off = groups(counts)
-    y = w8a8.matmul_w8a8_grouped(q, sx, w, sw, off, act=act, rows=rows, rows_div=3, out_dtype=torch.bfloat16)
-    there = (rows >= 0) & (rows < 3 * n)
-    src = torch.where(there, rows // 3, 0).long()
-    fq, fs = torch.where(there[:, None], q[src], 0), torch.where(there, sx[src], 0.0)
-    for e in range(E):
-        a, b = int(off[e]), int(off[e + 1])
-        if b > a:
-            check(y[a:b], *product(fq[a:b], fs[a:b], w[e], sw[e], None, act, torch.bfloat16))
-
-
 def test_offsets_that_fall_are_empty_groups():
     g = gen(3)
     q, w, sx, sw = i8(g, 30, 64), i8(g, 4, 48, 64), scales(g, 30), scales(g, 4, 48)
@@ -319,8 +301,6 @@ def test_experts_behind_the_router(cfg, T):
     # the four steps one by one
     q, s = w8a8.quantize_i8(x, perm, k)
     h = w8a8.matmul_w8a8_grouped(q, s, w_up, s_up, off, act=cfg.act)
-    q, s = w8a8.quantize_i8(x)
-    assert torch.equal(h, w8a8.matmul_w8a8_grouped(q, s, w_up, s_up, off, act=cfg.act, rows=perm, rows_div=k))
     hq, hs = w8a8.quantize_i8(h)
     steps = w8a8.matmul_w8a8_grouped(hq, hs, w_dn, s_dn, off, out_rows=perm, out=torch.empty_like(y))
     assert torch.equal(y, steps)

@@ -20,8 +20,8 @@ def matmul(lib, x=A, ldx=64, sx=A, w=A, ldw=64, sw=A, bias=None, M=4, N=32, K=64
     return lib.chimere_b200_matmul_w8a8(x, ldx, sx, w, ldw, sw, bias, M, N, K, act, y, y_type, ldy, None, None)
 
 
-def grouped(lib, x=A, w=A, ldw=64, stride=2048, offsets=A, E=3, M=4, N=32, K=64, act=abi.ACT_NONE, y_rows=4, rows=None, div=1, x_rows=4, out_rows=None, ldy=32):
-    return lib.chimere_b200_matmul_w8a8_grouped(x, 64, A, w, ldw, stride, A, None, offsets, E, M, N, K, act, A, abi.TYPE_F32, ldy, y_rows, rows, div, x_rows, out_rows, None, None)
+def grouped(lib, x=A, w=A, ldw=64, stride=2048, offsets=A, E=3, M=4, N=32, K=64, act=abi.ACT_NONE, y_rows=4, out_rows=None, ldy=32):
+    return lib.chimere_b200_matmul_w8a8_grouped(x, 64, A, w, ldw, stride, A, None, offsets, E, M, N, K, act, A, abi.TYPE_F32, ldy, y_rows, out_rows, None, None)
 
 
 def linear(lib, x=A, ldx=64, M=4, N=32, K=64, ws=A, nbytes=1 << 20, w=A):
@@ -47,8 +47,7 @@ def test_matmul(lib, want, kw):
     assert matmul(lib, **kw) == want
 
 
-@pytest.mark.parametrize("want,kw", [(-2, dict(E=0)), (-2, dict(E=1025)), (-2, dict(stride=2040)), (-2, dict(stride=1024)), (-2, dict(act=abi.ACT_SWIGLU)), (-2, dict(y_rows=3)), (-2, dict(y_rows=-1)), (-2, dict(x_rows=3)), (-2, dict(rows=A, x_rows=0)), (-2, dict(div=0)),
-                                     (-5, dict(rows=A + 2)),
+@pytest.mark.parametrize("want,kw", [(-2, dict(E=0)), (-2, dict(E=1025)), (-2, dict(stride=2040)), (-2, dict(stride=1024)), (-2, dict(act=abi.ACT_SWIGLU)), (-2, dict(y_rows=3)), (-2, dict(y_rows=-1)),
                                      (-1, dict(offsets=None)), (-5, dict(offsets=A + 1)), (-5, dict(out_rows=A + 2)), (0, dict(M=0, offsets=None))])
 def test_grouped(lib, want, kw):
     assert grouped(lib, **kw) == want
