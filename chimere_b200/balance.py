@@ -54,7 +54,7 @@ def _place(t: torch.Tensor, a: _Args) -> Tuple[int, int, int]:
 
 def _forward(logits, topk_idx, mask, a: _Args, grad_loss, d_logits) -> BalanceLoss:
     dev = logits.device
-    nbytes = abi.load().chimere_b200_balance_loss_bytes(a.S, a.L, a.E, a.k)
+    nbytes = (abi._lib or abi.load()).chimere_b200_balance_loss_bytes(a.S, a.L, a.E, a.k)
     _need(nbytes > 0, "logits up to 256 wide, up to 256 ids per row, fewer than 2^31 rows and ids")
     S = () if logits.dim() == 2 else (a.S,)
     loss = torch.empty(S, dtype=torch.float32, device=dev)
@@ -64,7 +64,7 @@ def _forward(logits, topk_idx, mask, a: _Args, grad_loss, d_logits) -> BalanceLo
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     p, ld, stride = _place(logits, a)
     dp, ldd, stride_d = (None, a.E, 0) if d_logits is None else _place(d_logits, a)
-    _call("chimere_b200_balance_loss", dev, p, _TYPES[logits.dtype], ld, stride, topk_idx.data_ptr(), None if mask is None else mask.data_ptr(), a.S, a.L, a.E, a.k, a.mode,
+    _call("chimere_b200_balance_loss", logits.get_device(), p, _TYPES[logits.dtype], ld, stride, topk_idx.data_ptr(), None if mask is None else mask.data_ptr(), a.S, a.L, a.E, a.k, a.mode,
           a.coef, loss.data_ptr(), counts.data_ptr(), prob.data_ptr(), tokens.data_ptr(), None if grad_loss is None else grad_loss.data_ptr(), dp, ldd, stride_d,
           ws.data_ptr(), nbytes)
     return BalanceLoss(loss, counts, prob, tokens)
@@ -127,6 +127,6 @@ def balance_loss_backward(logits: torch.Tensor, counts: torch.Tensor, tokens: to
     d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     p, ld, stride = _place(logits, a)
     dp, ldd, stride_d = _place(d, a)
-    _call("chimere_b200_balance_loss_backward", logits.device, p, _TYPES[logits.dtype], ld, stride, None if mask is None else mask.data_ptr(), counts.data_ptr(),
+    _call("chimere_b200_balance_loss_backward", logits.get_device(), p, _TYPES[logits.dtype], ld, stride, None if mask is None else mask.data_ptr(), counts.data_ptr(),
           tokens.data_ptr(), a.S, a.L, a.E, top_k, a.mode, a.coef, None if g is None else g.data_ptr(), dp, ldd, stride_d)
     return d

@@ -83,8 +83,8 @@ struct RowScale {
     __device__ __forceinline__ uint32_t q4(float a, float b, float c, float d) const { return prmt(prmt(q(a), q(b), 0x0040u), prmt(q(c), q(d), 0x0040u), 0x5410u); }
 };
 
-// GROUP 32: a warp per row, eight rows per CTA; GROUP 0: a CTA per row
-template <int TYPE, int GROUP, int VECS>
+// GROUP 32: a warp per row, eight rows per CTA; GROUP 0: a CTA per row.  VEC: rows on 16-byte boundaries
+template <int TYPE, int GROUP, int VECS, bool VEC = true>
 __global__ void __launch_bounds__(GROUP ? 256 : 1024) quantize_rows_kernel(QuantParams p) {
     using E = Elem<TYPE>;
     __shared__ uint32_t s_max[32];
@@ -105,9 +105,17 @@ __global__ void __launch_bounds__(GROUP ? 256 : 1024) quantize_rows_kernel(Quant
         return;
     }
     const typename E::T* x = reinterpret_cast<const typename E::T*>(p.x) + src * p.ldx;
-    const int nv = p.vec ? p.K >> 3 : 0;
-    typename E::Raw v[VECS];
     uint32_t m = 0;
+    constexpr int kOnes = VEC ? 1 : 16;   // rows off the 16-byte boundaries: value by value
+    float one[kOnes];
+    if (!VEC) {
+#pragma unroll
+        for (int i = 0; i < kOnes; ++i) one[i] = tid + i * nt < p.K ? E::one(x + tid + i * nt) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kOnes; ++i) m = max(m, __float_as_uint(one[i]) & 0x7FFFFFFFu);
+    }
+    const int nv = VEC ? p.K >> 3 : 0, ones = VEC ? 8 * nv : min(p.K, kOnes * nt);
+    typename E::Raw v[VECS];
 #pragma unroll
     for (int i = 0; i < VECS; ++i)
         if (tid + i * nt < nv) v[i] = E::load8(x + 8 * (tid + i * nt));
@@ -115,7 +123,7 @@ __global__ void __launch_bounds__(GROUP ? 256 : 1024) quantize_rows_kernel(Quant
     for (int i = 0; i < VECS; ++i)
         if (tid + i * nt < nv) m = E::top(v[i], m);
     for (int i = tid + VECS * nt; i < nv; i += nt) m = E::top(E::load8(x + 8 * i), m);
-    for (int i = 8 * nv + tid; i < p.K; i += nt) m = max(m, __float_as_uint(E::one(x + i)) & 0x7FFFFFFFu);
+    for (int i = ones + tid; i < p.K; i += nt) m = max(m, __float_as_uint(E::one(x + i)) & 0x7FFFFFFFu);
     m = __reduce_max_sync(0xffffffffu, m);
     if (!GROUP && nt > 32) {
         if ((tid & 31) == 0) s_max[tid >> 5] = m;
@@ -147,7 +155,12 @@ __global__ void __launch_bounds__(GROUP ? 256 : 1024) quantize_rows_kernel(Quant
     for (int i = 0; i < VECS; ++i)
         if (tid + i * nt < nv) put(tid + i * nt, v[i]);
     for (int i = tid + VECS * nt; i < nv; i += nt) put(i, E::load8(x + 8 * i));
-    for (int i = 8 * nv + tid; i < p.K; i += nt) q[i] = (int8_t)s.q(E::one(x + i));
+    if (!VEC) {
+#pragma unroll
+        for (int i = 0; i < kOnes; ++i)
+            if (tid + i * nt < p.K) q[tid + i * nt] = (int8_t)s.q(one[i]);
+    }
+    for (int i = ones + tid; i < p.K; i += nt) q[i] = (int8_t)s.q(E::one(x + i));
 }
 
 template <int TYPE>
@@ -166,10 +179,10 @@ cudaError_t launch_quantize_type(const QuantParams& p, cudaStream_t stream, bool
         if (pieces <= 8) return go(quantize_rows_kernel<TYPE, 32, 8 / k>, grid, 256);
         return go(quantize_rows_kernel<TYPE, 32, 16 / k>, grid, 256);
     }
-    // two pieces of eight values per thread, at least a warp
+    // sixteen values per thread, at least a warp
     int nt = (p.K + 15) / 16;
     nt = nt > 1024 ? 1024 : (nt + 31) / 32 * 32;
-    return go(quantize_rows_kernel<TYPE, 0, 2>, p.M, nt);
+    return p.vec ? go(quantize_rows_kernel<TYPE, 0, 2>, p.M, nt) : go(quantize_rows_kernel<TYPE, 0, 2, false>, p.M, nt);
 }
 cudaError_t launch_quantize(QuantParams p, int type, cudaStream_t stream, bool pdl) {
     p.vec = ((uintptr_t)p.x & 15) == 0 && (p.ldx * (type == kF32 ? 4 : 2)) % 16 == 0;
@@ -180,7 +193,7 @@ cudaError_t launch_quantize(QuantParams p, int type, cudaStream_t stream, bool p
 // tcgen05 kind::i8; operands by TMA as rows of 128 bytes (128-byte swizzle), zeros beyond K and beyond the last row.  Two kernels, which differ
 // in whose rows are the MMA's:
 //   few tokens (matmul_kernel)   128 weight rows (two such blocks, gate and up, where the activation joins them) x BN tokens, BN the narrowest of
-//       16 .. 256 that suits the batch.  Where there are fewer tiles than SMs a cluster of up to eight CTAs shares a tile, each with a
+//       16, 32 and 64 that suits the batch.  Where there are fewer tiles than SMs a cluster of up to eight CTAs shares a tile, each with a
 //       part of K; their int32 sums meet in shared memory over the cluster, exact in any order.
 //   many tokens (wide_kernel)    256 tokens x 256 weight rows by a pair of CTAs (cta_group::2): each fetches its 128 tokens and 128 of the weight rows
 //       (with SwiGLU one the gate's, the other the up matrix'), half of what a CTA alone would need for the same MMAs.  A thread of the epilogue has
@@ -385,7 +398,7 @@ __device__ __forceinline__ void put(const MatmulParams& p, int64_t at, float v) 
     else reinterpret_cast<__half*>(p.y)[at] = Out<kF16>::of(v);
 }
 // (the channel's scale first: a token's may lie anywhere in fp32's range, and then only a result that does not fit overflows)
-__device__ __forceinline__ float scaled(int acc, float sw, float sx, float b) { return (float)acc * sw * sx + b; }
+__device__ __forceinline__ float scaled(int acc, float sw, float sx, float b) { return __fmaf_rn(__fmul_rn((float)acc, sw), sx, b); }
 __device__ __forceinline__ float relu2(float v) { v = v > 0.0f || v != v ? v : 0.0f; return v * v; }
 
 // what one thread needs of its weight row(s)
@@ -437,8 +450,8 @@ struct MatmulShared {
     uint64_t drain;
     uint32_t tmem_base;
     int failed;
-    float sx[2][256];
-    int row[2][256];
+    float sx[2][64];
+    int row[2][64];
 };
 
 template <int BN, bool DUAL>
@@ -459,6 +472,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
     const int total = (p.offsets ? group_table<BN>(p, table) : p.mt) * p.nt;
     if (first >= total) {   // (the whole cluster; nothing has been allocated)
         griddep_launch();
+        griddep_wait();   // (whoever waits for this grid has what lies before it as well)
         return;
     }
 
@@ -628,10 +642,12 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
             const int m = i >> 7, n = t.n0 + (i & 127);
             if (n >= p.N) continue;
             int acc = 0, up = 0;
-            for (int s = 0; s < S; ++s) {
-                acc += ld_cluster(cluster_addr(stages + 4 * i, s));
-                if (DUAL) up += ld_cluster(cluster_addr(stages + 4 * (i + BN * 128), s));
-            }
+#pragma unroll
+            for (int s = 0; s < 8; ++s)   // (all on their way at once)
+                if (s < S) {
+                    acc += ld_cluster(cluster_addr(stages + 4 * i, s));
+                    if (DUAL) up += ld_cluster(cluster_addr(stages + 4 * (i + BN * 128), s));
+                }
             const int64_t r = p.out_rows ? p.out_rows[t.row0 + m] : t.row0 + m;
             float o[2];
             finish2<DUAL>(p, channel(p, DUAL, t.expert, n), p.sx[t.row0 + m], 0.0f, acc, 0, up, 0, o);
@@ -640,6 +656,199 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
         cluster_sync();   // ... and has been read
     }
     if (tid == 0 && sh.failed && p.status) atomicOr(p.status, kStatusWaitTimeout);
+}
+
+// ---- a few tokens ----
+// Up to eight tokens at a time times 16 weight rows (or 16 of the gate and the same 16 of the up matrix) per warp, or per 2, 4 or 8 warps that share K in
+// pieces of 64 bytes, so that each has about four of them; the sums on the warp-level int8 MMA (m16n8k32), its K order that of the bytes a lane holds: 16 neighbouring ones of a weight row and the same 16 of a token's.
+// All of a warp's first weights are on their way before it looks at the tokens, which the CTA quantises itself (kI8: takes as they are): a call is one launch.
+// Bound: the weights' bytes, and what a launch takes.  y by the formula of the other kernels, the same bits.
+constexpr int kI8 = -2;                 // rows that are quantised already
+constexpr int kR_Threads = 256, kR_Warps = 8, kR_Tokens = 8, kR_Units = 4;   // units of 64 bytes of K that a warp has on their way
+constexpr int kR_MaxK = 8192;
+
+struct RowsParams {
+    MatmulParams m;
+    const void* x;
+    int64_t ldx, x_rows;
+    const int32_t* rows;       // or null
+    int rows_div, vec;
+    const int8_t* w;
+    int64_t ldw, w_plane;
+    int kw;                    // warps that share K
+    int ks;                    // bytes between tokens in shared memory: 64 modulo 128, so that neighbouring tokens lie in different banks
+};
+
+__device__ __forceinline__ void mma_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Grouped: blockIdx.y is a pair, whose CTAs take its expert if it is the expert's first.
+template <int TYPE, bool DUAL>
+__global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant__ RowsParams p) {
+    constexpr int TILES = DUAL ? 2 : 1;
+    extern __shared__ __align__(16) int8_t xs[];          // [token][ks]
+    __shared__ uint32_t s_max[kR_Tokens][kR_Warps];
+    __shared__ float s_scale[kR_Tokens];
+    __shared__ int red[kR_Warps][TILES][16][kR_Tokens + 1];
+    __shared__ int group[3];
+    const MatmulParams& mp = p.m;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int kw = p.kw, wk = warp & (kw - 1), outs = 16 * (kR_Warps / kw);
+    const int n0 = blockIdx.x * outs, K = mp.K, units = (K + 63) >> 6;
+    if (!mp.early) griddep_wait();
+    griddep_launch();
+    int e = 0, start = 0, end = mp.M;
+    if (mp.offsets) {
+        if (tid == 0) group[0] = -1;
+        __syncthreads();
+        for (int i = tid; i < mp.E; i += kR_Threads) {
+            const int a = min(max(mp.offsets[i], 0), mp.M), b = min(max(mp.offsets[i + 1], a), mp.M);
+            if (a == (int)blockIdx.y && b > a) { group[0] = i; group[1] = a; group[2] = b; }
+        }
+        __syncthreads();
+        e = group[0]; start = group[1]; end = group[2];
+        if (e < 0) { griddep_wait(); return; }   // (whoever waits for this grid has what lies before it as well)
+    }
+    // this lane's rows (behind the last one: the last one again, not stored)
+    const int8_t* wr[TILES][2];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int n = min(n0 + 16 * (warp / kw) + g + 8 * h, mp.N - 1) + i * mp.N;
+            wr[i][h] = p.w + e * p.w_plane + n * p.ldw + 16 * t;
+        }
+    uint4 v[kR_Units][TILES][2];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kR_Units; ++u) {
+            const int unit = base + wk + kw * u;
+            const bool in = unit < units && 64 * unit + 16 * t < K;
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v[u][i][h] = make_uint4(0, 0, 0, 0);
+                    if (in) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(v[u][i][h].x), "=r"(v[u][i][h].y), "=r"(v[u][i][h].z), "=r"(v[u][i][h].w) : "l"(wr[i][h] + 64 * unit));
+                }
+        }
+    };
+    load(0);
+    if (mp.early) griddep_wait();
+
+    for (int c0 = start; c0 < end; c0 += kR_Tokens) {
+        const int ntok = min(kR_Tokens, end - c0);
+        auto source = [&](int m) -> int64_t {
+            if (!p.rows) return c0 + m;
+            const int r = p.rows[c0 + m], s = r < 0 ? -1 : r / p.rows_div;
+            return s < p.x_rows ? s : -1;
+        };
+        if constexpr (TYPE == kI8) {
+            for (int m = 0; m < ntok; ++m) {
+                const int8_t* x = reinterpret_cast<const int8_t*>(p.x) + (int64_t)(c0 + m) * p.ldx;
+                for (int i = tid; i < 4 * units; i += kR_Threads) {
+                    uint4 q = make_uint4(0, 0, 0, 0);
+                    if (16 * i < K) q = __ldg(reinterpret_cast<const uint4*>(x) + i);
+                    uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {   // (nothing behind the row's last value)
+                        const int left = K - 16 * i - 4 * j;
+                        if (left < 4) w[j] = left <= 0 ? 0u : w[j] & (0xFFFFFFFFu >> (32 - 8 * left));
+                    }
+                    *reinterpret_cast<uint4*>(xs + m * p.ks + 16 * i) = q;
+                }
+                if (tid == 0) s_scale[m] = mp.sx[c0 + m];
+            }
+        } else {
+            using E = Elem<TYPE>;
+            const int nv = p.vec ? K >> 3 : 0;
+            for (int m = 0; m < ntok; ++m) {
+                const int64_t src = source(m);
+                uint32_t top = 0;
+                if (src >= 0) {
+                    const typename E::T* x = reinterpret_cast<const typename E::T*>(p.x) + src * p.ldx;
+                    for (int i = tid; i < nv; i += kR_Threads) top = E::top(E::load8(x + 8 * i), top);
+                    for (int i = 8 * nv + tid; i < K; i += kR_Threads) top = max(top, __float_as_uint(E::one(x + i)) & 0x7FFFFFFFu);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) s_max[m][warp] = top;
+            }
+            __syncthreads();
+            for (int m = 0; m < ntok; ++m) {
+                const int64_t src = source(m);
+                const uint32_t top = __reduce_max_sync(0xffffffffu, s_max[m][lane & (kR_Warps - 1)]);
+                const float amax = __uint_as_float(top);
+                int8_t* q = xs + m * p.ks;
+                for (int i = K + tid; i < 64 * units; i += kR_Threads) q[i] = 0;
+                if (src < 0 || top == 0u || top >= 0x7F800000u) {
+                    for (int i = tid; i < K; i += kR_Threads) q[i] = 0;
+                    if (tid == 0) s_scale[m] = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : 0.0f;
+                    continue;
+                }
+                const typename E::T* x = reinterpret_cast<const typename E::T*>(p.x) + src * p.ldx;
+                if (!RowScale::wide(amax)) {
+                    const float scale = fmaxf(amax / 127.0f, 1.17549435e-38f);
+#pragma unroll 1
+                    for (int i = tid; i < K; i += kR_Threads) q[i] = (int8_t)__float2int_rn(E::one(x + i) / scale);
+                    if (tid == 0) s_scale[m] = scale;
+                    continue;
+                }
+                const RowScale s(amax);
+                for (int i = tid; i < nv; i += kR_Threads) {
+                    const typename E::Raw w = E::load8(x + 8 * i);
+                    uint2 o;
+                    o.x = s.q4(E::value(w, 0), E::value(w, 1), E::value(w, 2), E::value(w, 3));
+                    o.y = s.q4(E::value(w, 4), E::value(w, 5), E::value(w, 6), E::value(w, 7));
+                    *reinterpret_cast<uint2*>(q + 8 * i) = o;
+                }
+                for (int i = 8 * nv + tid; i < K; i += kR_Threads) q[i] = (int8_t)s.q(E::one(x + i));
+                if (tid == 0) s_scale[m] = s.scale;
+            }
+        }
+        __syncthreads();
+
+        int acc[TILES][4] = {};
+        for (int base = 0; base < units; base += kw * kR_Units) {
+            if (base > 0 || c0 > start) load(base);
+#pragma unroll
+            for (int u = 0; u < kR_Units; ++u) {
+                const int unit = base + wk + kw * u;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (unit < units && g < ntok) x = *reinterpret_cast<const uint4*>(xs + g * p.ks + 64 * unit + 16 * t);
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    const uint4 a = v[u][i][0], b = v[u][i][1];
+                    mma_16832(acc[i], a.x, b.x, a.y, b.y, x.x, x.y);
+                    mma_16832(acc[i], a.z, b.z, a.w, b.w, x.z, x.w);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            red[warp][i][g][2 * t] = acc[i][0];
+            red[warp][i][g][2 * t + 1] = acc[i][1];
+            red[warp][i][g + 8][2 * t] = acc[i][2];
+            red[warp][i][g + 8][2 * t + 1] = acc[i][3];
+        }
+        __syncthreads();
+        for (int o = tid; o < outs * ntok; o += kR_Threads) {   // neighbouring threads: neighbouring outputs of a token
+            const int m = o / outs, c = o % outs, n = n0 + c;
+            if (n >= mp.N) continue;
+            int sum = 0, up = 0;
+            for (int w = c / 16 * kw; w < (c / 16 + 1) * kw; ++w) {
+                sum += red[w][0][c & 15][m];
+                if (DUAL) up += red[w][TILES - 1][c & 15][m];
+            }
+            float y[2];
+            finish2<DUAL>(mp, channel(mp, DUAL, e, n), s_scale[m], 0.0f, sum, 0, up, 0, y);
+            const int64_t r = mp.out_rows ? mp.out_rows[c0 + m] : c0 + m;
+            if (r >= 0 && r < mp.y_rows) put(mp, r * mp.ldy + n, y[0]);
+        }
+        __syncthreads();
+    }
 }
 
 // ---- many tokens ----
@@ -738,6 +947,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
     const int total = (p.offsets ? group_table<kW_Tokens>(p, table) : p.mt) * p.nt;
     if (first >= total) {   // (both CTAs; nothing has been allocated)
         griddep_launch();
+        griddep_wait();   // (whoever waits for this grid has what lies before it as well)
         return;
     }
     if (tid == 0) {
@@ -1001,52 +1211,119 @@ int64_t token_tiles(const MatmulCall& c, int bn) {
     return c.p.offsets ? c.p.M / bn + (c.p.M < c.p.E ? c.p.M : c.p.E) : (c.p.M + bn - 1) / bn;
 }
 
+// warps of a CTA that share K: as many as have kR_Units units each
+int rows_warps(int K) {
+    int kw = 1;
+    while (kw < kR_Warps && kw * kR_Units * 64 < K) kw *= 2;
+    return kw;
+}
+int rows_outs(int K) { return 16 * (kR_Warps / rows_warps(K)); }
+
+template <int TYPE, bool DUAL>
+int launch_rows(const MatmulCall& c, const QuantParams* x, bool pdl, cudaStream_t stream) {
+    static bool done[64];
+    RowsParams r{};
+    r.m = c.p;
+    r.x = x ? x->x : c.x;
+    r.ldx = x ? x->ldx : c.ldx;
+    if (x) { r.x_rows = x->x_rows; r.rows = x->rows; r.rows_div = x->rows_div; r.vec = x->vec; }
+    r.w = c.w; r.ldw = c.ldw; r.w_plane = c.w_plane;
+    const int units = (c.p.K + 63) / 64, tokens = c.p.M < kR_Tokens ? c.p.M : kR_Tokens;
+    r.ks = 64 * (units | 1);
+    r.kw = rows_warps(c.p.K);
+    const int outs = rows_outs(c.p.K);
+    auto kernel = rows_kernel<TYPE, DUAL>;
+    cudaError_t e = max_smem_once(kernel, kR_Tokens * 64 * (kR_MaxK / 64 + 1), done);
+    if (e != cudaSuccess) return -(100 + (int)e);
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = launch_config((c.p.N + outs - 1) / outs, (size_t)tokens * r.ks, 1, pdl, stream, attr);
+    cfg.blockDim = dim3(kR_Threads);
+    cfg.gridDim.y = c.p.offsets ? c.p.M : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, r);
+    return e == cudaSuccess ? 0 : -(100 + (int)e);
+}
+template <int TYPE>
+int launch_rows_type(const MatmulCall& c, const QuantParams* x, bool pdl, cudaStream_t stream) {
+    return c.dual ? launch_rows<TYPE, true>(c, x, pdl, stream) : launch_rows<TYPE, false>(c, x, pdl, stream);
+}
+// x null: rows that are quantised already
+int launch_rows_any(const MatmulCall& c, const QuantParams* x, int x_type, bool pdl, cudaStream_t stream) {
+    if (!x) return launch_rows_type<kI8>(c, x, pdl, stream);
+    return x_type == kF32 ? launch_rows_type<kF32>(c, x, pdl, stream) : x_type == kF16 ? launch_rows_type<kF16>(c, x, pdl, stream) : launch_rows_type<kBF16>(c, x, pdl, stream);
+}
+// Batches for the kernel of a few tokens: dense ones of up to four (4096 x 2048, us, this / tensor-core tiles: 1 token 4.4 / 6.1, 4: 5.1 / 6.1, 6: 5.9 / 6.1; 2048 x
+// 4096 6: 6.9 / 6.9; 4096 x 8192 3: 11.9 / 11.9, 6: 17.3 / 12.1).  Grouped ones while their CTAs, if every pair has a group of its own, are four per SM at most (experts of 512 x 2048,
+// both products, 8 pairs 12.3 / 18.4, 16: 20.5 / 20.5, 32: 34 / 27; of 1856 x 2688 6 pairs, 696 and 1008 CTAs, 24.6 / 20.6; of 2048 x 2048 4 pairs 21 / 25, 8: 31 / 26).
+constexpr int kR_DenseTokens = 4, kR_MaxCtas = 4 * 148;
+bool few_tokens(const MatmulCall& c) {
+    if (c.p.K > kR_MaxK) return false;
+    return c.p.offsets ? (int64_t)c.p.M * ((c.p.N + rows_outs(c.p.K) - 1) / rows_outs(c.p.K)) <= kR_MaxCtas : c.p.M <= kR_DenseTokens;
+}
+// ... whose CTAs quantise the tokens themselves: dense, up to so many values and two CTAs per SM (4096 x 2048 1 token 4.9 against 5.4 with a launch in front,
+// 8192 x 4096 12.3 against 10.2; 4096 x 2048 3 tokens 6.4 against 5.9).
+constexpr int64_t kR_Values = 4096;
+bool few_values(int64_t M, int N, int K) { return M <= kR_DenseTokens && K <= kR_MaxK && M * K <= kR_Values && (N + rows_outs(K) - 1) / rows_outs(K) <= 2 * 148; }
+bool few_values(const MatmulCall& c) { return few_tokens(c) && (c.p.offsets || few_values(c.p.M, c.p.N, c.p.K)); }
+
 int launch_matmul(const MatmulCall& c, bool pdl, cudaStream_t stream) {
     if (c.p.M == 0) return 0;
+    if (few_tokens(c)) return launch_rows_any(c, nullptr, 0, pdl, stream);
     if (!encoder()) return -6;
-    const int64_t nt = (c.p.N + 127) / 128;
     const int sms = sm_count();
-    // Width of the token tiles.  Cycles per 128 of K: the MMAs (2.1 per column and block of weight rows), or the tile's bytes through L2.
-    const int widest = c.dual ? 128 : 256;
-    int bn = 16;
-    double best = 1e30;
-    const int64_t per = c.p.offsets ? (c.p.M + c.p.E - 1) / c.p.E : c.p.M, of = c.p.offsets ? c.p.E : 1;   // (grouped: of an even load)
-    for (int b = 16; b <= widest; b *= 2) {
-        const double mma = 2.1 * b * (c.dual ? 2 : 1), load = (16384.0 * (c.dual ? 2 : 1) + 128.0 * b) / 50.0;
-        const int64_t tiles = of * ((per + b - 1) / b) * nt;
-        const double cost = (double)((tiles + sms - 1) / sms) * (mma > load ? mma : load);
-        if (cost < best) { best = cost; bn = b; }
+    // Pairs of CTAs: dense batches of more than 128 tokens with sixteen tiles or more, grouped ones of 32 tokens per group or more on average.
+    const int outs = c.dual ? 128 : 256;
+    const int64_t wide = token_tiles(c, kW_Tokens) * ((c.p.N + outs - 1) / outs);
+    if (c.p.offsets ? c.p.M >= 32 * (int64_t)c.p.E : c.p.M > 128 && wide >= 16) {
+        if (wide > 0x3FFFFFFF) return -2;
+        switch (c.p.y_type) {
+            case kF32: return c.dual ? launch_wide<kF32, true>(c, wide, pdl, stream) : launch_wide<kF32, false>(c, wide, pdl, stream);
+            case kF16: return c.dual ? launch_wide<kF16, true>(c, wide, pdl, stream) : launch_wide<kF16, false>(c, wide, pdl, stream);
+            default: return c.dual ? launch_wide<kBF16, true>(c, wide, pdl, stream) : launch_wide<kBF16, false>(c, wide, pdl, stream);
+        }
     }
-    {   // a pair's tile: 256 x 256 in the time of its MMAs
-        const int outs = c.dual ? 128 : 256;
-        const int64_t wide = of * ((per + kW_Tokens - 1) / kW_Tokens) * ((c.p.N + outs - 1) / outs);
-        if (per > 64 && (double)((wide + sms / 2 - 1) / (sms / 2)) * 2.1 * 256 * 1.2 < best) {
-            const int64_t tiles = token_tiles(c, kW_Tokens) * ((c.p.N + outs - 1) / outs);
-            if (tiles > 0x3FFFFFFF) return -2;
-            switch (c.p.y_type) {
-                case kF32: return c.dual ? launch_wide<kF32, true>(c, tiles, pdl, stream) : launch_wide<kF32, false>(c, tiles, pdl, stream);
-                case kF16: return c.dual ? launch_wide<kF16, true>(c, tiles, pdl, stream) : launch_wide<kF16, false>(c, tiles, pdl, stream);
-                default: return c.dual ? launch_wide<kBF16, true>(c, tiles, pdl, stream) : launch_wide<kBF16, false>(c, tiles, pdl, stream);
+    // Width of the token tiles and the CTAs that share one.
+    const int64_t nt = (c.p.N + 127) / 128;
+    const int nkb = (c.p.K + kMM_KBytes - 1) / kMM_KBytes;
+    int bn = 16, split = 1;
+    if (c.p.offsets) {
+        bn = c.p.M < c.p.E ? 16 : c.p.M < 4 * (int64_t)c.p.E ? 32 : 64;
+        while (split < 8 && token_tiles(c, bn) * nt * split * 2 <= sms && split * 4 <= nkb) split *= 2;
+    } else {
+        // cycles: a stage is its bytes through L2 (50 per cycle); a tile's results, and with a shared tile the exchange of its parts
+        double best = 1e30;
+        for (int b = 16; b <= 64; b *= 2) {
+            const int64_t tiles = (int64_t)(c.p.M + b - 1) / b * nt;
+            const int tokens = c.p.M < b ? c.p.M : b;
+            for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= sms && s * 2 <= nkb)); s *= 2) {
+                const double stage = (16384.0 * (c.dual ? 2 : 1) + 128.0 * b) / 50.0, tail = s > 1 ? 1200.0 + 20.0 * tokens : 25.0 * tokens;
+                const double cost = (double)((tiles * s + sms - 1) / sms) * ((nkb + s - 1) / s * stage + tail);
+                if (cost < best) { best = cost; bn = b; split = s; }
             }
         }
     }
     const int64_t tiles = token_tiles(c, bn) * nt;
     if (tiles > 0x3FFFFFFF) return -2;
-    int split = 1;
-    const int nkb = (c.p.K + kMM_KBytes - 1) / kMM_KBytes;
-    if (bn <= 64)
-        while (split < 8 && tiles * split * 2 <= sms && split * 4 <= nkb) split *= 2;
     switch (bn + (c.dual ? 1 : 0)) {
         case 16: return launch_tile<16, false>(c, (int)tiles, split, pdl, stream);
         case 32: return launch_tile<32, false>(c, (int)tiles, split, pdl, stream);
         case 64: return launch_tile<64, false>(c, (int)tiles, split, pdl, stream);
-        case 128: return launch_tile<128, false>(c, (int)tiles, split, pdl, stream);
-        case 256: return launch_tile<256, false>(c, (int)tiles, split, pdl, stream);
         case 17: return launch_tile<16, true>(c, (int)tiles, split, pdl, stream);
         case 33: return launch_tile<32, true>(c, (int)tiles, split, pdl, stream);
-        case 65: return launch_tile<64, true>(c, (int)tiles, split, pdl, stream);
-        default: return launch_tile<128, true>(c, (int)tiles, split, pdl, stream);
+        default: return launch_tile<64, true>(c, (int)tiles, split, pdl, stream);
     }
+}
+
+// Rows of f32, f16 or bf16 times a matrix: quantised in the product's own CTAs where that is little, else by a kernel in front.  `first`: nothing of this
+// call has been launched before.
+int launch_linear(MatmulCall c, QuantParams x, int x_type, bool first, cudaStream_t stream) {
+    x.vec = ((uintptr_t)x.x & 15) == 0 && (x.ldx * (x_type == kF32 ? 4 : 2)) % 16 == 0;
+    c.p.early = !first;
+    if (few_values(c)) return launch_rows_any(c, &x, x_type, !first, stream);
+    if (!few_tokens(c) && !encoder()) return -6;
+    const cudaError_t e = launch_quantize(x, x_type, stream, !first);
+    if (e != cudaSuccess) return -(100 + (int)e);
+    c.p.early = true;
+    return launch_matmul(c, true, stream);
 }
 
 // ------------------------------------------------------------------ checks ----
@@ -1130,32 +1407,31 @@ int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float
     return launch_matmul(matmul_call(d_x, ldx, d_x_scale, d_w, ldw, stride_w, d_w_scale, d_bias, d_offsets, E, M, N, K, act, d_y, y_type, ldy, y_rows, d_out_rows, d_status, false), false, stream);
 }
 
-size_t chimere_b200_linear_w8a8_bytes(int64_t M, int K) {
-    if (M < 0 || M > 0x7FFFFFFF || K <= 0 || K > kMaxK) return 0;
-    return rows_bytes(M, K) + 256;
+int64_t chimere_b200_linear_w8a8_bytes(int64_t M, int N, int K) {
+    if (M < 0 || M > 0x7FFFFFFF || N <= 0 || K <= 0 || K > kMaxK) return -2;
+    return M == 0 || few_values(M, N, K) ? 0 : (int64_t)rows_bytes(M, K);
 }
 
 int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias, int64_t M, int N, int K,
                              int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes, int32_t* d_status, cudaStream_t stream) {
     Carver ws{(uint8_t*)d_ws, 0};
-    int8_t* q = (int8_t*)ws.take((size_t)(M < 0 ? 0 : M) * up16(K));
-    float* scale = (float*)ws.take((size_t)(M < 0 ? 0 : M) * 4);
-    if (M > 0 && !d_ws) return -1;
+    const bool none = few_values(M, N, K);      // (no scratch; the pointers below are not used then)
+    int8_t* q = none ? (int8_t*)256 : (int8_t*)ws.take((size_t)(M < 0 ? 0 : M) * up16(K));
+    float* scale = none ? (float*)256 : (float*)ws.take((size_t)(M < 0 ? 0 : M) * 4);
+    if (M > 0 && !none && !d_ws) return -1;
     if (misaligned(d_ws, 256)) return -5;
     int rc = check_quantize(d_x, x_type, ldx, M, nullptr, 1, M, K, q, up16(K), scale);
     if (rc) return rc;
     rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
     if (rc || M == 0) return rc;
     if (ws_bytes < ws.at) return -4;
-    if (!encoder()) return -6;
-    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, stream, false));
-    if (rc) return rc;
-    return launch_matmul(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, true), true, stream);
+    return launch_linear(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, false),
+                         QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, true, stream);
 }
 
-size_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F) {
-    if (pairs < 0 || pairs > 0x7FFFFFFF || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return 0;
-    return rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up8(F) * 4) + 256;
+int64_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F) {
+    if (pairs < 0 || pairs > 0x7FFFFFFF || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return -2;
+    return (int64_t)(rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up8(F) * 4));
 }
 
 int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
@@ -1181,15 +1457,12 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
     rc = check_matmul(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm);
     if (rc || P == 0) return rc;
     if (ws_bytes < ws.at) return -4;
-    if (!encoder()) return -6;
-    rc = rc_of(launch_quantize(QuantParams{d_x, ldx, T, d_perm, top_k, H, q, up16(H), scale, P, 0}, x_type, stream, false));
+    rc = launch_linear(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up8(F), P, nullptr, d_status, false),
+                       QuantParams{d_x, ldx, T, d_perm, top_k, H, q, up16(H), scale, P, 0}, x_type, true, stream);
     if (rc) return rc;
-    rc = launch_matmul(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up8(F), P, nullptr, d_status, true), true, stream);
-    if (rc) return rc;
-    rc = rc_of(launch_quantize(QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, P, 0}, kF32, stream, true));
-    if (rc) return rc;
-    return launch_matmul(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm,
-                                     d_status, true), true, stream);
+    return launch_linear(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm,
+                                     d_status, false),
+                         QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, P, 0}, kF32, false, stream);
 }
 
 }  // extern "C"

@@ -388,9 +388,9 @@ int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float
                                      int act, void* d_y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* d_out_rows,
                                      int32_t* d_status, cudaStream_t stream);
 
-/* quantize_i8 of the M rows of x and matmul_w8a8 in one call.  d_ws: scratch of at least linear_w8a8_bytes(M, K), 256-byte aligned, used by no other call
- * at the same time (0 from the size function: bad arguments). */
-size_t chimere_b200_linear_w8a8_bytes(int64_t M, int K);
+/* quantize_i8 of the M rows of x and matmul_w8a8 in one call (a token or two: one launch).  d_ws: scratch of at least linear_w8a8_bytes(M, N, K), 256-byte aligned, used by
+ * no other call at the same time; the size function returns 0 where the call needs none (d_ws may be NULL then) and an error below 0. */
+int64_t chimere_b200_linear_w8a8_bytes(int64_t M, int N, int K);
 int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,
                              int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes,
                              int32_t* d_status, cudaStream_t stream);
@@ -399,7 +399,7 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
  * of d_perm (d_offsets[e] .. d_offsets[e + 1]) holds the pair; d_perm and d_offsets as chimere_b200_moe_route / _permute leave them.  The rows between the two products
  * are held in f32 and quantised by token again.  w_up [E][2 F (SWIGLU: gate rows, then up) or F (RELU2)][H], w_down [E][H][F].  Rows of y whose pair is in no expert's range are
  * not written.  Scratch as above. */
-size_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F);
+int64_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F);
 int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
                               const int8_t* d_w_up, int64_t ld_up, int64_t stride_up, const float* d_up_scale,
                               const int8_t* d_w_down, int64_t ld_down, int64_t stride_down, const float* d_down_scale,

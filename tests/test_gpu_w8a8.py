@@ -134,7 +134,7 @@ def test_quantize_rows_of_a_wider_matrix_and_gathered(dtype):
 
 
 # ---- dense ----
-SHAPES = [(1, 1, 1), (1, 2048, 4096), (2, 128, 128), (3, 129, 5), (7, 2688, 3712), (16, 512, 100), (17, 100, 130), (33, 2005, 257), (61, 4096, 2048), (64, 64, 64),
+SHAPES = [(1, 1, 1), (1, 2048, 4096), (8, 2688, 96), (5, 8192, 70), (5, 8193, 70), (8, 65, 33), (4, 4100, 515), (9, 2048, 4096), (2, 128, 128), (3, 129, 5), (7, 2688, 3712), (16, 512, 100), (17, 100, 130), (33, 2005, 257), (61, 4096, 2048), (64, 64, 64),
           (65, 300, 700), (129, 1000, 513), (300, 640, 1000), (777, 2005, 1031), (1500, 384, 2500), (5000, 130, 260), (4000, 2048, 2048), (2300, 1000, 1024), (1111, 640, 4099), (20000, 64, 320)]
 
 
@@ -196,7 +196,7 @@ def groups(counts, first=0):
 
 
 @pytest.mark.parametrize("act", [abi.ACT_NONE, abi.ACT_SWIGLU, abi.ACT_RELU2])
-@pytest.mark.parametrize("counts,K,N", [([1], 64, 64), ([0, 0, 3, 0], 100, 33), ([1, 1, 1, 1, 1, 1, 1, 1], 2048, 512), ([16, 17, 0, 15, 33], 257, 130), ([300, 0, 1, 129, 64], 512, 260),
+@pytest.mark.parametrize("counts,K,N", [([1], 64, 64), ([0, 0, 3, 0], 100, 33), ([1, 1, 1, 1, 1, 1, 1, 1], 2048, 512), ([0] * 30 + [19, 1, 0, 8, 9], 2048, 100), ([2, 0, 0, 1], 9000, 50), ([16, 17, 0, 15, 33], 257, 130), ([300, 0, 1, 129, 64], 512, 260),
                                         ([0] * 100 + [5] + [0] * 900 + [7], 128, 40), ([2000, 3, 700], 384, 200), ([40] * 64, 640, 192)])
 def test_grouped(counts, K, N, act):
     g = gen(K + N + len(counts))
@@ -271,7 +271,7 @@ def test_stack_inside_a_wider_one():
 
 # ---- the chains ----
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,K,N,act", [(1, 2048, 4096, abi.ACT_NONE), (5, 77, 130, abi.ACT_SWIGLU), (200, 1000, 640, abi.ACT_RELU2), (1025, 512, 300, abi.ACT_NONE)])
+@pytest.mark.parametrize("M,K,N,act", [(1, 2048, 4096, abi.ACT_NONE), (5, 77, 130, abi.ACT_SWIGLU), (8, 3000, 515, abi.ACT_RELU2), (8, 8190, 64, abi.ACT_NONE), (3, 8192, 130, abi.ACT_SWIGLU), (1, 20000, 64, abi.ACT_NONE), (200, 1000, 640, abi.ACT_RELU2), (1025, 512, 300, abi.ACT_NONE)])
 def test_linear_is_its_two_steps(M, K, N, act, dtype):
     g = gen(M + K)
     R = 2 * N if act == abi.ACT_SWIGLU else N
@@ -320,6 +320,45 @@ def test_experts_behind_the_router(cfg, T):
 
 
 # ---- streams, graphs, nothing to do ----
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_of_rows_at_the_ends_of_the_range(dtype):
+    """What a batch of a few tokens quantises itself: the same rows, the same bits."""
+    g = gen(21)
+    x = torch.randn(8, 333, generator=g, device="cuda")
+    x[1], x[2], x[3, 5], x[4, 332] = 0, x[2] * 1e-30, float("inf"), float("nan")
+    wide = torch.zeros(8, 340, device="cuda").to(dtype)
+    wide[:, 3:336] = x.to(dtype)
+    w, sw = i8(g, 50, 333), scales(g, 50)
+    for rows in (x.to(dtype), wide[:, 3:336]):
+        q, s = w8a8.quantize_i8(rows)
+        rq, rs = quantized(rows)
+        assert torch.equal(q, rq) and same(s, rs)
+        y = w8a8.linear_w8a8(rows, w, sw, out_dtype=torch.float32)
+        assert same(y, w8a8.matmul_w8a8(q, s, w, sw)) and torch.isnan(y[3:5]).all() and (y[1] == 0).all()
+        ok = [0, 1, 2, 5, 6, 7]
+        check(y[ok], *product(q[ok], s[ok], w, sw, None, abi.ACT_NONE, torch.float32))
+
+
+def test_experts_with_ids_outside_the_rows():
+    """A permutation entry that is no pair: a row of zeros goes in, and nothing comes out for it."""
+    g = gen(22)
+    for T, E in ((6, 32), (200, 4)):
+        H, F, k = 160, 64, 2
+        x = torch.randn(T, H, generator=g, device="cuda")
+        perm = torch.randperm(T * k, generator=g, device="cuda").to(torch.int32)
+        off = groups([T * k // E] * (E - 1) + [T * k - (E - 1) * (T * k // E)])
+        wu, su, wd, sd = i8(g, E, 2 * F, H), scales(g, E, 2 * F) * 0.05, i8(g, E, H, F), scales(g, E, H) * 0.05
+        want = w8a8.experts_w8a8(x, perm, off, k, wu, su, wd, sd)
+        bad = perm.clone()
+        bad[0], bad[3], bad[5] = -1, T * k, -2 ** 31
+        out = torch.full_like(want, 7.0)
+        w8a8.experts_w8a8(x, bad, off, k, wu, su, wd, sd, out=out)
+        lost = perm[[0, 3, 5]].long()
+        keep = torch.ones(T * k, dtype=torch.bool, device="cuda")
+        keep[lost] = False
+        assert torch.equal(out[keep], want[keep]) and (out[lost] == 7).all()
+
+
 def test_capture_and_replay_with_new_inputs():
     g = gen(6)
     x, w, sw = torch.randn(12, 500, generator=g, device="cuda"), i8(g, 300, 500), scales(g, 300)

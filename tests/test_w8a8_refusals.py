@@ -24,7 +24,7 @@ def grouped(lib, x=A, w=A, ldw=64, stride=2048, offsets=A, E=3, M=4, N=32, K=64,
     return lib.chimere_b200_matmul_w8a8_grouped(x, 64, A, w, ldw, stride, A, None, offsets, E, M, N, K, act, A, abi.TYPE_F32, ldy, y_rows, out_rows, None, None)
 
 
-def linear(lib, x=A, ldx=64, M=4, N=32, K=64, ws=A, nbytes=1 << 20, w=A):
+def linear(lib, x=A, ldx=64, M=40, N=32, K=64, ws=A, nbytes=1 << 20, w=A):
     return lib.chimere_b200_linear_w8a8(x, abi.TYPE_BF16, ldx, w, 64, A, None, M, N, K, abi.ACT_NONE, A, abi.TYPE_BF16, N, ws, nbytes, None, None)
 
 
@@ -66,7 +66,9 @@ def test_experts(lib, want, kw):
 
 
 def test_scratch_sizes(lib):
-    assert lib.chimere_b200_linear_w8a8_bytes(-1, 64) == 0 and lib.chimere_b200_linear_w8a8_bytes(4, 0) == 0 and lib.chimere_b200_linear_w8a8_bytes(4, 131072) == 0
-    assert lib.chimere_b200_linear_w8a8_bytes(4, 2005) >= 4 * 2016 + 16
-    assert lib.chimere_b200_experts_w8a8_bytes(8, 64, 0) == 0
-    assert lib.chimere_b200_experts_w8a8_bytes(8, 64, 33) >= 8 * (64 + 4 + 48 + 4 + 33 * 4)
+    linear, experts = lib.chimere_b200_linear_w8a8_bytes, lib.chimere_b200_experts_w8a8_bytes
+    assert linear(-1, 32, 64) == -2 and linear(4, 32, 0) == -2 and linear(4, 32, 131072) == -2 and linear(4, 0, 64) == -2
+    assert linear(0, 32, 64) == 0 and linear(1, 4096, 2048) == 0            # one launch: no scratch
+    assert linear(9, 32, 2005) >= 9 * (2016 + 4) and linear(1, 32, 20000) >= 20004 and linear(70000, 32, 131071) >= 70000 * 131076
+    assert experts(8, 64, 0) == -2 and experts(-1, 64, 64) == -2
+    assert experts(8, 64, 33) >= 8 * (64 + 4 + 48 + 4 + 33 * 4)
