@@ -113,10 +113,10 @@ PROTOTYPES = {
     "chimere_b200_matmul_w8a8_grouped": (C.c_int, [_P, _L, _P, _P, _L, _L, _P, _P, _P, C.c_int, _L, C.c_int, C.c_int, C.c_int, _P, C.c_int, _L, _L, _P, _P, _P]),
     "chimere_b200_linear_w8a8_bytes": (_L, [_L, C.c_int, C.c_int]),
     "chimere_b200_linear_w8a8": (C.c_int, [_P, C.c_int, _L, _P, _L, _P, _P, _L, C.c_int, C.c_int, C.c_int, _P, C.c_int, _L, _P, C.c_size_t, _P, _P]),
-    "chimere_b200_experts_w8a8_bytes": (_L, [_L, C.c_int, C.c_int]),
+    "chimere_b200_experts_w8a8_bytes": (_L, [_L, C.c_int, C.c_int, C.c_int]),
     "chimere_b200_experts_w8a8": (C.c_int, [_P, C.c_int, _L, _L, _P, _P, C.c_int, C.c_int, _P, _L, _L, _P, _P, _L, _L, _P, C.c_int, C.c_int, C.c_int,
                                             _P, C.c_int, _L, _P, C.c_size_t, _P, _P]),
-    "chimere_b200_balance_loss_bytes": (C.c_size_t, [_L, _L, C.c_int, C.c_int]),
+    "chimere_b200_balance_loss_bytes": (_L, [_L, _L, C.c_int, C.c_int]),
     "chimere_b200_balance_loss": (C.c_int, [_P, C.c_int, _L, _L, _P, _P, _L, _L, C.c_int, C.c_int, C.c_int, C.c_float, _P, _P, _P, _P, _P, _P, _L, _L, _P, C.c_size_t, _P]),
     "chimere_b200_balance_loss_backward": (C.c_int, [_P, C.c_int, _L, _L, _P, _P, _P, _L, _L, C.c_int, C.c_int, C.c_int, C.c_float, _P, _P, _L, _L, _P]),
     "chimere_b200_rmsnorm": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_float, _P]),

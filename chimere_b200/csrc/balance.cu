@@ -564,7 +564,7 @@ inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 struct Scratch { size_t count_part, part, group_part, counters, total; };
 Scratch scratch_of(const Plan& r, int64_t S, int E) {
     Scratch a{};
-    if (r.count_pieces == 0) { a.total = 256; return a; }
+    if (r.count_pieces == 0) return a;
     size_t o = 0;
     a.group_part = o; o += up256((size_t)S * groups_of(r.pieces) * E * 8);
     a.part = o; o += up256((size_t)S * r.pieces * E * 4);
@@ -597,9 +597,9 @@ using namespace chimere;
 
 extern "C" {
 
-size_t chimere_b200_balance_loss_bytes(int64_t S, int64_t L, int E, int top_k) {
-    if (check_dims(S, L, E, top_k, CHIMERE_ROUTE_SOFTMAX_RENORM, CHIMERE_TYPE_F32, E, 0)) return 0;
-    return S == 0 ? 256 : scratch_of(plan_of(S, (int)L, top_k), S, E).total;
+int64_t chimere_b200_balance_loss_bytes(int64_t S, int64_t L, int E, int top_k) {
+    const int rc = check_dims(S, L, E, top_k, CHIMERE_ROUTE_SOFTMAX_RENORM, CHIMERE_TYPE_F32, E, 0);
+    return rc ? rc : S == 0 ? 0 : (int64_t)scratch_of(plan_of(S, (int)L, top_k), S, E).total;
 }
 
 int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_t stride_s, const int32_t* d_topk_idx, const uint8_t* d_mask, int64_t S, int64_t L, int E,
@@ -609,16 +609,17 @@ int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_
     if (rc) return rc;
     if (d_grad_logits && (ld_grad < E || (S > 1 && stride_grad_s < (L > 0 ? (L - 1) * ld_grad + E : 0)))) return -2;
     if (S == 0) return 0;
-    if (!d_loss || !d_counts || !d_prob || !d_tokens || !d_ws || (L > 0 && (!d_logits || !d_topk_idx))) return -1;
+    if (!d_loss || !d_counts || !d_prob || !d_tokens || (L > 0 && (!d_logits || !d_topk_idx))) return -1;
     const int size = type == CHIMERE_TYPE_F32 ? 4 : 2;
     if (misaligned(d_ws, 256) || misaligned(d_logits, size) || misaligned(d_grad_logits, size) || misaligned(d_topk_idx, 4) || misaligned(d_loss, 4) || misaligned(d_counts, 4) ||
         misaligned(d_prob, 4) || misaligned(d_tokens, 4) || misaligned(d_grad_loss, 4)) return -5;
     const Plan plan = plan_of(S, (int)L, top_k);
     const Scratch a = scratch_of(plan, S, E);
+    if (a.total && !d_ws) return -1;
     if (ws_bytes < a.total) return -4;
     uint8_t* ws = (uint8_t*)d_ws;
     BalanceParams p{};
-    p.logits = d_logits; p.ld = ld; p.stride_s = stride_s; p.ids = d_topk_idx ? d_topk_idx : (const int32_t*)d_ws; p.mask = d_mask;
+    p.logits = d_logits; p.ld = ld; p.stride_s = stride_s; p.ids = d_topk_idx ? d_topk_idx : d_counts;   /* (no tokens: not read) */ p.mask = d_mask;
     p.S = (int)S; p.L = (int)L; p.E = E; p.k = top_k; p.mode = route_mode; p.coef = coef;
     p.loss = d_loss; p.counts = d_counts; p.prob = d_prob; p.tokens = d_tokens;
     p.d_loss = d_grad_loss; p.d_logits = d_grad_logits; p.ldd = ld_grad; p.stride_ds = stride_grad_s;

@@ -163,6 +163,30 @@ __global__ void __launch_bounds__(GROUP ? 256 : 1024) quantize_rows_kernel(Quant
     for (int i = ones + tid; i < p.K; i += nt) q[i] = (int8_t)s.q(E::one(x + i));
 }
 
+// Row i of (q, scale) = row rows[i] / rows_div of (from, from_scale), a warp each; 16 bytes at a time (what lies behind a row's K values goes along).
+__global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* from, const float* from_scale, int64_t from_rows, const int32_t* rows, int rows_div, int8_t* q, float* scale,
+                                                          int64_t M, int64_t ld) {
+    griddep_wait();
+    griddep_launch();
+    const int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    if (i >= M) return;
+    const int32_t r = rows[i];
+    const int64_t src = r < 0 ? -1 : r / rows_div;
+    const bool there = src >= 0 && src < from_rows;
+    const uint4* a = reinterpret_cast<const uint4*>(from + (there ? src : 0) * ld);
+    uint4* b = reinterpret_cast<uint4*>(q + i * ld);
+    const int n = (int)(ld / 16);
+    for (int j = lane; j < n; j += 128) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = j + 32 * u < n && there ? __ldg(a + j + 32 * u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) if (j + 32 * u < n) b[j + 32 * u] = v[u];
+    }
+    if (lane == 0) scale[i] = there ? from_scale[src] : 0.0f;
+}
+
 template <int TYPE>
 cudaError_t launch_quantize_type(const QuantParams& p, cudaStream_t stream, bool pdl) {
     auto go = [&](auto kernel, int64_t grid, int nt) -> cudaError_t {
@@ -311,6 +335,12 @@ __device__ __forceinline__ int ld_cluster(uint32_t addr) {
     int v;
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
+}
+__device__ __forceinline__ void ld_cluster4(uint32_t addr, int (&sum)[4]) {   // added to four sums
+    int v[4];
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += v[i];
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
@@ -638,20 +668,25 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
         cluster_sync();   // every part is there
         bool bad = false;
         for (int s = 0; s < S; ++s) bad |= ld_cluster(cluster_addr(smem_u32(&sh.failed), s)) != 0;
-        for (int i = rank * kMM_Threads + tid; i < t.ntok * 128; i += S * kMM_Threads) {
-            const int m = i >> 7, n = t.n0 + (i & 127);
+        for (int i = rank * kMM_Threads + tid; i < t.ntok * 32; i += S * kMM_Threads) {   // four neighbouring results
+            const int m = i >> 5, n = t.n0 + 4 * (i & 31);
             if (n >= p.N) continue;
-            int acc = 0, up = 0;
+            int acc[4] = {}, up[4] = {};
 #pragma unroll
             for (int s = 0; s < 8; ++s)   // (all on their way at once)
                 if (s < S) {
-                    acc += ld_cluster(cluster_addr(stages + 4 * i, s));
-                    if (DUAL) up += ld_cluster(cluster_addr(stages + 4 * (i + BN * 128), s));
+                    ld_cluster4(cluster_addr(stages + 16 * i, s), acc);
+                    if (DUAL) ld_cluster4(cluster_addr(stages + 16 * (i + BN * 32), s), up);
                 }
             const int64_t r = p.out_rows ? p.out_rows[t.row0 + m] : t.row0 + m;
-            float o[2];
-            finish2<DUAL>(p, channel(p, DUAL, t.expert, n), p.sx[t.row0 + m], 0.0f, acc, 0, up, 0, o);
-            if (r >= 0 && r < p.y_rows) put(p, r * p.ldy + n, bad ? __uint_as_float(0x7FC00000u) : o[0]);
+            const float sx = p.sx[t.row0 + m];
+            if (r < 0 || r >= p.y_rows) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float o[2];
+                finish2<DUAL>(p, channel(p, DUAL, t.expert, n + j), sx, 0.0f, acc[j], 0, up[j], 0, o);
+                if (n + j < p.N) put(p, r * p.ldy + n + j, bad ? __uint_as_float(0x7FC00000u) : o[0]);
+            }
         }
         cluster_sync();   // ... and has been read
     }
@@ -1313,14 +1348,25 @@ int launch_matmul(const MatmulCall& c, bool pdl, cudaStream_t stream) {
     }
 }
 
+// A batch's pairs share rows: from so many values on each row is quantised once and copied to its pairs (32768 pairs of 2048 values, eight per row, bf16: 37 us when each pair
+// quantises its own, NN so).
+constexpr int64_t kGatherValues = 1 << 22;
+bool gather_apart(int64_t pairs, int top_k, int K) { return top_k > 1 && pairs * K >= kGatherValues; }
+
 // Rows of f32, f16 or bf16 times a matrix: quantised in the product's own CTAs where that is little, else by a kernel in front.  `first`: nothing of this
 // call has been launched before.
-int launch_linear(MatmulCall c, QuantParams x, int x_type, bool first, cudaStream_t stream) {
+// `apart` (with x.rows): scratch for the x_rows rows of x and their scales, quantised once and copied; null: each row of the product quantises its own.
+int launch_linear(MatmulCall c, QuantParams x, int x_type, bool first, int8_t* apart, float* apart_scale, cudaStream_t stream) {
     x.vec = ((uintptr_t)x.x & 15) == 0 && (x.ldx * (x_type == kF32 ? 4 : 2)) % 16 == 0;
     c.p.early = !first;
     if (few_values(c)) return launch_rows_any(c, &x, x_type, !first, stream);
     if (!few_tokens(c) && !encoder()) return -6;
-    const cudaError_t e = launch_quantize(x, x_type, stream, !first);
+    QuantParams once = x;
+    if (apart) { once.rows = nullptr; once.rows_div = 1; once.M = x.x_rows; once.q = apart; once.scale = apart_scale; }
+    cudaError_t e = launch_quantize(once, x_type, stream, !first);
+    if (e == cudaSuccess && apart)
+        e = launch_pdl(gather_rows_kernel, dim3((unsigned)((x.M + 7) / 8)), 256, 0, stream, (const int8_t*)apart, (const float*)apart_scale, x.x_rows, x.rows, x.rows_div, x.q, x.scale, x.M,
+                       x.ldq);
     if (e != cudaSuccess) return -(100 + (int)e);
     c.p.early = true;
     return launch_matmul(c, true, stream);
@@ -1426,12 +1472,13 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
     if (rc || M == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     return launch_linear(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, false),
-                         QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, true, stream);
+                         QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, true, nullptr, nullptr, stream);
 }
 
-int64_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F) {
-    if (pairs < 0 || pairs > 0x7FFFFFFF || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return -2;
-    return (int64_t)(rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up8(F) * 4));
+int64_t chimere_b200_experts_w8a8_bytes(int64_t T, int top_k, int H, int F) {
+    if (T < 0 || top_k <= 0 || T > 0x7FFFFFFF / top_k || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return -2;
+    const int64_t pairs = T * top_k;
+    return (int64_t)(rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up8(F) * 4) + (gather_apart(pairs, top_k, H) ? rows_bytes(T, H) : 0));
 }
 
 int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
@@ -1448,6 +1495,12 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
     int8_t* hq = (int8_t*)ws.take((size_t)P * up16(F));
     float* h_scale = (float*)ws.take((size_t)P * 4);
     float* h = (float*)ws.take((size_t)P * up8(F) * 4);
+    int8_t* apart = nullptr;
+    float* apart_scale = nullptr;
+    if (gather_apart(P, top_k, H)) {
+        apart = (int8_t*)ws.take((size_t)T * up16(H));
+        apart_scale = (float*)ws.take((size_t)T * 4);
+    }
     if (P > 0 && (!d_ws || !d_perm || !d_offsets)) return -1;
     if (misaligned(d_ws, 256) || misaligned(d_offsets, 4)) return -5;
     int rc = check_quantize(d_x, x_type, ldx, T, d_perm, top_k, P, H, q, up16(H), scale);
@@ -1458,11 +1511,11 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
     if (rc || P == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     rc = launch_linear(matmul_call(q, up16(H), scale, d_w_up, ld_up, stride_up, d_up_scale, nullptr, d_offsets, E, P, F, H, act, h, kF32, up8(F), P, nullptr, d_status, false),
-                       QuantParams{d_x, ldx, T, d_perm, top_k, H, q, up16(H), scale, P, 0}, x_type, true, stream);
+                       QuantParams{d_x, ldx, T, d_perm, top_k, H, q, up16(H), scale, P, 0}, x_type, true, apart, apart_scale, stream);
     if (rc) return rc;
     return launch_linear(matmul_call(hq, up16(F), h_scale, d_w_down, ld_down, stride_down, d_down_scale, nullptr, d_offsets, E, P, H, F, CHIMERE_ACT_NONE, d_y, y_type, ldy, P, d_perm,
                                      d_status, false),
-                         QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, P, 0}, kF32, false, stream);
+                         QuantParams{h, up8(F), P, nullptr, 1, F, hq, up16(F), h_scale, P, 0}, kF32, false, nullptr, nullptr, stream);
 }
 
 }  // extern "C"

@@ -196,7 +196,7 @@ def experts_w8a8(x: torch.Tensor, perm: torch.Tensor, offsets: torch.Tensor, top
     out, yp, kind, ldy = _output(out, P, H, out_dtype or (None if out is not None else x.dtype), x)
     up, ld_up, plane_up = _stack(w_up, "w_up", index)
     down, ld_down, plane_down = _stack(w_down, "w_down", index)
-    ws, nbytes = _scratch(x, (abi._lib or abi.load()).chimere_b200_experts_w8a8_bytes(P, H, F))
+    ws, nbytes = _scratch(x, (abi._lib or abi.load()).chimere_b200_experts_w8a8_bytes(T, top_k, H, F))
     _call("chimere_b200_experts_w8a8", index, xp, x_kind, ldx, T, _vector(perm, "perm", (P,), torch.int32, index),
           _vector(offsets, "offsets", (E + 1,), torch.int32, index), top_k, E, up, ld_up, plane_up, _vector(up_scale, "up_scale", (E, R), torch.float32, index),
           down, ld_down, plane_down, _vector(down_scale, "down_scale", (E, H), torch.float32, index), H, F, act, yp, kind, ldy,

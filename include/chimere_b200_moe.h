@@ -399,7 +399,7 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
  * of d_perm (d_offsets[e] .. d_offsets[e + 1]) holds the pair; d_perm and d_offsets as chimere_b200_moe_route / _permute leave them.  The rows between the two products
  * are held in f32 and quantised by token again.  w_up [E][2 F (SWIGLU: gate rows, then up) or F (RELU2)][H], w_down [E][H][F].  Rows of y whose pair is in no expert's range are
  * not written.  Scratch as above. */
-int64_t chimere_b200_experts_w8a8_bytes(int64_t pairs, int H, int F);
+int64_t chimere_b200_experts_w8a8_bytes(int64_t T, int top_k, int H, int F);
 int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
                               const int8_t* d_w_up, int64_t ld_up, int64_t stride_up, const float* d_up_scale,
                               const int8_t* d_w_down, int64_t ld_down, int64_t stride_down, const float* d_down_scale,
@@ -417,9 +417,10 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
  * router leaves it, mask uint8 [S][L] or NULL, grad_loss f32 [S] or NULL (ones); loss f32 [S], counts int32 [S][E], prob f32 [S][E], tokens int32 [S] (n).
  * E <= 256, top_k <= 256, S * L and L * top_k below 2^31.  A token whose logits are all -inf has no probabilities (it adds none and its gradient is
  * zero; its pairs count); a NaN, or +inf under softmax, makes its sequence's loss and prob and its own gradient NaN.
- * d_grad_logits NULL: no gradient.  d_ws: scratch of balance_loss_bytes, 256-byte aligned, used by no other call at the same time.  Sums are added in an order
+ * d_grad_logits NULL: no gradient.  d_ws: scratch of balance_loss_bytes (0: none needed, d_ws may be NULL; below 0: an error), 256-byte aligned, used by no
+ * other call at the same time.  Sums are added in an order
  * that depends on S, L, E and top_k alone: the same bits every time.  Errors as above. */
-size_t chimere_b200_balance_loss_bytes(int64_t S, int64_t L, int E, int top_k);
+int64_t chimere_b200_balance_loss_bytes(int64_t S, int64_t L, int E, int top_k);
 int chimere_b200_balance_loss(const void* d_logits, int type, int64_t ld, int64_t stride_s, const int32_t* d_topk_idx, const uint8_t* d_mask,
                               int64_t S, int64_t L, int E, int top_k, int route_mode, float coef, float* d_loss, int32_t* d_counts, float* d_prob,
                               int32_t* d_tokens, const float* d_grad_loss, void* d_grad_logits, int64_t ld_grad, int64_t stride_grad_s,

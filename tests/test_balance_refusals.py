@@ -25,7 +25,7 @@ BAD = [(-2, dict(S=-1)), (-2, dict(L=-1)), (-2, dict(E=0)), (-2, dict(E=257, ld=
        (-5, dict(counts=A + 2)), (-5, dict(gl=A + 2)), (-2, dict(d=A, ldd=15)), (-2, dict(d=A, stride_d=159)), (-5, dict(d=A + 1)), (0, dict(S=0))]
 
 
-@pytest.mark.parametrize("want,kw", BAD + [(-1, dict(ids=None)), (-1, dict(out=None)), (-1, dict(prob=None)), (-1, dict(ws=None)), (-5, dict(ws=A + 64)), (-5, dict(ids=A + 2)), (-4, dict(nbytes=128)),
+@pytest.mark.parametrize("want,kw", BAD + [(-1, dict(ids=None)), (-1, dict(out=None)), (-1, dict(prob=None)), (-1, dict(ws=None, L=100000, stride=1600000)), (-5, dict(ws=A + 64)), (-5, dict(ids=A + 2)),
                                            (-4, dict(L=100000, nbytes=4096, stride=1600000))])
 def test_loss(lib, want, kw):
     assert loss(lib, **kw) == want
@@ -38,5 +38,5 @@ def test_backward(lib, want, kw):
 
 def test_scratch_sizes(lib):
     f = lib.chimere_b200_balance_loss_bytes
-    assert f(0, 10, 16, 2) > 0 and f(1, 0, 16, 2) > 0 and f(1, 10, 0, 2) == 0 and f(1, 10, 257, 2) == 0 and f(1, 10, 16, 0) == 0 and f(-1, 10, 16, 2) == 0
+    assert f(0, 10, 16, 2) == 0 and f(1, 0, 16, 2) == 0 and f(1, 10, 16, 2) == 0 and f(1, 10, 0, 2) == -2 and f(1, 10, 257, 2) == -2 and f(1, 10, 16, 0) == -2 and f(-1, 10, 16, 2) == -2
     assert f(1, 1 << 20, 256, 8) > f(1, 1 << 10, 256, 8) and f(16, 8192, 256, 8) < 1 << 22

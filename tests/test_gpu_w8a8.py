@@ -342,8 +342,8 @@ def test_linear_of_rows_at_the_ends_of_the_range(dtype):
 def test_experts_with_ids_outside_the_rows():
     """A permutation entry that is no pair: a row of zeros goes in, and nothing comes out for it."""
     g = gen(22)
-    for T, E in ((6, 32), (200, 4)):
-        H, F, k = 160, 64, 2
+    for T, E, H in ((6, 32, 160), (200, 4, 160), (1100, 5, 2005)):
+        F, k = 64, 2
         x = torch.randn(T, H, generator=g, device="cuda")
         perm = torch.randperm(T * k, generator=g, device="cuda").to(torch.int32)
         off = groups([T * k // E] * (E - 1) + [T * k - (E - 1) * (T * k // E)])
@@ -357,6 +357,15 @@ def test_experts_with_ids_outside_the_rows():
         keep = torch.ones(T * k, dtype=torch.bool, device="cuda")
         keep[lost] = False
         assert torch.equal(out[keep], want[keep]) and (out[lost] == 7).all()
+        if T > 1000:     # rows quantised once and copied, against a gather of the rows themselves
+            q, s = w8a8.quantize_i8(x, perm, k)
+            hq, hs = w8a8.quantize_i8(w8a8.matmul_w8a8_grouped(q, s, wu, su, off, act=abi.ACT_SWIGLU))
+            assert torch.equal(want, w8a8.matmul_w8a8_grouped(hq, hs, wd, sd, off, out_rows=perm, out=torch.empty_like(want)))
+            twice = perm.clone()
+            twice[7] = twice[8]                       # one pair in two places of the same group: its row is written twice, alike
+            twice[7:9] = twice[8]
+            again = w8a8.experts_w8a8(x, twice, off, k, wu, su, wd, sd, out=torch.full_like(want, 7.0))
+            assert torch.equal(again[twice.long()], want[twice.long()]) and (again[perm[7].long()] == 7).all()
 
 
 def test_capture_and_replay_with_new_inputs():

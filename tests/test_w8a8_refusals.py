@@ -70,5 +70,6 @@ def test_scratch_sizes(lib):
     assert linear(-1, 32, 64) == -2 and linear(4, 32, 0) == -2 and linear(4, 32, 131072) == -2 and linear(4, 0, 64) == -2
     assert linear(0, 32, 64) == 0 and linear(1, 4096, 2048) == 0            # one launch: no scratch
     assert linear(9, 32, 2005) >= 9 * (2016 + 4) and linear(1, 32, 20000) >= 20004 and linear(70000, 32, 131071) >= 70000 * 131076
-    assert experts(8, 64, 0) == -2 and experts(-1, 64, 64) == -2
-    assert experts(8, 64, 33) >= 8 * (64 + 4 + 48 + 4 + 33 * 4)
+    assert experts(8, 2, 64, 0) == -2 and experts(-1, 2, 64, 64) == -2 and experts(1, 0, 64, 64) == -2 and experts(1 << 30, 8, 64, 64) == -2
+    assert experts(4, 2, 64, 33) >= 8 * (64 + 4 + 48 + 4 + 33 * 4)
+    assert experts(4096, 8, 2048, 64) >= 32768 * (2048 + 4 + 64 + 4 + 64 * 4) + 4096 * 2052
