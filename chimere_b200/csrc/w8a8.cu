@@ -1288,11 +1288,12 @@ int launch_rows_any(const MatmulCall& c, const QuantParams* x, int x_type, bool 
 }
 // Batches for the kernel of a few tokens: dense ones of up to four (4096 x 2048, us, this / tensor-core tiles: 1 token 4.4 / 6.1, 4: 5.1 / 6.1, 6: 5.9 / 6.1; 2048 x
 // 4096 6: 6.9 / 6.9; 4096 x 8192 3: 11.9 / 11.9, 6: 17.3 / 12.1).  Grouped ones while their CTAs, if every pair has a group of its own, are four per SM at most (experts of 512 x 2048,
-// both products, 8 pairs 12.3 / 18.4, 16: 20.5 / 20.5, 32: 34 / 27; of 1856 x 2688 6 pairs, 696 and 1008 CTAs, 24.6 / 20.6; of 2048 x 2048 4 pairs 21 / 25, 8: 31 / 26).
-constexpr int kR_DenseTokens = 4, kR_MaxCtas = 4 * 148;
+// both products, 8 pairs 12.3 / 18.4, 16: 20.5 / 20.5, 32: 34 / 27; of 1856 x 2688 6 pairs, 696 and 1008 CTAs, 24.6 / 20.6; of 2048 x 2048 4 pairs 21 / 25, 8: 31 / 26), and no more than 32 pairs, since they may all be one group's, which
+// its CTAs take eight at a time.
+constexpr int kR_DenseTokens = 4, kR_MaxCtas = 4 * 148, kR_MaxPairs = 32;
 bool few_tokens(const MatmulCall& c) {
     if (c.p.K > kR_MaxK) return false;
-    return c.p.offsets ? (int64_t)c.p.M * ((c.p.N + rows_outs(c.p.K) - 1) / rows_outs(c.p.K)) <= kR_MaxCtas : c.p.M <= kR_DenseTokens;
+    return c.p.offsets ? c.p.M <= kR_MaxPairs && (int64_t)c.p.M * ((c.p.N + rows_outs(c.p.K) - 1) / rows_outs(c.p.K)) <= kR_MaxCtas : c.p.M <= kR_DenseTokens;
 }
 // ... whose CTAs quantise the tokens themselves: dense, up to so many values and two CTAs per SM (4096 x 2048 1 token 4.9 against 5.4 with a launch in front,
 // 8192 x 4096 12.3 against 10.2; 4096 x 2048 3 tokens 6.4 against 5.9).
