@@ -250,7 +250,7 @@ struct Tile { int expert, row0, ntok, n0; };
 // Token tiles per expert, summed over the experts in front, and where the experts' rows start.
 struct GroupTable {
     int prefix[kMaxGroups + 1], start[kMaxGroups + 1];
-    int scan[kMM_Threads / 32];
+    int scan[32];
 };
 
 __device__ __forceinline__ bool elect1() {
@@ -342,14 +342,16 @@ __device__ __forceinline__ void ld_cluster4(uint32_t addr, int (&sum)[4]) {   //
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum[i] += v[i];
 }
+// An arrival that orders nothing but what the tensor-memory fence in front of it does: with the cluster's release it would wait for the tile's stores to
+// reach L2 (a microsecond per tile).
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 
 // By all threads; returns the call's token tiles.
-template <int TOKENS>
+template <int TOKENS, int THREADS>
 __device__ __forceinline__ int group_table(const MatmulParams& p, GroupTable& g) {
-    constexpr int kPer = (kMaxGroups + kMM_Threads - 1) / kMM_Threads;
+    constexpr int kPer = (kMaxGroups + THREADS) / THREADS;   // (the table's end included)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int mine[kPer], start[kPer], sum = 0;
 #pragma unroll
@@ -381,7 +383,6 @@ __device__ __forceinline__ int group_table(const MatmulParams& p, GroupTable& g)
     __syncthreads();
     return g.prefix[p.E];
 }
-static_assert((kMaxGroups + kMM_Threads - 1) / kMM_Threads * kMM_Threads > kMaxGroups, "a thread writes the table's end");
 
 // Tile `id` of the call: token tiles fastest, so that the CTAs at work at a time share weight rows.
 template <int TOKENS, int OUTS>
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
     const uint32_t stages = smem_u32(smem);
 
     if (!p.early) griddep_wait();
-    const int total = (p.offsets ? group_table<BN>(p, table) : p.mt) * p.nt;
+    const int total = (p.offsets ? group_table<BN, kMM_Threads>(p, table) : p.mt) * p.nt;
     if (first >= total) {   // (the whole cluster; nothing has been allocated)
         griddep_launch();
         griddep_wait();   // (whoever waits for this grid has what lies before it as well)
@@ -888,10 +889,15 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
 
 // ---- many tokens ----
 constexpr int kW_Tokens = 256, kW_Cols = 256;                 // of a pair's tile: tokens, weight rows (SwiGLU: 128 gate, 128 up)
-constexpr int kW_Stage = 2 * kMM_ABytes, kW_Stages = 6, kW_StagesTurned = 5;
-constexpr int kW_EpiWarps = 8;
-constexpr int kW_TurnFloats = 32 * 33;                        // a warp's 32 x 32 results on their way to rows that are not aligned
-constexpr int kW_Smem = 1024 + kW_Stages * kW_Stage, kW_SmemTurned = 1024 + kW_StagesTurned * kW_Stage + kW_EpiWarps * kW_TurnFloats * 4;
+constexpr int kW_Stage = 2 * kMM_ABytes, kW_Stages = 6;
+constexpr int kW_EpiWarps = 16, kW_Threads = 32 * (kMM_FirstEpi + kW_EpiWarps);   // (rows off the 32-byte boundaries with eight: 777 x 4099 of 2000 19.5 us, now 14.6)
+// a warp's 32 x 32 results on their way to rows that are not aligned: rows an odd number of words apart
+template <int TYPE> __host__ __device__ constexpr int turn_pitch() { return TYPE == kF32 ? 33 : 34; }
+template <int TYPE> __host__ __device__ constexpr int turn_bytes() { return 32 * turn_pitch<TYPE>() * (TYPE == kF32 ? 4 : 2); }
+template <int TYPE> __host__ __device__ constexpr int turned_stages() { return TYPE == kF32 ? 4 : 5; }
+template <int TYPE> __host__ __device__ constexpr int wide_smem(bool vec) {
+    return 1024 + (vec ? kW_Stages * kW_Stage : turned_stages<TYPE>() * kW_Stage + kW_EpiWarps * turn_bytes<TYPE>());
+}
 
 struct WideShared {
     uint64_t full[kW_Stages], empty[kW_Stages];
@@ -917,31 +923,35 @@ __device__ __forceinline__ void stg256(void* p, const uint32_t* v) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
+template <int TYPE>
+__device__ __forceinline__ void pack32(const float (&o)[32], uint32_t (&w)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (TYPE == kF16) {
+            const __half2 h = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+}
 // 32 results of one row, all of them inside it and 32-byte aligned
 template <int TYPE>
 __device__ __forceinline__ void store_row32(typename Out<TYPE>::T* y, const float (&o)[32]) {
-    if (TYPE == kF32) {
+    if constexpr (TYPE == kF32) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) stg256(y + 8 * i, reinterpret_cast<const uint32_t*>(o) + 8 * i);
     } else {
         uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (TYPE == kF16) {
-                const __half2 h = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-        }
+        pack32<TYPE>(o, w);
         stg256(y, w);
         stg256(y + 16, w + 8);
     }
 }
 // A warp's 32 rows x 32 results from column n on.  r: this lane's row of y, -1 if it has none.
 template <int TYPE>
-__device__ __forceinline__ void store_block(const MatmulParams& p, float* turn, int64_t r, int n, const float (&o)[32], int lane) {
+__device__ __forceinline__ void store_block(const MatmulParams& p, typename Out<TYPE>::T* turn, int r, int n, const float (&o)[32], int lane) {
     using T = typename Out<TYPE>::T;
     T* y = reinterpret_cast<T*>(p.y);
     if (p.vec) {
@@ -956,19 +966,27 @@ __device__ __forceinline__ void store_block(const MatmulParams& p, float* turn, 
     }
     // a lane per column: 32 neighbours of a row at a time
     __syncwarp();
+    T* mine = turn + lane * turn_pitch<TYPE>();
+    if constexpr (TYPE == kF32) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = o[j];
+        for (int j = 0; j < 32; ++j) mine[j] = o[j];
+    } else {
+        uint32_t w[16];
+        pack32<TYPE>(o, w);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) reinterpret_cast<uint32_t*>(mine)[j] = w[j];
+    }
     __syncwarp();
     const bool in = n + lane < p.N;
 #pragma unroll 8
     for (int i = 0; i < 32; ++i) {
-        const int64_t ri = __shfl_sync(0xffffffffu, r, i);
-        if (ri >= 0 && in) y[ri * p.ldy + n + lane] = Out<TYPE>::of(turn[i * 33 + lane]);
+        const int ri = __shfl_sync(0xffffffffu, r, i);
+        if (ri >= 0 && in) y[ri * p.ldy + n + lane] = turn[i * turn_pitch<TYPE>() + lane];
     }
 }
 
 template <int TYPE, bool DUAL>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, MatmulParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW_Threads, 1) wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, MatmulParams p) {
     constexpr int kOuts = DUAL ? 128 : 256;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) WideShared sh;
@@ -979,7 +997,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
     const uint32_t stages = smem_u32(smem);
 
     if (!p.early) griddep_wait();
-    const int total = (p.offsets ? group_table<kW_Tokens>(p, table) : p.mt) * p.nt;
+    const int total = (p.offsets ? group_table<kW_Tokens, kW_Threads>(p, table) : p.mt) * p.nt;
     if (first >= total) {   // (both CTAs; nothing has been allocated)
         griddep_launch();
         griddep_wait();   // (whoever waits for this grid has what lies before it as well)
@@ -1063,21 +1081,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
             mbar_wait(&sh.drain, 0);
         }
     } else if (warp >= kMM_FirstEpi) {
-        const int q = warp & 3, half = (warp - kMM_FirstEpi) >> 2, row = q * 32 + lane, et = tid - 32 * kMM_FirstEpi;
+        const int q = warp & 3, part = (warp - kMM_FirstEpi) >> 2, row = q * 32 + lane, et = tid - 32 * kMM_FirstEpi;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-        float* turn = reinterpret_cast<float*>(smem + kW_StagesTurned * kW_Stage) + (warp - kMM_FirstEpi) * kW_TurnFloats;   // (where rows are not aligned)
+        constexpr int kMine = kOuts / (kW_EpiWarps / 4);   // columns of a warp
+        auto* turn = reinterpret_cast<typename Out<TYPE>::T*>(smem + turned_stages<TYPE>() * kW_Stage + (warp - kMM_FirstEpi) * turn_bytes<TYPE>());   // (where rows are not aligned)
         bool ok = true;
         griddep_wait();   // (the tokens' scales; and nothing of y is written before what used its memory has ended)
         // a tile's scales and places are looked up while the one before is on its way
         Tile t;
-        float sw_next, bias_next, sx_next;
+        float sw_next = 0.0f, bias_next = 0.0f, sx_next;
         int64_t r_next;
         auto look_up = [&](int id) {
             t = take_tile<kW_Tokens, kOuts>(p, table, id);
-            const int c = DUAL ? t.n0 + (et & 127) : t.n0 + et;   // accumulator column `et`
-            const int64_t at = ((int64_t)t.expert * (DUAL ? 2 : 1) + (DUAL ? et >> 7 : 0)) * p.N + c;
-            sw_next = c < p.N ? p.sw[at] : 0.0f;
-            bias_next = c < p.N && p.bias ? p.bias[at] : 0.0f;
+            if (et < kW_Cols) {
+                const int c = DUAL ? t.n0 + (et & 127) : t.n0 + et;   // accumulator column `et`
+                const int64_t at = ((int64_t)t.expert * (DUAL ? 2 : 1) + (DUAL ? et >> 7 : 0)) * p.N + c;
+                sw_next = c < p.N ? p.sw[at] : 0.0f;
+                bias_next = c < p.N && p.bias ? p.bias[at] : 0.0f;
+            }
             const int i = 128 * rank + row;   // this thread's token of the tile
             r_next = -1;
             sx_next = 0.0f;
@@ -1090,18 +1111,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMM_Threads, 1) wide
         int n = 0;
         for (int id = first; id < total; id += step, ++n) {
             const int buf = n & 1, ntok = t.ntok, n0 = t.n0;
-            sh.sw[buf][et] = sw_next;
-            sh.bias[buf][et] = bias_next;
-            const int64_t r = r_next >= 0 && r_next < p.y_rows ? r_next : -1;
+            if (et < kW_Cols) { sh.sw[buf][et] = sw_next; sh.bias[buf][et] = bias_next; }
+            const int r = r_next >= 0 && r_next < p.y_rows ? (int)r_next : -1;
             float sx = sx_next;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kW_EpiWarps) : "memory");
             if (id + step < total) look_up(id + step);
             if (ok && !mbar_wait(&sh.tfull[buf], (n >> 1) & 1)) { ok = false; sh.failed = 1; }
             fence_after();
             if (!ok) sx = __uint_as_float(0x7FC00000u);
             if (128 * rank + q * 32 < ntok) {
 #pragma unroll 1
-                for (int c0 = half * (kOuts / 2); c0 < (half + 1) * (kOuts / 2); c0 += 32) {
+                for (int c0 = part * kMine; c0 < (part + 1) * kMine; c0 += 32) {
                     if (n0 + c0 >= p.N) break;
                     int v[32];
                     float o[32];
@@ -1229,14 +1249,16 @@ int launch_wide(const MatmulCall& c, int64_t tiles, bool pdl, cudaStream_t strea
     p.nt = (p.N + kOuts - 1) / kOuts;
     p.split = 1;
     p.vec = ((uintptr_t)p.y & 31) == 0 && p.ldy * kSize % 32 == 0;
-    p.n_stages = p.vec ? kW_Stages : kW_StagesTurned;
+    p.n_stages = p.vec ? kW_Stages : turned_stages<TYPE>();
     auto kernel = wide_kernel<TYPE, DUAL>;
-    constexpr int kMost = kW_Smem > kW_SmemTurned ? kW_Smem : kW_SmemTurned;
+    constexpr int kMost = wide_smem<TYPE>(true) > wide_smem<TYPE>(false) ? wide_smem<TYPE>(true) : wide_smem<TYPE>(false);
+    static_assert(kMost + (int)sizeof(WideShared) + (int)sizeof(GroupTable) <= 227 * 1024, "one CTA's shared memory");
     cudaError_t e = max_smem_once(kernel, kMost, done);
     if (e != cudaSuccess) return -(100 + (int)e);
     const int pairs = sm_count() / 2;
     cudaLaunchAttribute attr[2];
-    const cudaLaunchConfig_t cfg = launch_config(2 * (int)(tiles < pairs ? tiles : pairs), p.vec ? kW_Smem : kW_SmemTurned, 1, pdl, stream, attr);
+    cudaLaunchConfig_t cfg = launch_config(2 * (int)(tiles < pairs ? tiles : pairs), wide_smem<TYPE>(p.vec), 1, pdl, stream, attr);
+    cfg.blockDim = dim3(kW_Threads);
     e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, p);
     return e == cudaSuccess ? 0 : -(100 + (int)e);
 }
@@ -1350,7 +1372,7 @@ int launch_matmul(const MatmulCall& c, bool pdl, cudaStream_t stream) {
 }
 
 // A batch's pairs share rows: from so many values on each row is quantised once and copied to its pairs (32768 pairs of 2048 values, eight per row, bf16: 37 us when each pair
-// quantises its own, NN so).
+// quantises its own, 9 + 16 so).
 constexpr int64_t kGatherValues = 1 << 22;
 bool gather_apart(int64_t pairs, int top_k, int K) { return top_k > 1 && pairs * K >= kGatherValues; }
 
