@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
                 for (int i = 0; i < 2; ++i) {
                     uint64_t w = mul2(v[u][j][i], add2(g[j][i], less));
                     if (SIGMOID) w = mul2(w, slope[u][j][i]);
-                    unpack2(w, d[2 * i], d[2 * i + 1]);
+                    unpack2(sum[u] == 0.0f ? 0 : w, d[2 * i], d[2 * i + 1]);   // (zero also where grad_loss is not finite)
                 }
                 store4<TYPE, FULL>(p.d_logits, at + 4 * LANES * j, r < r1 ? there[j] : 0, p.vec, d);
             }
@@ -537,19 +537,24 @@ cudaError_t launch_balance(const BalanceParams& p, int type, cudaStream_t stream
          : type == CHIMERE_TYPE_F16 ? launch_balance_mode<CHIMERE_TYPE_F16>(p, stream) : launch_balance_mode<CHIMERE_TYPE_BF16>(p, stream);
 }
 
-// Pieces of a sequence.  With the counting in front: as many CTAs as run at once.  In clusters: two to eight, at least kB_PieceRows rows in each; taken
+// Pieces of a sequence.  With the counting in front: as many CTAs as run at once.  In clusters: up to eight, at least kB_PieceRows rows in each; taken
 // for short sequences, and for so many of them that eight pieces of each fill the GPU.
 constexpr int kB_PieceRows = 32, kB_Cluster = 8, kB_ClusterRows = 512, kB_Sms = 148;   // (the scratch's size goes by these: constants)
 struct Plan { int pieces, rows, count_pieces, count_rows; };
 Plan plan_of(int64_t S, int L, int k) {
     Plan r{};
-    if (L <= kB_ClusterRows || S * kB_Cluster >= kB_CtasPerSm * kB_Sms) {
-        r.pieces = 1;
-        while (r.pieces < kB_Cluster && L > r.pieces * kB_PieceRows) r.pieces *= 2;
+    constexpr int64_t slots = kB_CtasPerSm * kB_Sms;
+    if (L <= kB_ClusterRows || S * kB_Cluster >= slots) {
+        // waves times rows, a CTA's fixed cost taken for those of kB_PieceRows
+        int64_t best = 0;
+        for (int n = 1; n <= kB_Cluster && (n == 1 || (int64_t)(n - 1) * kB_PieceRows < L); ++n) {
+            const int64_t cost = ((S * n + slots - 1) / slots) * (((int64_t)L + n - 1) / n + kB_PieceRows);
+            if (n == 1 || cost < best) { best = cost; r.pieces = n; }
+        }
         r.rows = (int)(((int64_t)L + r.pieces - 1) / r.pieces);
         return r;
     }
-    const int64_t n = kB_CtasPerSm * kB_Sms / S;      // (rounded down: one more wave for a few pieces would double the time)
+    const int64_t n = slots / S;      // (rounded down: one more wave for a few pieces would double the time)
     r.rows = (int)((L + n - 1) / n);
     r.rows = r.rows < kB_PieceRows ? kB_PieceRows : r.rows;
     r.pieces = (int)(((int64_t)L + r.rows - 1) / r.rows);

@@ -87,7 +87,7 @@ def bits(r, d):
     return [t.clone() for t in r] + ([] if d is None else [d.clone()])
 
 
-SHAPES = [(1, 1, 1, 1), (1, 1, 256, 8), (1, 24, 256, 8), (3, 17, 5, 2), (2, 64, 32, 4), (2, 65, 33, 3), (4, 1000, 128, 6), (5, 333, 64, 1), (1, 3000, 255, 8), (2, 2048, 60, 7), (300, 70, 16, 2),
+SHAPES = [(1, 1, 1, 1), (1, 1, 256, 8), (1, 24, 256, 8), (3, 17, 5, 2), (2, 64, 32, 4), (2, 65, 33, 3), (4, 1000, 128, 6), (5, 333, 64, 1), (1, 3000, 255, 8), (2, 2048, 60, 7), (300, 70, 16, 2), (60, 700, 40, 3), (100, 600, 64, 4), (500, 513, 8, 1), (7, 513, 256, 8),
           (1, 40000, 256, 8), (64, 129, 130, 256), (1, 100000, 8, 2)]
 
 
@@ -191,6 +191,35 @@ def test_ids_outside_and_repeated(L):
     ids[:] = -7
     r, d = balance.balance_loss_grad(logits, ids)
     assert (r.loss == 0).all() and (r.counts == 0).all() and (d == 0).all()
+
+
+@pytest.mark.parametrize("L", [40, 4000])
+def test_a_grad_loss_that_is_not_finite_leaves_masked_rows_alone(L):
+    logits, ids = inputs(3, L, 64, 4, seed=15)
+    mask = torch.rand(3, L, generator=gen(3), device="cuda") < 0.5
+    mask[2] = False
+    _, d = balance.balance_loss_grad(logits, ids, mask=mask, grad_loss=torch.tensor([float("nan"), float("inf"), float("inf")], device="cuda"))
+    assert (d[~mask] == 0).all() and torch.isnan(d[0][mask[0]]).all()
+
+
+def test_more_than_2_31_logits():
+    """Offsets beyond 32 bits: the last rows' gradients, and counts and mean probabilities of all."""
+    T, E = (1 << 31) // 256 + 1000, 256
+    logits = torch.zeros(T, E, dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    logits[-500:] = torch.randn(500, E, generator=gen(1), device="cuda").to(torch.bfloat16)
+    ids[-500:] = torch.randint(0, E, (500, 1), generator=gen(2), device="cuda", dtype=torch.int32)
+    r, d = balance.balance_loss_grad(logits, ids, grad_loss=torch.tensor(1e9, device="cuda"))
+    counts = torch.bincount(ids.reshape(-1).long(), minlength=E)
+    assert torch.equal(r.counts.long(), counts) and r.tokens.item() == T
+    p = torch.softmax(logits[-500:].double(), 1)
+    prob = (p.sum(0) + (T - 500) / E) / T
+    assert ((r.prob.double() - prob).abs() <= prob * 20000 * U).all()       # (a lane adds 19000 / 8 values of 1 / 256 and fewer)
+    g = 1e9 * E / float(T) ** 2 * (counts.double() - T / E)
+    want = p * (g - (p * g).sum(1, keepdim=True))
+    assert ((d[-500:].double() - want).abs() <= want.abs() * 2.0 ** -8 + 1e-3 * want.abs().max()).all()
+    flat = 1 / E * (g - g.mean())
+    assert ((d[12345].double() - flat).abs() <= flat.abs() * 2.0 ** -7 + 1e-6 * flat.abs().max()).all()
 
 
 def test_even_load_gives_coef():

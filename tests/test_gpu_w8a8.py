@@ -428,6 +428,21 @@ def test_two_streams_at_once():
     assert all(torch.equal(v, want) for v in got) and all(torch.equal(v, want2) for v in got2)
 
 
+@pytest.mark.parametrize("N", [32768, 32749])
+def test_more_than_2_31_results(N):
+    """Offsets beyond 32 bits, in the rows that are quantised and in the results (aligned and not)."""
+    M, K = (1 << 31) // 32749 + 300, 64
+    g = gen(30)
+    x, w, sw = torch.randn(M, K, generator=g, device="cuda"), i8(g, N, K), scales(g, N)
+    y = w8a8.linear_w8a8(x, w, sw, out_dtype=torch.bfloat16)
+    rows = torch.cat([torch.arange(3, device="cuda"), torch.arange(M - 290, M, device="cuda")])
+    q, s = quantized(x[rows])
+    check(y[rows], *product(q, s, w, sw, None, abi.ACT_NONE, torch.bfloat16))
+    qy, sy = w8a8.quantize_i8(y)
+    rq, rs = quantized(y[rows])
+    assert torch.equal(qy[rows], rq) and torch.equal(sy[rows], rs)
+
+
 def test_no_rows():
     g = gen(1)
     x, w, sw = torch.empty(0, 64, device="cuda"), i8(g, 40, 64), scales(g, 40)
