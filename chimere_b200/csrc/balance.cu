@@ -539,7 +539,7 @@ cudaError_t launch_balance(const BalanceParams& p, int type, cudaStream_t stream
 
 // Pieces of a sequence.  With the counting in front: as many CTAs as run at once.  In clusters: up to eight, at least kB_PieceRows rows in each; taken
 // for short sequences, and for so many of them that eight pieces of each fill the GPU.
-constexpr int kB_PieceRows = 32, kB_Cluster = 8, kB_ClusterRows = 512, kB_Sms = 148;   // (the scratch's size goes by these: constants)
+constexpr int kB_PieceRows = 32, kB_Cluster = 8, kB_ClusterRows = 1024, kB_Sms = 148;   // (the scratch's size goes by these: constants)
 struct Plan { int pieces, rows, count_pieces, count_rows; };
 Plan plan_of(int64_t S, int L, int k) {
     Plan r{};

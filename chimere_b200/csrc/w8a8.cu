@@ -697,7 +697,8 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
 // ---- a few tokens ----
 // Up to eight tokens at a time times 16 weight rows (or 16 of the gate and the same 16 of the up matrix) per warp, or per 2, 4 or 8 warps that share K in
 // pieces of 64 bytes, so that each has about four of them; the sums on the warp-level int8 MMA (m16n8k32), its K order that of the bytes a lane holds: 16 neighbouring ones of a weight row and the same 16 of a token's.
-// All of a warp's first weights are on their way before it looks at the tokens, which the CTA quantises itself (kI8: takes as they are): a call is one launch.
+// All of a warp's first weights are on their way before it looks at the tokens, which the CTA quantises itself, or the CTAs of a cluster one or two each for all of
+// them (kI8: takes as they are): a call is one launch.
 // Bound: the weights' bytes, and what a launch takes.  y by the formula of the other kernels, the same bits.
 constexpr int kI8 = -2;                 // rows that are quantised already
 constexpr int kR_Threads = 256, kR_Warps = 8, kR_Tokens = 8, kR_Units = 4;   // units of 64 bytes of K that a warp has on their way
@@ -712,6 +713,7 @@ struct RowsParams {
     const int8_t* w;
     int64_t ldw, w_plane;
     int kw;                    // warps that share K
+    int cluster;               // CTAs that share the quantising of the tokens (1, 2, 4 or 8; more than one: a single group of up to eight tokens)
     int ks;                    // bytes between tokens in shared memory: 64 modulo 128, so that neighbouring tokens lie in different banks
 };
 
@@ -732,6 +734,7 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
     const MatmulParams& mp = p.m;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kw = p.kw, wk = warp & (kw - 1), outs = 16 * (kR_Warps / kw);
+    const int C = TYPE == kI8 ? 1 : p.cluster, rank = C > 1 ? blockIdx.x & (C - 1) : 0;
     const int n0 = blockIdx.x * outs, K = mp.K, units = (K + 63) >> 6;
     if (!mp.early) griddep_wait();
     griddep_launch();
@@ -761,7 +764,7 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
 #pragma unroll
         for (int u = 0; u < kR_Units; ++u) {
             const int unit = base + wk + kw * u;
-            const bool in = unit < units && 64 * unit + 16 * t < K;
+            const bool in = unit < units && 64 * unit + 16 * t < K && n0 < mp.N;   // (a cluster's last CTAs may have no rows)
 #pragma unroll
             for (int i = 0; i < TILES; ++i)
 #pragma unroll
@@ -801,7 +804,7 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
         } else {
             using E = Elem<TYPE>;
             const int nv = p.vec ? K >> 3 : 0;
-            for (int m = 0; m < ntok; ++m) {
+            for (int m = rank; m < ntok; m += C) {
                 const int64_t src = source(m);
                 uint32_t top = 0;
                 if (src >= 0) {
@@ -813,7 +816,7 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
                 if (lane == 0) s_max[m][warp] = top;
             }
             __syncthreads();
-            for (int m = 0; m < ntok; ++m) {
+            for (int m = rank; m < ntok; m += C) {
                 const int64_t src = source(m);
                 const uint32_t top = __reduce_max_sync(0xffffffffu, s_max[m][lane & (kR_Warps - 1)]);
                 const float amax = __uint_as_float(top);
@@ -842,6 +845,19 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
                 }
                 for (int i = 8 * nv + tid; i < K; i += kR_Threads) q[i] = (int8_t)s.q(E::one(x + i));
                 if (tid == 0) s_scale[m] = s.scale;
+            }
+            if (C > 1) {   // the others' tokens from their shared memory
+                cluster_sync();
+                for (int i = tid; i < ntok * 4 * units; i += kR_Threads) {
+                    const int m = i / (4 * units), at = m * p.ks + 16 * (i - m * 4 * units), owner = m & (C - 1);
+                    if (owner == rank) continue;
+                    uint32_t w[4];
+                    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(cluster_addr(smem_u32(xs + at), owner)) : "memory");
+                    *reinterpret_cast<uint4*>(xs + at) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                if (tid < ntok && (tid & (C - 1)) != rank) s_scale[tid] = __int_as_float(ld_cluster(cluster_addr(smem_u32(&s_scale[tid]), tid & (C - 1))));
+                asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (a CTA's tokens stay until all have read them: the wait is at the end)
             }
         }
         __syncthreads();
@@ -885,6 +901,7 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
         }
         __syncthreads();
     }
+    if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---- many tokens ----
@@ -1289,11 +1306,14 @@ int launch_rows(const MatmulCall& c, const QuantParams* x, bool pdl, cudaStream_
     r.ks = 64 * (units | 1);
     r.kw = rows_warps(c.p.K);
     const int outs = rows_outs(c.p.K);
+    r.cluster = 1;
+    while (!c.p.offsets && TYPE != kI8 && r.cluster < c.p.M) r.cluster *= 2;
     auto kernel = rows_kernel<TYPE, DUAL>;
     cudaError_t e = max_smem_once(kernel, kR_Tokens * 64 * (kR_MaxK / 64 + 1), done);
     if (e != cudaSuccess) return -(100 + (int)e);
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t cfg = launch_config((c.p.N + outs - 1) / outs, (size_t)tokens * r.ks, 1, pdl, stream, attr);
+    const int ctas = (c.p.N + outs - 1) / outs;
+    cudaLaunchConfig_t cfg = launch_config((ctas + r.cluster - 1) / r.cluster * r.cluster, (size_t)tokens * r.ks, r.cluster, pdl, stream, attr);
     cfg.blockDim = dim3(kR_Threads);
     cfg.gridDim.y = c.p.offsets ? c.p.M : 1;
     e = cudaLaunchKernelEx(&cfg, kernel, r);
@@ -1317,11 +1337,12 @@ bool few_tokens(const MatmulCall& c) {
     if (c.p.K > kR_MaxK) return false;
     return c.p.offsets ? c.p.M <= kR_MaxPairs && (int64_t)c.p.M * ((c.p.N + rows_outs(c.p.K) - 1) / rows_outs(c.p.K)) <= kR_MaxCtas : c.p.M <= kR_DenseTokens;
 }
-// ... whose CTAs quantise the tokens themselves: dense, up to so many values and two CTAs per SM (4096 x 2048 1 token 4.9 against 5.4 with a launch in front,
-// 8192 x 4096 12.3 against 10.2; 4096 x 2048 3 tokens 6.4 against 5.9).
-constexpr int64_t kR_Values = 4096;
-bool few_values(int64_t M, int N, int K) { return M <= kR_DenseTokens && K <= kR_MaxK && M * K <= kR_Values && (N + rows_outs(K) - 1) / rows_outs(K) <= 2 * 148; }
-bool few_values(const MatmulCall& c) { return few_tokens(c) && (c.p.offsets || few_values(c.p.M, c.p.N, c.p.K)); }
+// ... whose CTAs quantise the tokens themselves, in clusters: dense ones of up to eight tokens, rows of up to 2048 values (one token: up to kR_MaxK) and two CTAs per SM.  us,
+// in one launch / with one in front: 1024 x 2048 1 token 3.8 / 4.6, 8: 6.1 / 7.2; 4096 x 2048 1: 4.9 / 4.6, 4: 6.4 / 6.1, 8: 7.4 / 7.4; 512 x 512 8: 5.4 / 6.1; 2048 x 4096 1: 5.9 / 6.1,
+// 8: 11.0 / 8.5; 3712 x 2688 7: 9.4 / 7.7; 8192 x 4096 (512 CTAs) 1: 12.4 / 9.4; 16384 x 2048 8: 23 / 12.
+constexpr int kR_InlineK = 2048;
+bool few_values(int64_t M, int N, int K) { return M <= kR_Tokens && K <= (M == 1 ? kR_MaxK : kR_InlineK) && (N + rows_outs(K) - 1) / rows_outs(K) <= 2 * 148; }
+bool few_values(const MatmulCall& c) { return c.p.offsets ? few_tokens(c) : few_values(c.p.M, c.p.N, c.p.K); }
 
 int launch_matmul(const MatmulCall& c, bool pdl, cudaStream_t stream) {
     if (c.p.M == 0) return 0;

@@ -388,7 +388,7 @@ int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float
                                      int act, void* d_y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* d_out_rows,
                                      int32_t* d_status, cudaStream_t stream);
 
-/* quantize_i8 of the M rows of x and matmul_w8a8 in one call (a token or two: one launch).  d_ws: scratch of at least linear_w8a8_bytes(M, N, K), 256-byte aligned, used by
+/* quantize_i8 of the M rows of x and matmul_w8a8 in one call (up to eight tokens of small matrices: one launch).  d_ws: scratch of at least linear_w8a8_bytes(M, N, K), 256-byte aligned, used by
  * no other call at the same time; the size function returns 0 where the call needs none (d_ws may be NULL then) and an error below 0. */
 int64_t chimere_b200_linear_w8a8_bytes(int64_t M, int N, int K);
 int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,

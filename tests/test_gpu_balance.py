@@ -87,7 +87,7 @@ def bits(r, d):
     return [t.clone() for t in r] + ([] if d is None else [d.clone()])
 
 
-SHAPES = [(1, 1, 1, 1), (1, 1, 256, 8), (1, 24, 256, 8), (3, 17, 5, 2), (2, 64, 32, 4), (2, 65, 33, 3), (4, 1000, 128, 6), (5, 333, 64, 1), (1, 3000, 255, 8), (2, 2048, 60, 7), (300, 70, 16, 2), (60, 700, 40, 3), (100, 600, 64, 4), (500, 513, 8, 1), (7, 513, 256, 8),
+SHAPES = [(1, 1, 1, 1), (1, 1, 256, 8), (1, 24, 256, 8), (3, 17, 5, 2), (2, 64, 32, 4), (2, 65, 33, 3), (4, 1000, 128, 6), (5, 333, 64, 1), (1, 3000, 255, 8), (2, 2048, 60, 7), (300, 70, 16, 2), (60, 700, 40, 3), (100, 600, 64, 4), (500, 513, 8, 1), (7, 513, 256, 8), (2, 1025, 100, 4), (3, 1024, 48, 2),
           (1, 40000, 256, 8), (64, 129, 130, 256), (1, 100000, 8, 2)]
 
 
@@ -179,7 +179,7 @@ def test_values_at_the_ends_of_the_range(mode, L):
         check(r3, d3, reference(top, ids, mode=mode))
 
 
-@pytest.mark.parametrize("L", [30, 900])
+@pytest.mark.parametrize("L", [30, 900, 1900])
 def test_ids_outside_and_repeated(L):
     logits, ids = inputs(2, L, 48, 4, seed=10)
     ids[0, :, 0] = -1

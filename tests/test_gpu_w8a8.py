@@ -271,7 +271,7 @@ def test_stack_inside_a_wider_one():
 
 # ---- the chains ----
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,K,N,act", [(1, 2048, 4096, abi.ACT_NONE), (5, 77, 130, abi.ACT_SWIGLU), (8, 3000, 515, abi.ACT_RELU2), (8, 8190, 64, abi.ACT_NONE), (3, 8192, 130, abi.ACT_SWIGLU), (1, 20000, 64, abi.ACT_NONE), (200, 1000, 640, abi.ACT_RELU2), (1025, 512, 300, abi.ACT_NONE)])
+@pytest.mark.parametrize("M,K,N,act", [(1, 2048, 4096, abi.ACT_NONE), (5, 77, 130, abi.ACT_SWIGLU), (8, 3000, 515, abi.ACT_RELU2), (2, 2688, 33, abi.ACT_NONE), (7, 500, 1000, abi.ACT_SWIGLU), (6, 8192, 4100, abi.ACT_NONE), (8, 64, 20000, abi.ACT_NONE), (8, 8190, 64, abi.ACT_NONE), (3, 8192, 130, abi.ACT_SWIGLU), (1, 20000, 64, abi.ACT_NONE), (200, 1000, 640, abi.ACT_RELU2), (1025, 512, 300, abi.ACT_NONE)])
 def test_linear_is_its_two_steps(M, K, N, act, dtype):
     g = gen(M + K)
     R = 2 * N if act == abi.ACT_SWIGLU else N
