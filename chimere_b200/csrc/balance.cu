@@ -344,12 +344,6 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
 #pragma unroll 1
     for (int row0 = row_first; row0 < r1; row0 += kB_Warps * kRows * kU) {
         uint64_t v[kU][G][2];   // two values each
-#pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) v[u][j][i] = pack2f(next[u][j].value(2 * i), next[u][j].value(2 * i + 1));
         // step by step for all of the warp's rows, so that one row's exchanges between lanes pass behind the others'
         float mx[kU], sum[kU], dot[kU];
         uint64_t slope[SIGMOID ? kU : 1][G][2];   // 1 - sigmoid(l)
@@ -361,7 +355,6 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx[u] = fmaxf(mx[u], next[u][j].value(i));
         }
-        fetch(row0 + kB_Warps * kRows * kU);   // (the rows after these are on their way while these are worked on)
         lanes_max<LANES>(mx);
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
@@ -376,10 +369,9 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
             for (int j = 0; j < G; ++j)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
+                    const float a = next[u][j].value(2 * i), b = next[u][j].value(2 * i + 1);
                     uint64_t& l = v[u][j][i];
                     if (SIGMOID) {
-                        float a, b;
-                        unpack2(l, a, b);
                         const uint64_t t = exp_pair(add2(pack2f(-fabsf(a), -fabsf(b)), shift2));
                         float d0, d1;
                         unpack2(fma2(t, one2, pack2f(1.0f, 1.0f)), d0, d1);
@@ -391,7 +383,7 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
                         slope[u][j][i] = pack2f(up0 ? t0 : q0, up1 ? t1 : q1);
                         l = pack2f(up0 ? q0 : t0, up1 ? q1 : t1);
                     } else {
-                        l = exp_pair(add2(l, shift2));
+                        l = exp_pair(add2(pack2f(a, b), shift2));
                     }
                     sum2 = add2(sum2, l);
                     dot2 = fma2(l, g[j][i], dot2);
@@ -402,6 +394,7 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
             unpack2(dot2, a, b);
             dot[u] = a + b;
         }
+        fetch(row0 + kB_Warps * kRows * kU);   // (the rows after these are on their way while these are finished, and copied nowhere)
         lanes_sum<LANES>(sum);
         if (grad) lanes_sum<LANES>(dot);
 #pragma unroll
