@@ -88,7 +88,8 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, mask: Optional[to
                  coef: float = 1.0) -> BalanceLoss:
     """Loss, counts, mean probabilities and tokens of each sequence.  logits [T, E] or [S, L, E] (E <= 256) of float32, float16 or bfloat16; topk_idx int32 [..., top_k]: an
     id outside [0, E) counts nowhere; mask bool or uint8 [T] or [S, L]: tokens that are false are left out, whatever they hold.  The loss is differentiable
-    with respect to the logits (the counts are constants in it); where gradients are wanted at once, balance_loss_grad saves a pass."""
+    with respect to the logits (the counts are constants in it); where gradients are wanted at once, balance_loss_grad saves a pass.  (A backward() captured in a CUDA graph follows torch's rule: no earlier autograd graph of the same
+    leaves may be alive on another stream.  balance_loss_grad has no such rule.)"""
     a = _check(logits, topk_idx, mask, route_mode, coef)
     if torch.is_grad_enabled() and logits.requires_grad:
         return BalanceLoss(*_Loss.apply(logits, topk_idx, mask, a))

@@ -490,7 +490,7 @@ struct MatmulShared {
     uint64_t drain;
     uint32_t tmem_base;
     int failed;
-    float sx[2][64];
+    float sx[2][64];   // of a tile's tokens: scale and row of y
     int row[2][64];
 };
 
@@ -599,22 +599,20 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
         // four warps take every other tile, and look up a tile's scales and places while the one before is on its way
         const int q = warp & 3, buf = (warp - kMM_FirstEpi) >> 2, row = q * 32 + lane;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + buf * kAccCols;
-        constexpr int kPer = (BN + 127) / 128;
         bool ok = true;
         griddep_wait();   // (the tokens' scales; and nothing of y is written before what used its memory has ended)
         Tile t;
         Channel ch;
-        float sx[kPer];
-        int to[kPer];
+        float sx = 0.0f;
+        int to = -1;
+        static_assert(BN <= 128, "a token per thread");
         auto look_up = [&](int id) {
             t = take_tile<BN, 128>(p, table, id);
             ch = channel(p, DUAL, t.expert, t.n0 + row);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (row + 128 * i < t.ntok) {
-                    sx[i] = p.sx[t.row0 + row + 128 * i];
-                    to[i] = p.out_rows ? p.out_rows[t.row0 + row + 128 * i] : t.row0 + row + 128 * i;
-                }
+            if (row < t.ntok) {
+                sx = p.sx[t.row0 + row];
+                to = p.out_rows ? p.out_rows[t.row0 + row] : t.row0 + row;
+            }
         };
         int id = first + buf * step;
         if (id < total && S == 1) look_up(id);
@@ -637,9 +635,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
                 break;
             }
             asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");   // (the tile before has been read)
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (row + 128 * i < t.ntok) { sh.sx[buf][row + 128 * i] = sx[i]; sh.row[buf][row + 128 * i] = to[i]; }
+            if (row < t.ntok) { sh.sx[buf][row] = sx; sh.row[buf][row] = to; }
             asm volatile("bar.sync %0, 128;" ::"r"(1 + buf) : "memory");
             const Channel c = ch;
             const int ntok = t.ntok, n = t.n0 + row;

@@ -381,7 +381,7 @@ int chimere_b200_matmul_w8a8(const int8_t* d_x, int64_t ldx, const float* d_x_sc
                              const float* d_bias, int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy,
                              int32_t* d_status, cudaStream_t stream);
 /* The same with a matrix per group of rows: rows d_offsets[e] .. d_offsets[e + 1] (device int32 [E + 1], as chimere_b200_moe_route leaves them in
- * ws->offsets; E <= 1024) by matrix e, which starts e * stride_w bytes behind the first; w_scale and bias [E][N or 2 N].  With d_out_rows row i goes to row
+ * ws->offsets: ascending, and cut to [0, M]; E <= 1024) by matrix e, which starts e * stride_w bytes behind the first; w_scale and bias [E][N or 2 N].  With d_out_rows row i goes to row
  * d_out_rows[i] of y.  Rows in no group, and rows whose index is not in [0, y_rows), are not written. */
 int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, int64_t stride_w,
                                      const float* d_w_scale, const float* d_bias, const int32_t* d_offsets, int E, int64_t M, int N, int K,
