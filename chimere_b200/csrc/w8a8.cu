@@ -323,6 +323,7 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
         asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // TMEM -> registers, thread = lane, neighbouring columns (the wait in the same statement: no use of a value can move in front of it)
 __device__ __forceinline__ void ld16(uint32_t taddr, int* v) {
     asm volatile(
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
     const int S = p.split, rank = S > 1 ? blockIdx.x % S : 0, first = blockIdx.x / S, step = gridDim.x / S;
     const uint32_t stages = smem_u32(smem);
 
+    if (tid == 0) { prefetch_map(&map_w); prefetch_map(&map_x); }
     if (!p.early) griddep_wait();
     const int total = (p.offsets ? group_table<BN, kMM_Threads>(p, table) : p.mt) * p.nt;
     if (first >= total) {   // (the whole cluster; nothing has been allocated)
@@ -671,6 +673,9 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
     if (S > 1) {
         const Tile t = take_tile<BN, 128>(p, table, first);
         griddep_wait();
+        Channel ch[4];   // of this thread's four neighbouring outputs, the same for all of its tokens (384 is a multiple of 32)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ch[j] = channel(p, DUAL, t.expert, t.n0 + 4 * (tid & 31) + j);
         cluster_sync();   // every part is there
         bool bad = false;
         for (int s = 0; s < S; ++s) bad |= ld_cluster(cluster_addr(smem_u32(&sh.failed), s)) != 0;
@@ -690,7 +695,7 @@ __global__ void __launch_bounds__(kMM_Threads) matmul_kernel(const __grid_consta
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float o[2];
-                finish2<DUAL>(p, channel(p, DUAL, t.expert, n + j), sx, 0.0f, acc[j], 0, up[j], 0, o);
+                finish2<DUAL>(p, ch[j], sx, 0.0f, acc[j], 0, up[j], 0, o);
                 if (n + j < p.N) put(p, r * p.ldy + n + j, bad ? __uint_as_float(0x7FC00000u) : o[0]);
             }
         }
@@ -734,6 +739,7 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
     extern __shared__ __align__(16) int8_t xs[];          // [token][ks]
     __shared__ uint32_t s_max[kR_Tokens][kR_Warps];
     __shared__ float s_scale[kR_Tokens];
+    __shared__ int s_row[kR_Tokens];
     __shared__ int red[kR_Warps][TILES][16][kR_Tokens + 1];
     __shared__ int group[3];
     const MatmulParams& mp = p.m;
@@ -781,10 +787,12 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
         }
     };
     load(0);
+    const Channel ch = channel(mp, DUAL, e, n0 + tid % outs);   // (a thread's results are all of one channel: 256 is a multiple of outs)
     if (mp.early) griddep_wait();
 
     for (int c0 = start; c0 < end; c0 += kR_Tokens) {
         const int ntok = min(kR_Tokens, end - c0);
+        if (tid < ntok) s_row[tid] = mp.out_rows ? mp.out_rows[c0 + tid] : c0 + tid;
         auto source = [&](int m) -> int64_t {
             if (!p.rows) return c0 + m;
             const int r = p.rows[c0 + m], s = r < 0 ? -1 : r / p.rows_div;
@@ -900,8 +908,8 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
                 if (DUAL) up += red[w][TILES - 1][c & 15][m];
             }
             float y[2];
-            finish2<DUAL>(mp, channel(mp, DUAL, e, n), s_scale[m], 0.0f, sum, 0, up, 0, y);
-            const int64_t r = mp.out_rows ? mp.out_rows[c0 + m] : c0 + m;
+            finish2<DUAL>(mp, ch, s_scale[m], 0.0f, sum, 0, up, 0, y);
+            const int64_t r = s_row[m];
             if (r >= 0 && r < mp.y_rows) put(mp, r * mp.ldy + n, y[0]);
         }
         __syncthreads();
@@ -1018,6 +1026,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW_Threads, 1) wide_
     const int rank = blockIdx.x & 1, first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const uint32_t stages = smem_u32(smem);
 
+    if (tid == 0) { prefetch_map(&map_w); prefetch_map(&map_x); }
     if (!p.early) griddep_wait();
     const int total = (p.offsets ? group_table<kW_Tokens, kW_Threads>(p, table) : p.mt) * p.nt;
     if (first >= total) {   // (both CTAs; nothing has been allocated)
