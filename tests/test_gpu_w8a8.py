@@ -135,7 +135,7 @@ def test_quantize_rows_of_a_wider_matrix_and_gathered(dtype):
 
 # ---- dense ----
 SHAPES = [(1, 1, 1), (1, 2048, 4096), (8, 2688, 96), (5, 8192, 70), (5, 8193, 70), (8, 65, 33), (4, 4100, 515), (9, 2048, 4096), (2, 128, 128), (3, 129, 5), (7, 2688, 3712), (16, 512, 100), (17, 100, 130), (33, 2005, 257), (61, 4096, 2048), (64, 64, 64),
-          (65, 300, 700), (129, 1000, 513), (300, 640, 1000), (777, 2005, 1031), (1500, 384, 2500), (5000, 130, 260), (4000, 2048, 2048), (2300, 1000, 1024), (1111, 640, 4099), (20000, 64, 320)]
+          (65, 300, 700), (129, 1000, 513), (300, 640, 1000), (777, 2005, 1031), (1500, 384, 2500), (5000, 130, 260), (4000, 2048, 2048), (2300, 1000, 1024), (1111, 640, 4099), (20000, 64, 320), (3000, 512, 2048), (2500, 400, 1040), (40000, 128, 512)]
 
 
 @pytest.mark.parametrize("act", [abi.ACT_NONE, abi.ACT_SWIGLU, abi.ACT_RELU2])
@@ -197,7 +197,7 @@ def groups(counts, first=0):
 
 @pytest.mark.parametrize("act", [abi.ACT_NONE, abi.ACT_SWIGLU, abi.ACT_RELU2])
 @pytest.mark.parametrize("counts,K,N", [([1], 64, 64), ([0, 0, 3, 0], 100, 33), ([1, 1, 1, 1, 1, 1, 1, 1], 2048, 512), ([0] * 30 + [19, 1, 0, 8, 9], 2048, 100), ([2, 0, 0, 1], 9000, 50), ([16, 17, 0, 15, 33], 257, 130), ([300, 0, 1, 129, 64], 512, 260),
-                                        ([0] * 100 + [5] + [0] * 900 + [7], 128, 40), ([2000, 3, 700], 384, 200), ([40] * 64, 640, 192)])
+                                        ([0] * 100 + [5] + [0] * 900 + [7], 128, 40), ([2000, 3, 700], 384, 200), ([700, 0, 300, 1, 128, 129, 255, 256, 257], 512, 1024), ([3000], 100, 2000), ([40] * 64, 640, 192)])
 def test_grouped(counts, K, N, act):
     g = gen(K + N + len(counts))
     M, E, R = sum(counts), len(counts), 2 * N if act == abi.ACT_SWIGLU else N
