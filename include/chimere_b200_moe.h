@@ -1,6 +1,6 @@
 /* chimere_b200_moe.h -- C ABI of the B200 (sm_100a) quantized MoE feed-forward library.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *
  *  1. Legacy operator entries.  Same names, argument order and meaning as the reference's
  *     FFI layer (chimere-server/ffi/ggml_cuda_gemv.cu, Rust declarations in
@@ -14,7 +14,10 @@
  *     for T tokens at once.  They return int: 0 = ok, <0 = argument error found on the host
  *     before anything was launched.
  *
- * Conventions (both groups): every pointer named dev / d_* is device memory owned by the
+ *  3. Operators beside the layer: W8A8 products (linear_w8a8, matmul_w8a8, experts_w8a8) and the router's balance loss
+ *     (balance_loss).  They return int as the second group does.
+ *
+ * Conventions (all groups): every pointer named dev / d_* is device memory owned by the
  * caller; the library never allocates, frees or keeps device memory; all work is enqueued on
  * the stream passed in (NULL = legacy default stream); no entry synchronises the host unless
  * its comment says so.  Quantized weights use the ggml block layouts unchanged
