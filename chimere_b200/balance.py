@@ -8,6 +8,7 @@ What a router is trained and watched with: it takes the logits and the expert id
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -47,17 +48,23 @@ def _place(t: torch.Tensor, S: int, L: int, E: int) -> Tuple[int, int, int]:
     return t.data_ptr(), strides[-2] if L > 1 else E, strides[0] if S > 1 else 0
 
 
+@lru_cache(maxsize=4096)
+def _bytes(S: int, L: int, E: int, k: int) -> int:
+    return abi.load().chimere_b200_balance_loss_bytes(S, L, E, k)
+
+
 def _forward(logits, topk_idx, mask, a: _Args, grad_loss, d_logits) -> BalanceLoss:
     dev = logits.device
     S, L, E, k, mode, coef = a
-    nbytes = (abi._lib or abi.load()).chimere_b200_balance_loss_bytes(S, L, E, k)
+    nbytes = _bytes(S, L, E, k)
     if nbytes < 0:
         raise ValueError("logits 1 to 256 wide, 1 to 256 ids per row, fewer than 2^31 rows and ids")
-    lead = () if logits.dim() == 2 else (S,)
-    loss = torch.empty(lead, dtype=torch.float32, device=dev)
-    tokens = torch.empty(lead, dtype=torch.int32, device=dev)
-    counts = torch.empty(*lead, E, dtype=torch.int32, device=dev)
-    prob = torch.empty(*lead, E, dtype=torch.float32, device=dev)
+    if logits.dim() == 2:
+        loss, tokens = torch.empty((), dtype=torch.float32, device=dev), torch.empty((), dtype=torch.int32, device=dev)
+        counts, prob = torch.empty(E, dtype=torch.int32, device=dev), torch.empty(E, dtype=torch.float32, device=dev)
+    else:
+        loss, tokens = torch.empty(S, dtype=torch.float32, device=dev), torch.empty(S, dtype=torch.int32, device=dev)
+        counts, prob = torch.empty(S, E, dtype=torch.int32, device=dev), torch.empty(S, E, dtype=torch.float32, device=dev)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     p, ld, stride = _place(logits, S, L, E)
     dp, ldd, stride_d = (None, E, 0) if d_logits is None else _place(d_logits, S, L, E)

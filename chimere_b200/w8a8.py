@@ -8,6 +8,7 @@ int8 rows start on 16-byte boundaries: a matrix whose width is no multiple of 16
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -167,11 +168,21 @@ def linear_w8a8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
     N = _outputs(R, act)
     out, yp, kind, ldy = _output(out, M, N, out_dtype or (None if out is not None else x.dtype), x)
     wp, ldw = _weight(w, "w", index)
-    ws, nbytes = _scratch(x, (abi._lib or abi.load()).chimere_b200_linear_w8a8_bytes(M, N, K))
+    ws, nbytes = _scratch(x, _linear_bytes(M, N, K))
     _call("chimere_b200_linear_w8a8", index, xp, x_kind, ldx, wp, ldw, _vector(w_scale, "w_scale", (R,), torch.float32, index),
           _vector(bias, "bias", (R,), torch.float32, index), M, N, K, act, yp, kind, ldy, None if ws is None else ws.data_ptr(), nbytes,
           _vector(status, "status", (1,), torch.int32, index))
     return out
+
+
+@lru_cache(maxsize=4096)
+def _linear_bytes(M: int, N: int, K: int) -> int:
+    return abi.load().chimere_b200_linear_w8a8_bytes(M, N, K)
+
+
+@lru_cache(maxsize=4096)
+def _experts_bytes(T: int, top_k: int, H: int, F: int) -> int:
+    return abi.load().chimere_b200_experts_w8a8_bytes(T, top_k, H, F)
 
 
 def _scratch(like: torch.Tensor, nbytes: int) -> Tuple[Optional[torch.Tensor], int]:
@@ -196,7 +207,7 @@ def experts_w8a8(x: torch.Tensor, perm: torch.Tensor, offsets: torch.Tensor, top
     out, yp, kind, ldy = _output(out, P, H, out_dtype or (None if out is not None else x.dtype), x)
     up, ld_up, plane_up = _stack(w_up, "w_up", index)
     down, ld_down, plane_down = _stack(w_down, "w_down", index)
-    ws, nbytes = _scratch(x, (abi._lib or abi.load()).chimere_b200_experts_w8a8_bytes(T, top_k, H, F))
+    ws, nbytes = _scratch(x, _experts_bytes(T, top_k, H, F))
     _call("chimere_b200_experts_w8a8", index, xp, x_kind, ldx, T, _vector(perm, "perm", (P,), torch.int32, index),
           _vector(offsets, "offsets", (E + 1,), torch.int32, index), top_k, E, up, ld_up, plane_up, _vector(up_scale, "up_scale", (E, R), torch.float32, index),
           down, ld_down, plane_down, _vector(down_scale, "down_scale", (E, H), torch.float32, index), H, F, act, yp, kind, ldy,
