@@ -1461,6 +1461,17 @@ int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w,
     if (misaligned(x, 16) || misaligned(w, 16) || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4) || misaligned(y, type_size(y_type)) || misaligned(out_rows, 4)) return -5;
     return 0;
 }
+// Rows of `bytes` bytes each, `pitch` apart.  Two matrices share memory if their ranges do, but for such with one pitch that lie side by side.
+struct RowsRange { uintptr_t at; int64_t pitch, bytes, rows; };
+bool share_memory(const RowsRange& a, const RowsRange& b) {
+    if (a.rows == 0 || b.rows == 0) return false;
+    const uintptr_t a_end = a.at + (uintptr_t)(a.pitch * (a.rows - 1) + a.bytes), b_end = b.at + (uintptr_t)(b.pitch * (b.rows - 1) + b.bytes);
+    if (a_end <= b.at || b_end <= a.at) return false;
+    if (a.rows == 1 || b.rows == 1 || a.pitch != b.pitch) return true;
+    const RowsRange &lo = a.at <= b.at ? a : b, &hi = a.at <= b.at ? b : a;
+    const int64_t off = (int64_t)((hi.at - lo.at) % (uintptr_t)a.pitch);
+    return off < lo.bytes || off + hi.bytes > a.pitch;
+}
 MatmulCall matmul_call(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, const int32_t* offsets, int E,
                        int64_t M, int N, int K, int act, void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows, int32_t* status, bool early) {
     MatmulCall c{};
@@ -1532,6 +1543,9 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
     rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
     if (rc || M == 0) return rc;
     if (ws_bytes < ws.at) return -4;
+    // in one launch some CTAs still read x when others store y
+    const int x_size = type_size(x_type), y_size = type_size(y_type);
+    if (none && share_memory({(uintptr_t)d_x, ldx * x_size, (int64_t)K * x_size, M}, {(uintptr_t)d_y, ldy * y_size, (int64_t)N * y_size, M})) return -2;
     return launch_linear(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, false),
                          QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, true, nullptr, nullptr, stream);
 }

@@ -161,18 +161,37 @@ def matmul_w8a8_grouped(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor,
 
 def linear_w8a8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, act: int = abi.ACT_NONE,
                 out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """matmul_w8a8(*quantize_i8(x), w, w_scale, ...) in one call.  out_dtype: that of x unless given."""
+    """matmul_w8a8(*quantize_i8(x), w, w_scale, ...) in one call.  out_dtype: that of x unless given.  `out` may share memory with x."""
     M, K, xp, x_kind, ldx = _floats(x, "x")
     _need(w.dim() == 2 and w.shape[1] == K, "x [M, K] and w [N, K]")
     index, R = x.get_device(), w.shape[0]
     N = _outputs(R, act)
+    given = out
     out, yp, kind, ldy = _output(out, M, N, out_dtype or (None if out is not None else x.dtype), x)
     wp, ldw = _weight(w, "w", index)
     ws, nbytes = _scratch(x, _linear_bytes(M, N, K))
+    if given is not None and nbytes == 0 and _share_memory(x, ldx, out, ldy):     # (what needs no scratch is one launch, which stores while it reads)
+        return matmul_w8a8(*quantize_i8(x), w, w_scale, bias, act, out=out, status=status)
     _call("chimere_b200_linear_w8a8", index, xp, x_kind, ldx, wp, ldw, _vector(w_scale, "w_scale", (R,), torch.float32, index),
           _vector(bias, "bias", (R,), torch.float32, index), M, N, K, act, yp, kind, ldy, None if ws is None else ws.data_ptr(), nbytes,
           _vector(status, "status", (1,), torch.int32, index))
     return out
+
+
+def _share_memory(a: torch.Tensor, lda: int, b: torch.Tensor, ldb: int) -> bool:
+    """Whether two matrices' ranges meet, but for matrices side by side in one wider one."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (rows, wa), (rows_b, wb) = ((t.shape[0], t.shape[1] * t.element_size()) for t in (a, b))
+    pitch, pitch_b, lo, hi = lda * a.element_size(), ldb * b.element_size(), a.data_ptr(), b.data_ptr()
+    if lo + pitch * (rows - 1) + wa <= hi or hi + pitch_b * (rows_b - 1) + wb <= lo:
+        return False
+    if rows == 1 or rows_b == 1 or pitch != pitch_b:
+        return True
+    if lo > hi:
+        lo, hi, wa, wb = hi, lo, wb, wa
+    off = (hi - lo) % pitch
+    return off < wa or off + wb > pitch
 
 
 @lru_cache(maxsize=4096)
@@ -196,7 +215,7 @@ def experts_w8a8(x: torch.Tensor, perm: torch.Tensor, offsets: torch.Tensor, top
                  status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows [T * top_k, H] of the routed pairs: down_e . act(gate|up_e . x[pair // top_k]), pair by pair (row t * top_k + j is slot j of token t).  perm int32 [T * top_k]
     and offsets int32 [E + 1]: the router's dispatch (MoeScratch.perm / .offsets).  w_up int8 [E, 2 F, H] (gate rows, then up) for ACT_SWIGLU, [E, F, H] for
-    ACT_RELU2; w_down int8 [E, H, F]; scales f32 [E, rows].  Pairs of no expert are not written (without `out`: not initialised).  out_dtype: that of x."""
+    ACT_RELU2; w_down int8 [E, H, F]; scales f32 [E, rows].  Pairs of no expert are not written (without `out`: not initialised).  out_dtype: that of x.  `out` may share memory with x."""
     T, H, xp, x_kind, ldx = _floats(x, "x")
     _need(act in (abi.ACT_SWIGLU, abi.ACT_RELU2), "act: ACT_SWIGLU or ACT_RELU2")
     _need(w_up.dim() == 3 and w_down.dim() == 3, "w_up [E, F or 2 F, H], w_down [E, H, F]")

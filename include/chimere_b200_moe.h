@@ -368,6 +368,7 @@ int chimere_b200_moe_ep_pack_sorted(const chimere_moe_layer* w, int T, chimere_m
  * form int8 checkpoints have for the projections around the MoE layer and for experts.  No counterpart in the reference, whose weights
  * are ggml blocks.  Rows of int8 start on 16-byte boundaries (base and row stride multiples of 16 bytes; the bytes behind a row's K values
  * are not looked at); K <= 131071, so that every sum is exact in 32 bits.  *_type: CHIMERE_TYPE_F32, _F16 or _BF16.  M = 0 is no work.
+ * Outputs and scratch share no memory with anything else a call reads or writes, except where its comment allows it.
  * d_status (may be NULL): raised if a bounded wait ran out; the outputs concerned are NaN then.
  * Errors: -1 null pointer, -2 bad dimension, -3 type, -4 workspace too small, -5 misaligned, -6 driver without tensor maps. */
 
@@ -392,7 +393,8 @@ int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float
                                      int32_t* d_status, cudaStream_t stream);
 
 /* quantize_i8 of the M rows of x and matmul_w8a8 in one call (up to eight tokens of small matrices: one launch).  d_ws: scratch of at least linear_w8a8_bytes(M, N, K), 256-byte aligned, used by
- * no other call at the same time; the size function returns 0 where the call needs none (d_ws may be NULL then) and an error below 0. */
+ * no other call at the same time; the size function returns 0 where the call needs none (d_ws may be NULL then) and an error below 0.  y may share memory
+ * with x where the call needs scratch (x has been read when y is written); where it needs none such a call is refused (-2). */
 int64_t chimere_b200_linear_w8a8_bytes(int64_t M, int N, int K);
 int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias,
                              int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes,
@@ -401,7 +403,7 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
 /* Routed experts in W8A8 behind the router of this library: y[pair] = down_e . act(gate|up_e . x[pair / top_k]) for the T * top_k pairs, e the expert whose range
  * of d_perm (d_offsets[e] .. d_offsets[e + 1]) holds the pair; d_perm and d_offsets as chimere_b200_moe_route / _permute leave them.  The rows between the two products
  * are held in f32 and quantised by token again.  w_up [E][2 F (SWIGLU: gate rows, then up) or F (RELU2)][H], w_down [E][H][F].  Rows of y whose pair is in no expert's range are
- * not written.  Scratch as above. */
+ * not written; y may share memory with x.  Scratch as above. */
 int64_t chimere_b200_experts_w8a8_bytes(int64_t T, int top_k, int H, int F);
 int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t T, const int32_t* d_perm, const int32_t* d_offsets, int top_k, int E,
                               const int8_t* d_w_up, int64_t ld_up, int64_t stride_up, const float* d_up_scale,
