@@ -5,6 +5,8 @@
 //         product           y[m][n] = act( (sum_k xq[m][k] * wq[n][k]) * sx[m] * sw[n] + bias[n] )
 // The sums are exact (int32; |sum| <= 128 * 128 * K < 2^31 for K <= 131071), everything behind them is fp32, and the result is rounded
 // once to the output's type.
+// Rows, scales and activations are read by ordinary loads: within a call the kernel in front may still be writing them when a grid starts, so they are no read-only
+// data of that grid.  The weights are, and go past the L1 cache by non-coherent loads or by TMA.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -46,7 +48,7 @@ template <int TYPE> struct Elem {   // eight values as they lie in memory
         Raw r;
 #pragma unroll
         for (int i = 0; i < kWords / 4; ++i) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            const uint4 a = reinterpret_cast<const uint4*>(p)[i];
             r.w[4 * i] = a.x; r.w[4 * i + 1] = a.y; r.w[4 * i + 2] = a.z; r.w[4 * i + 3] = a.w;
         }
         return r;
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const int8_t* from, co
     for (int j = lane; j < n; j += 128) {
         uint4 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = j + 32 * u < n && there ? __ldg(a + j + 32 * u) : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < 4; ++u) v[u] = j + 32 * u < n && there ? a[j + 32 * u] : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int u = 0; u < 4; ++u) if (j + 32 * u < n) b[j + 32 * u] = v[u];
     }
@@ -419,7 +421,7 @@ __device__ __forceinline__ Tile take_tile(const MatmulParams& p, const GroupTabl
     const int c = g.prefix[lo + 1] - g.prefix[lo], local = id - g.prefix[lo] * p.nt, m = local % c, start = g.start[lo];
     t.expert = lo;
     t.row0 = start + m * TOKENS;
-    t.ntok = min(TOKENS, min(max(__ldg(p.offsets + lo + 1), start), p.M) - t.row0);
+    t.ntok = min(TOKENS, min(max(p.offsets[lo + 1], start), p.M) - t.row0);
     t.n0 = local / c * OUTS;
     return t;
 }
@@ -806,7 +808,7 @@ __global__ void __launch_bounds__(kR_Threads) rows_kernel(const __grid_constant_
                 const int8_t* x = reinterpret_cast<const int8_t*>(p.x) + (int64_t)(c0 + m) * p.ldx;
                 for (int i = tid; i < 4 * units; i += kR_Threads) {
                     uint4 q = make_uint4(0, 0, 0, 0);
-                    if (16 * i < K) q = __ldg(reinterpret_cast<const uint4*>(x) + i);
+                    if (16 * i < K) q = reinterpret_cast<const uint4*>(x)[i];
                     uint32_t* w = reinterpret_cast<uint32_t*>(&q);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {   // (nothing behind the row's last value)
