@@ -1423,6 +1423,7 @@ int launch_linear(MatmulCall c, QuantParams x, int x_type, bool first, int8_t* a
     x.vec = ((uintptr_t)x.x & 15) == 0 && (x.ldx * (x_type == kF32 ? 4 : 2)) % 16 == 0;
     c.p.early = !first;
     if (few_values(c)) return launch_rows_any(c, &x, x_type, !first, stream);
+    if (!x.q || !x.scale) return -4;      // (what is left needs room for the quantised rows)
     if (!few_tokens(c) && !encoder()) return -6;
     QuantParams once = x;
     if (apart) { once.rows = nullptr; once.rows_div = 1; once.M = x.x_rows; once.q = apart; once.scale = apart_scale; }
@@ -1440,17 +1441,19 @@ inline bool float_type(int t) { return t == kF32 || t == kF16 || t == kBF16; }
 inline int type_size(int t) { return t == kF32 ? 4 : 2; }
 inline bool misaligned(const void* p, int to) { return ((uintptr_t)p & (uintptr_t)(to - 1)) != 0; }
 
-int check_quantize(const void* x, int type, int64_t ldx, int64_t x_rows, const int32_t* rows, int rows_div, int64_t M, int K, const int8_t* q, int64_t ldq, const float* scale) {
+// (one_launch: the quantised rows and their scales stay in the product's CTAs, q and scale are null)
+int check_quantize(const void* x, int type, int64_t ldx, int64_t x_rows, const int32_t* rows, int rows_div, int64_t M, int K, const int8_t* q, int64_t ldq, const float* scale,
+                   bool one_launch = false) {
     if (M < 0 || M > 0x7FFFFFFF || x_rows < 0 || K <= 0 || K > kMaxK || ldx < K || ldq < K || ldq % 16 || rows_div <= 0) return -2;
     if (!float_type(type)) return -3;
     if (!rows && x_rows < M) return -2;
     if (M == 0) return 0;
-    if ((!x && x_rows > 0) || !q || !scale) return -1;
+    if ((!x && x_rows > 0) || (!one_launch && (!q || !scale))) return -1;
     if (misaligned(x, type_size(type)) || misaligned(q, 16) || misaligned(scale, 4) || misaligned(rows, 4)) return -5;
     return 0;
 }
 int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, int E, int64_t M, int N, int K,
-                 int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows) {
+                 int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows, bool one_launch = false) {
     const int64_t R = (act == CHIMERE_ACT_SWIGLU ? 2 : 1) * (int64_t)N;
     if (M < 0 || M > 0x7FFFFFFF || N <= 0 || R > 0x7FFFFF00 || K <= 0 || K > kMaxK || E <= 0 || E > kMaxGroups) return -2;
     if (ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldy < N || y_rows < 0) return -2;
@@ -1459,7 +1462,7 @@ int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w,
     if (!float_type(y_type)) return -3;
     if (!out_rows && y_rows < M) return -2;
     if (M == 0) return 0;
-    if (!x || !sx || !w || !sw || (!y && y_rows > 0)) return -1;
+    if ((!one_launch && (!x || !sx)) || !w || !sw || (!y && y_rows > 0)) return -1;
     if (misaligned(x, 16) || misaligned(w, 16) || misaligned(sx, 4) || misaligned(sw, 4) || misaligned(bias, 4) || misaligned(y, type_size(y_type)) || misaligned(out_rows, 4)) return -5;
     return 0;
 }
@@ -1534,20 +1537,21 @@ int64_t chimere_b200_linear_w8a8_bytes(int64_t M, int N, int K) {
 
 int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int8_t* d_w, int64_t ldw, const float* d_w_scale, const float* d_bias, int64_t M, int N, int K,
                              int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes, int32_t* d_status, cudaStream_t stream) {
+    const bool one_launch = few_values(M, N, K);
+    const int64_t rows = M < 0 ? 0 : M;
     Carver ws{(uint8_t*)d_ws, 0};
-    const bool none = few_values(M, N, K);      // (no scratch; the pointers below are not used then)
-    int8_t* q = none ? (int8_t*)256 : (int8_t*)ws.take((size_t)(M < 0 ? 0 : M) * up16(K));
-    float* scale = none ? (float*)256 : (float*)ws.take((size_t)(M < 0 ? 0 : M) * 4);
-    if (M > 0 && !none && !d_ws) return -1;
+    int8_t* q = one_launch ? nullptr : (int8_t*)ws.take((size_t)rows * up16(K));
+    float* scale = one_launch ? nullptr : (float*)ws.take((size_t)rows * 4);
+    if (M > 0 && !one_launch && !d_ws) return -1;
     if (misaligned(d_ws, 256)) return -5;
-    int rc = check_quantize(d_x, x_type, ldx, M, nullptr, 1, M, K, q, up16(K), scale);
+    int rc = check_quantize(d_x, x_type, ldx, M, nullptr, 1, M, K, q, up16(K), scale, one_launch);
     if (rc) return rc;
-    rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr);
+    rc = check_matmul(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, one_launch);
     if (rc || M == 0) return rc;
     if (ws_bytes < ws.at) return -4;
     // in one launch some CTAs still read x when others store y
     const int x_size = type_size(x_type), y_size = type_size(y_type);
-    if (none && share_memory({(uintptr_t)d_x, ldx * x_size, (int64_t)K * x_size, M}, {(uintptr_t)d_y, ldy * y_size, (int64_t)N * y_size, M})) return -2;
+    if (one_launch && share_memory({(uintptr_t)d_x, ldx * x_size, (int64_t)K * x_size, M}, {(uintptr_t)d_y, ldy * y_size, (int64_t)N * y_size, M})) return -2;
     return launch_linear(matmul_call(q, up16(K), scale, d_w, ldw, 0, d_w_scale, d_bias, nullptr, 1, M, N, K, act, d_y, y_type, ldy, M, nullptr, d_status, false),
                          QuantParams{d_x, ldx, M, nullptr, 1, K, q, up16(K), scale, M, 0}, x_type, true, nullptr, nullptr, stream);
 }
