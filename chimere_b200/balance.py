@@ -12,6 +12,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import abi
 from .w8a8 import _TYPES, _call
@@ -32,6 +33,8 @@ def _check(logits, topk_idx, mask, route_mode, coef) -> _Args:
     shape, index = logits.shape, logits.get_device()
     if index < 0 or len(shape) not in (2, 3) or logits.dtype not in _TYPES:
         raise ValueError("logits: [T, E] or [S, L, E] of float32, float16 or bfloat16 on a CUDA device")
+    if unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("logits: a dual tensor (there is no forward mode, its tangent would be lost)")
     if logits.stride(-1) != 1 and shape[-1] != 1:
         raise ValueError("logits: the values of a row lie side by side")
     if topk_idx.dtype is not torch.int32 or topk_idx.get_device() != index or topk_idx.shape[:-1] != shape[:-1] or not topk_idx.is_contiguous():
@@ -95,7 +98,7 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, mask: Optional[to
                  coef: float = 1.0) -> BalanceLoss:
     """Loss, counts, mean probabilities and tokens of each sequence.  logits [T, E] or [S, L, E] (E <= 256) of float32, float16 or bfloat16; topk_idx int32 [..., top_k]: an
     id outside [0, E) counts nowhere; mask bool or uint8 [T] or [S, L]: tokens that are false are left out, whatever they hold.  The loss is differentiable
-    with respect to the logits (the counts are constants in it); where gradients are wanted at once, balance_loss_grad saves a pass.  (A backward() captured in a CUDA graph follows torch's rule: no earlier autograd graph of the same
+    with respect to the logits (the counts are constants in it); where gradients are wanted at once, balance_loss_grad saves a pass.  There is no forward mode: a dual tensor is refused.  (A backward() captured in a CUDA graph follows torch's rule: no earlier autograd graph of the same
     leaves may be alive on another stream.  balance_loss_grad has no such rule.)"""
     a = _check(logits, topk_idx, mask, route_mode, coef)
     if torch.is_grad_enabled() and logits.requires_grad:

@@ -2,7 +2,7 @@
 
 The form int8 checkpoints have for the projections around the MoE layer and for experts.  The reference has no counterpart: its
 weights are ggml blocks.  Every computation happens in the CUDA library; torch owns memory and streams.  All launches go to torch's
-current stream of the tensors' device, nothing synchronises, and every call can be captured in a CUDA graph.
+current stream of the tensors' device, nothing synchronises, and every call can be captured in a CUDA graph.  Nothing here is differentiable: results carry no gradient and no tangent.
 
 int8 rows start on 16-byte boundaries: a matrix whose width is no multiple of 16 lies in rows that are wider (`padded_i8`).
 """
