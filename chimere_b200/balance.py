@@ -15,7 +15,7 @@ import torch
 from torch.autograd.forward_ad import unpack_dual
 
 from . import abi
-from .w8a8 import _TYPES, _call
+from .w8a8 import _TYPES, _call, _ints
 
 
 class BalanceLoss(NamedTuple):
@@ -42,6 +42,7 @@ def _check(logits, topk_idx, mask, route_mode, coef) -> _Args:
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.get_device() != index or mask.shape != shape[:-1] or not mask.is_contiguous()):
         raise ValueError("mask: contiguous bool or uint8, one value per row of logits")
     S, L, E = shape if len(shape) == 3 else (1, *shape)
+    _ints(E, topk_idx.shape[-1], route_mode)
     return S, L, E, topk_idx.shape[-1], route_mode, float(coef)
 
 
@@ -128,6 +129,7 @@ def balance_loss_backward(logits: torch.Tensor, counts: torch.Tensor, tokens: to
     """The gradient of the logits from a balance_loss result's counts and tokens -- or from those of several ranks, added up, for a loss over the
     whole batch."""
     S, L, E, _, mode, coef = _check(logits, torch.empty(*logits.shape[:-1], 0, dtype=torch.int32, device=logits.device), mask, route_mode, coef)
+    _ints(top_k)
     lead = logits.shape[:-2]
     for t, s, name in ((counts, (*lead, E), "counts"), (tokens, lead, "tokens")):
         if t.dtype is not torch.int32 or t.get_device() != logits.get_device() or t.shape != s or not t.is_contiguous():

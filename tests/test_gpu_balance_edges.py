@@ -30,3 +30,16 @@ def test_forward_mode_is_refused():
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda l: balance.balance_loss(l, ids).loss, (logits,), (tangent,))
     assert torch.equal(balance.balance_loss(logits, ids).loss, r.loss)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """What the C entry would see cut to 32 bits."""
+    logits, ids = inputs(1, 4, 16, 2)
+    wide = torch.zeros(1, 2 ** 32 + 16, dtype=torch.float16, device="cuda")
+    r = balance.balance_loss(logits, ids)
+    calls = [lambda: balance.balance_loss(wide, ids[0, :1]), lambda: balance.balance_loss_grad(wide, ids[0, :1]), lambda: balance.balance_loss(logits, ids, route_mode=2 ** 32),
+             lambda: balance.balance_loss_backward(logits, r.counts, r.tokens, 2 ** 32 + 2), lambda: balance.balance_loss_backward(logits, r.counts, r.tokens, 2, route_mode=2 ** 32)]
+    for i, f in enumerate(calls):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was taken")

@@ -69,3 +69,20 @@ def test_experts_over_their_own_rows(T):
         want = w8a8.experts_w8a8(x, perm, off, 1, wu, su, wd, sd)
         on_a_busy_gpu(lambda: w8a8.experts_w8a8(x, perm, off, 1, wu, su, wd, sd, out=x))
         assert torch.equal(x, want)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """What the C entry would see cut to 32 bits."""
+    g = gen(3)
+    x, w, sw = torch.randn(4, 64, generator=g, device="cuda"), i8(g, 32, 64), scales(g, 32)
+    q, s = w8a8.quantize_i8(x)
+    rows, off = torch.arange(4, dtype=torch.int32, device="cuda"), torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    wide = torch.ones(1, 2 ** 32 + 64, dtype=torch.float16, device="cuda")
+    calls = [lambda: w8a8.quantize_i8(x, rows, 2 ** 32 + 1), lambda: w8a8.quantize_i8(wide), lambda: w8a8.quantize_i8(wide, rows[:1], 1),
+             lambda: w8a8.linear_w8a8(x, w, sw, act=2 ** 32 + abi.ACT_RELU2), lambda: w8a8.matmul_w8a8(q, s, w, sw, act=2 ** 32 + abi.ACT_RELU2),
+             lambda: w8a8.matmul_w8a8_grouped(q, s, w[None], sw[None], off, act=2 ** 32 + abi.ACT_RELU2),
+             lambda: w8a8.experts_w8a8(x, rows, off, 2 ** 32 + 1, w[None], sw[None], i8(g, 1, 64, 32), scales(g, 1, 64), act=abi.ACT_RELU2)]
+    for i, f in enumerate(calls):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was taken")
