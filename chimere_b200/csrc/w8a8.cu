@@ -21,6 +21,7 @@ namespace {
 constexpr int kF32 = CHIMERE_TYPE_F32, kF16 = CHIMERE_TYPE_F16, kBF16 = CHIMERE_TYPE_BF16;
 constexpr int kMaxGroups = 1024;
 constexpr int kMaxK = 131071;
+constexpr int64_t kMaxRows = 0x7FFFFF00;   // of a product: a tile's last row, filled up, is counted in 32 bits
 
 // ------------------------------------------------------------------ rows -> int8 ----
 // A row by GROUP threads, which keep it as it came (16 bytes of kQ_Vecs pieces each) between the maximum and the division, so that it is read
@@ -1455,7 +1456,7 @@ int check_quantize(const void* x, int type, int64_t ldx, int64_t x_rows, const i
 int check_matmul(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, int64_t w_plane, const float* sw, const float* bias, int E, int64_t M, int N, int K,
                  int act, const void* y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* out_rows, bool one_launch = false) {
     const int64_t R = (act == CHIMERE_ACT_SWIGLU ? 2 : 1) * (int64_t)N;
-    if (M < 0 || M > 0x7FFFFFFF || N <= 0 || R > 0x7FFFFF00 || K <= 0 || K > kMaxK || E <= 0 || E > kMaxGroups) return -2;
+    if (M < 0 || M > kMaxRows || N <= 0 || R > 0x7FFFFF00 || K <= 0 || K > kMaxK || E <= 0 || E > kMaxGroups) return -2;
     if (ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldy < N || y_rows < 0) return -2;
     if (E > 1 && (w_plane % 16 || w_plane < (R - 1) * ldw + K)) return -2;
     if (act != CHIMERE_ACT_NONE && act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
@@ -1531,7 +1532,7 @@ int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float
 }
 
 int64_t chimere_b200_linear_w8a8_bytes(int64_t M, int N, int K) {
-    if (M < 0 || M > 0x7FFFFFFF || N <= 0 || K <= 0 || K > kMaxK) return -2;
+    if (M < 0 || M > kMaxRows || N <= 0 || K <= 0 || K > kMaxK) return -2;
     return M == 0 || few_values(M, N, K) ? 0 : (int64_t)rows_bytes(M, K);
 }
 
@@ -1557,7 +1558,7 @@ int chimere_b200_linear_w8a8(const void* d_x, int x_type, int64_t ldx, const int
 }
 
 int64_t chimere_b200_experts_w8a8_bytes(int64_t T, int top_k, int H, int F) {
-    if (T < 0 || top_k <= 0 || T > 0x7FFFFFFF / top_k || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return -2;
+    if (T < 0 || top_k <= 0 || T > kMaxRows / top_k || H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return -2;
     const int64_t pairs = T * top_k;
     return (int64_t)(rows_bytes(pairs, H) + rows_bytes(pairs, F) + up256((size_t)pairs * up8(F) * 4) + (gather_apart(pairs, top_k, H) ? rows_bytes(T, H) : 0));
 }
@@ -1566,7 +1567,7 @@ int chimere_b200_experts_w8a8(const void* d_x, int x_type, int64_t ldx, int64_t 
                               const int8_t* d_w_up, int64_t ld_up, int64_t stride_up, const float* d_up_scale,
                               const int8_t* d_w_down, int64_t ld_down, int64_t stride_down, const float* d_down_scale,
                               int H, int F, int act, void* d_y, int y_type, int64_t ldy, void* d_ws, size_t ws_bytes, int32_t* d_status, cudaStream_t stream) {
-    if (T < 0 || top_k <= 0 || T > 0x7FFFFFFF / top_k) return -2;
+    if (T < 0 || top_k <= 0 || T > kMaxRows / top_k) return -2;
     if (H <= 0 || F <= 0 || H > kMaxK || F > kMaxK) return -2;
     if (act != CHIMERE_ACT_SWIGLU && act != CHIMERE_ACT_RELU2) return -2;
     const int64_t P = T * top_k;

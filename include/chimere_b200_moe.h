@@ -367,7 +367,8 @@ int chimere_b200_moe_ep_pack_sorted(const chimere_moe_layer* w, int T, chimere_m
 /* Matrices of 8-bit integers with one f32 scale per output channel, times rows of 8-bit integers with one f32 scale per token: the
  * form int8 checkpoints have for the projections around the MoE layer and for experts.  No counterpart in the reference, whose weights
  * are ggml blocks.  Rows of int8 start on 16-byte boundaries (base and row stride multiples of 16 bytes; the bytes behind a row's K values
- * are not looked at); K <= 131071, so that every sum is exact in 32 bits.  *_type: CHIMERE_TYPE_F32, _F16 or _BF16.  M = 0 is no work.
+ * are not looked at); K <= 131071, so that every sum is exact in 32 bits.  *_type: CHIMERE_TYPE_F32, _F16 or _BF16.  M = 0 is no work;
+ * a product takes up to 0x7FFFFF00 rows.
  * Outputs and scratch share no memory with anything else a call reads or writes, except where its comment allows it.
  * d_status (may be NULL): raised if a bounded wait ran out; the outputs concerned are NaN then.
  * Errors: -1 null pointer, -2 bad dimension, -3 type, -4 workspace too small, -5 misaligned, -6 driver without tensor maps. */
