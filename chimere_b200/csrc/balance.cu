@@ -15,6 +15,8 @@
 // that remains does not lose the digits of the load all experts share.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -23,6 +25,7 @@ namespace {
 
 constexpr int kB_Threads = 256, kB_Warps = kB_Threads / 32;
 constexpr int kB_CtasPerSm = 3;
+constexpr int kB_Turns = 16, kB_LongTurns = 64;   // of a warp, between two sums in fp64; from more turns than these on
 constexpr int kB_Group = 32;          // pieces that are added up together, and groups of them
 constexpr int kB_CountCluster = 8, kB_MaxCountPieces = 16;
 constexpr int kB_CountIds = 4096;     // ids of a counting CTA, where that gives few enough of them
@@ -233,19 +236,19 @@ __device__ __forceinline__ uint64_t exp_pair(uint64_t x) {
     return fma2(e, r, e);
 }
 
-struct BalanceShared {
+template <class Part> struct BalanceShared {
     int hist[kMaxExperts + 1];        // of the whole sequence; [E]: tokens
     int mine[kMaxExperts + 1];        // of this CTA's rows (cluster)
     float sums[kMaxExperts];          // ... and their probabilities
     float g[kMaxExperts];
-    float part[kB_Warps][kMaxExperts];
+    Part part[kB_Warps][kMaxExperts];
     double sum[kB_Warps];
     int last;
 };
 
 // prob and loss from the probabilities' sums: sum_of(e), thread e % kB_Threads asks
-template <class Sum>
-__device__ __forceinline__ void finish_sequence(const BalanceParams& p, BalanceShared& sh, int s, Sum sum_of) {
+template <class Shared, class Sum>
+__device__ __forceinline__ void finish_sequence(const BalanceParams& p, Shared& sh, int s, Sum sum_of) {
     const int n = sh.hist[p.E], tid = threadIdx.x;
     double dot = 0.0;
     for (int e = tid; e < p.E; e += kB_Threads) {
@@ -268,10 +271,15 @@ __device__ __forceinline__ void finish_sequence(const BalanceParams& p, BalanceS
 
 // A row by LANES lanes, G groups of four values each: lane i owns values 4 (i + LANES g) .. + 3.
 // FULL: as many logits as the lanes hold, rows that are read and written four values at a time: no lane looks at what it has.
-template <int TYPE, int LANES, int G, bool SIGMOID, bool FULL>
+// LONG: pieces of more than kB_LongTurns turns of a warp.  A lane adds up a probability per row of its own, off by their number in half-steps of fp32 at most (mean
+// probabilities of 2^23 equal rows were 437 off), so there the sums of kB_Turns turns are added up in fp64.  A kernel of its own: in the other one the second loop costs up to a
+// quarter in spilled registers (8 x 8192 x 255 bf16 sigmoid 37.5 us, 48.6 with it) and 0.4 us of 4 in small calls.
+template <int G> __host__ __device__ constexpr int rows_at_a_time() { return G == 2 ? 2 : 4; }
+template <int LANES, int G> __host__ __device__ constexpr int turn_rows() { return kB_Warps * (32 / LANES) * rows_at_a_time<G>(); }
+template <int TYPE, int LANES, int G, bool SIGMOID, bool FULL, bool LONG>
 __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(BalanceParams p) {
-    constexpr int kRows = 32 / LANES, kU = G == 2 ? 2 : 4;   // rows of a warp at a time: kRows * kU
-    __shared__ BalanceShared sh;
+    constexpr int kRows = 32 / LANES, kU = rows_at_a_time<G>(), kStep = turn_rows<LANES, G>();   // rows of a warp at a time: kRows * kU
+    __shared__ BalanceShared<typename std::conditional<LONG, double, float>::type> sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / LANES, i4 = 4 * (lane % LANES);
     const int s = blockIdx.x / p.pieces, piece = blockIdx.x % p.pieces;
     const int r0 = (int)min((int64_t)piece * p.rows, (int64_t)p.L), r1 = (int)min((int64_t)r0 + p.rows, (int64_t)p.L);
@@ -342,8 +350,16 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
             g[j][i] = pack2f(grad && e < p.E ? sh.g[e] : 0.0f, grad && e + 1 < p.E ? sh.g[e + 1] : 0.0f);
         }
 
+    if (LONG) {
+        for (int e = lane; e < p.E; e += 32) sh.part[warp][e] = 0;
+        __syncwarp();
+    }
+    int row0 = row_first;
 #pragma unroll 1
-    for (int row0 = row_first; row0 < r1; row0 += kB_Warps * kRows * kU) {
+    do {
+    const int turns_end = LONG ? min(r1, row0 + kB_Turns * kStep) : r1;
+#pragma unroll 1
+    for (; row0 < turns_end; row0 += kStep) {
         uint64_t v[kU][G][2];   // two values each
         // step by step for all of the warp's rows, so that one row's exchanges between lanes pass behind the others'
         float mx[kU], sum[kU], dot[kU];
@@ -395,7 +411,7 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
             unpack2(dot2, a, b);
             dot[u] = a + b;
         }
-        fetch(row0 + kB_Warps * kRows * kU);   // (the rows after these are on their way while these are finished, and copied nowhere)
+        fetch(row0 + kStep);   // (the rows after these are on their way while these are finished, and copied nowhere)
         lanes_sum<LANES>(sum);
         if (grad) lanes_sum<LANES>(dot);
 #pragma unroll
@@ -430,10 +446,11 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
             }
         }
     }
-    griddep_launch();
-    if (!stats) return;
-
-    // the piece's sums: over the rows of a warp, then over the warps
+    if (!LONG) {
+        griddep_launch();
+        if (!stats) return;
+    }
+    // the sums of these turns over the rows of a warp
 #pragma unroll
     for (int j = 0; j < G; ++j)
 #pragma unroll
@@ -444,8 +461,17 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
 #pragma unroll
             for (int d = LANES; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
             const int e = i4 + 4 * LANES * j + i;
-            if (sub == 0 && e < p.E) sh.part[warp][e] = v;
+            if (sub == 0 && e < p.E) {
+                if (LONG) sh.part[warp][e] += v;
+                else sh.part[warp][e] = v;
+            }
         }
+    if (LONG) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) acc[j][0] = acc[j][1] = 0;
+    }
+    } while (LONG && row0 < r1);
+    if (LONG) griddep_launch();
     __syncthreads();
     auto of_piece = [&](int e) {
         double v = 0.0;
@@ -517,11 +543,18 @@ cudaError_t launch_balance_type(const BalanceParams& p, cudaStream_t stream) {
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.numAttrs = 1;
     }
-    auto go = [&](auto full, auto any, int logits) { return cudaLaunchKernelEx(&cfg, p.vec && p.E == logits ? full : any, p); };
-    if (p.E <= 32) return go(balance_kernel<TYPE, 8, 1, SIGMOID, true>, balance_kernel<TYPE, 8, 1, SIGMOID, false>, 32);
-    if (p.E <= 64) return go(balance_kernel<TYPE, 16, 1, SIGMOID, true>, balance_kernel<TYPE, 16, 1, SIGMOID, false>, 64);
-    if (p.E <= 128) return go(balance_kernel<TYPE, 32, 1, SIGMOID, true>, balance_kernel<TYPE, 32, 1, SIGMOID, false>, 128);
-    return go(balance_kernel<TYPE, 32, 2, SIGMOID, true>, balance_kernel<TYPE, 32, 2, SIGMOID, false>, 256);
+    auto go = [&](auto lanes, auto groups) {
+        constexpr int LANES = decltype(lanes)::value, G = decltype(groups)::value;
+        const bool full = p.vec && p.E == 4 * LANES * G, many = p.loss && p.rows > kB_LongTurns * turn_rows<LANES, G>();
+        auto kernel = many ? full ? balance_kernel<TYPE, LANES, G, SIGMOID, true, true> : balance_kernel<TYPE, LANES, G, SIGMOID, false, true>
+                           : full ? balance_kernel<TYPE, LANES, G, SIGMOID, true, false> : balance_kernel<TYPE, LANES, G, SIGMOID, false, false>;
+        return cudaLaunchKernelEx(&cfg, kernel, p);
+    };
+    using std::integral_constant;
+    if (p.E <= 32) return go(integral_constant<int, 8>(), integral_constant<int, 1>());
+    if (p.E <= 64) return go(integral_constant<int, 16>(), integral_constant<int, 1>());
+    if (p.E <= 128) return go(integral_constant<int, 32>(), integral_constant<int, 1>());
+    return go(integral_constant<int, 32>(), integral_constant<int, 2>());
 }
 template <int TYPE> cudaError_t launch_balance_mode(const BalanceParams& p, cudaStream_t stream) {
     return p.mode == CHIMERE_ROUTE_SIGMOID_NORM_SCALE ? launch_balance_type<TYPE, true>(p, stream) : launch_balance_type<TYPE, false>(p, stream);

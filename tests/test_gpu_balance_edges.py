@@ -3,9 +3,11 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from chimere_b200 import balance
+from chimere_b200 import abi, balance
+from test_gpu_balance import check, reference
 
 pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
 
 
 def inputs(S, L, E, k, seed=0):
@@ -43,3 +45,38 @@ def test_sizes_beyond_32_bits_are_refused():
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("mode", [abi.ROUTE_SOFTMAX_RENORM, abi.ROUTE_SIGMOID_NORM_SCALE])
+@pytest.mark.parametrize("S,L,E", [(56, 400000, 3), (60, 40000, 130), (1, 1 << 23, 200), (1, 1 << 23, 64)])
+def test_mean_probabilities_of_long_pieces(S, L, E, mode):
+    """Equal rows, whose probabilities are no powers of two: sums in fp32 would drift, all in one direction.  Of a probability: the difference of the logits and the weighted
+    one, 1 u each, and 32 u (as in the bounds of the other tests); in sigmoid mode 2 |z| + 4 <= 6.7 u more for log sigmoid, for the value and for the row's sum.  Up to 64 values, and the lanes of
+    a warp that have the same expert, are added up in fp32: 63 + 2 u; the piece's sum and the mean are rounded once each."""
+    row = torch.zeros(E, dtype=torch.float64, device="cuda")
+    row[0] = 1.0
+    logits = torch.zeros(S, L, E, dtype=torch.bfloat16, device="cuda")
+    logits[..., 0] = 1.0
+    ids = torch.zeros(S, L, 1, dtype=torch.int32, device="cuda")
+    r = balance.balance_loss(logits, ids, route_mode=mode)
+    p = torch.softmax(row if mode == abi.ROUTE_SOFTMAX_RENORM else torch.nn.functional.logsigmoid(row), 0)
+    bound = (2 + 32 + (14 if mode == abi.ROUTE_SIGMOID_NORM_SCALE else 0) + 65 + 2) * U
+    off = ((r.prob.double() - p) / p).abs().max().item()
+    assert off <= bound, (off / U, bound / U)
+    assert ((r.loss.double() - E * p[0]).abs() <= E * p[0] * (bound + 2 * U)).all() and (r.tokens == L).all() and (r.counts[:, 0] == L).all()
+
+
+@pytest.mark.parametrize("mode", [abi.ROUTE_SOFTMAX_RENORM, abi.ROUTE_SIGMOID_NORM_SCALE])
+@pytest.mark.parametrize("S,L,E,k,dtype", [(60, 9001, 256, 2, torch.float32), (1, 700001, 130, 1, torch.bfloat16), (57, 70003, 31, 3, torch.float16), (60, 30001, 64, 2, torch.bfloat16)])
+def test_long_pieces_against_64_bits(S, L, E, k, dtype, mode):
+    logits, ids = inputs(S, L, E, k, seed=L)
+    logits = logits.to(dtype)
+    mask = torch.rand(S, L, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < 0.6
+    mask[0, L // 3:] = False
+    r, d = balance.balance_loss_grad(logits, ids, mask=mask, route_mode=mode)
+    alone = balance.balance_loss(logits, ids, mask=mask, route_mode=mode)
+    assert all(torch.equal(a, b) for a, b in zip(alone, r))
+    assert torch.equal(d, balance.balance_loss_backward(logits, r.counts, r.tokens, k, mask=mask, route_mode=mode))
+    for s in range(0, S, 20):       # (64-bit copies of a few sequences at a time)
+        part = slice(s, min(s + 20, S))
+        check(balance.BalanceLoss(*(t[part] for t in r)), d[part], reference(logits[part], ids[part], mask[part], mode))
