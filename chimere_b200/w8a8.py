@@ -89,11 +89,13 @@ def _output(out: Optional[torch.Tensor], rows: int, cols: int, dtype: Optional[t
 
 
 def padded_i8(q: torch.Tensor) -> torch.Tensor:
-    """The same int8 matrix (or stack of matrices) with rows that start on 16-byte boundaries: a copy where they do not already."""
+    """The same int8 matrix (or stack of matrices) with rows that start on 16-byte boundaries: itself if it is contiguous and they do, else a copy."""
     _need(q.dtype == torch.int8 and q.dim() >= 2, "padded_i8: an int8 matrix or a stack of them")
     K = q.shape[-1]
     if K % 16 == 0:
-        return q.contiguous()
+        q = q.contiguous()
+        if q.data_ptr() % 16 == 0:
+            return q
     out = torch.zeros(*q.shape[:-1], (K + 15) // 16 * 16, dtype=torch.int8, device=q.device)[..., :K]
     out.copy_(q)
     return out
