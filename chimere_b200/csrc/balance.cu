@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
     int row0 = row_first;
 #pragma unroll 1
     do {
-    const int turns_end = LONG ? min(r1, row0 + kB_Turns * kStep) : r1;
+    const int turns_end = LONG && r1 - row0 > kB_Turns * kStep ? row0 + kB_Turns * kStep : r1;   // (no sum beyond r1: it may pass 31 bits)
 #pragma unroll 1
     for (; row0 < turns_end; row0 += kStep) {
         uint64_t v[kU][G][2];   // two values each

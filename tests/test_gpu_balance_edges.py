@@ -80,3 +80,16 @@ def test_long_pieces_against_64_bits(S, L, E, k, dtype, mode):
     for s in range(0, S, 20):       # (64-bit copies of a few sequences at a time)
         part = slice(s, min(s + 20, S))
         check(balance.BalanceLoss(*(t[part] for t in r)), d[part], reference(logits[part], ids[part], mask[part], mode))
+
+
+def test_the_longest_sequence():
+    """Row numbers up to the last that 32 bits hold: one expert, whose probability is 1, and a mask that leaves the last rows and some in front."""
+    L = 0x7FFFFF00
+    logits, ids = torch.zeros(L, 1, dtype=torch.bfloat16, device="cuda"), torch.zeros(L, 1, dtype=torch.int32, device="cuda")
+    r, d = balance.balance_loss_grad(logits, ids)
+    assert r.tokens.item() == L and r.counts.item() == L and r.prob.item() == 1 and r.loss.item() == 1 and not d.any()
+    mask = torch.zeros(L, dtype=torch.bool, device="cuda")
+    mask[-1000:], mask[5], mask[L // 2] = True, True, True
+    ids[-3:] = -1
+    r = balance.balance_loss(logits, ids, mask=mask, route_mode=abi.ROUTE_SIGMOID_NORM_SCALE)
+    assert r.tokens.item() == 1002 and r.counts.item() == 999 and r.prob.item() == 1 and abs(r.loss.item() - 999 / 1002) <= 2 * U
