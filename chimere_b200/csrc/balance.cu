@@ -7,8 +7,8 @@
 // The counts need the ids alone, which are a few percent of the bytes; with them known one pass over the logits gives both the sums
 // and the gradient, so every logit is read once and every gradient written once.  Bound: memory in large batches (16 sequences
 // of 8192 x 256 f32 with gradient: 48 us behind 6.5 of counting, 5.6 TB/s), launches and latency in small ones (24 tokens: 4.1 us; 4 x 1000 x 128: 13).
-//   balance_kernel a piece of a sequence per CTA, a row by 8, 16 or 32 lanes; sums of a piece in fp32, of the pieces in fp64 and always in the same
-//                  order.  Short sequences, and many of them: the pieces of a sequence are a cluster of up to eight CTAs, which count its pairs and add up its sums over
+//   balance_kernel a piece of a sequence per CTA, a row by 8, 16 or 32 lanes; sums of a lane in fp32 (of up to 256 values, then in fp64), of the warps and pieces in
+//                  fp64 and always in the same order.  Short sequences, and many of them: the pieces of a sequence are a cluster of up to eight CTAs, which count its pairs and add up its sums over
 //                  shared memory, one launch in all.  A few long sequences: dozens of pieces each, whose sums the CTAs that finish last add up, behind
 //   count_kernel   pairs per expert of a piece of a sequence.
 // In the gradient f_e is replaced by f_e - (sum_j f_j) / E, a constant less: it drops out (the p of a row add up to 1), and the difference
@@ -566,6 +566,10 @@ cudaError_t launch_balance(const BalanceParams& p, int type, cudaStream_t stream
 
 // Pieces of a sequence.  With the counting in front: as many CTAs as run at once.  In clusters: up to eight, at least kB_PieceRows rows in each; taken
 // for short sequences, and for so many of them that eight pieces of each fill the GPU.
+// us, with gradient, in clusters / with counting in front, of 1, 4, 16 and 32 sequences: 256 f32 logits, 512 rows 9.7 / 10.0, 10.2 / 10.0, 11.8 / 12.9, 12.4 / 15.4; 1024 rows
+// 13.7 / 11.0, 14.1 / 12.0, 17.1 / 15.4, 17.6 / 20.0; 2048 rows 21.9 / 12.8, 21.8 / 14.0, 27.5 / 20.2, 29.0 / 29.5.  128 bf16 logits, sigmoid, 512 rows 8.0 / 8.7, 8.6 / 9.0,
+// 10.1 / 10.6, 10.4 / 14.0; 1024 rows 11.0 / 9.4, 11.4 / 10.2, 14.3 / 13.9, 14.8 / 17.5; 2048 rows 16.7 / 11.0, 17.4 / 12.3, 22.8 / 17.7, 23.3 / 25.0.  (Between 512 and 1024
+// rows clusters are up to 3 us slower for few sequences, up to 3 faster for many.)
 constexpr int kB_PieceRows = 32, kB_Cluster = 8, kB_ClusterRows = 1024, kB_Sms = 148;   // (the scratch's size goes by these: constants)
 struct Plan { int pieces, rows, count_pieces, count_rows; };
 Plan plan_of(int64_t S, int L, int k) {

@@ -464,8 +464,9 @@ __device__ __forceinline__ Channel channel(const MatmulParams& p, bool dual, int
     return c;
 }
 // silu(g) * u for two pairs: g / (1 + exp(-g)), exp as 2^h times 1 + r with h = -g log2(e) rounded and r what the rounding left out (ln(2) in two parts), the
-// quotient with the hardware's reciprocal.  silu is off by ten half-steps of fp32 at most: ex2 four, 1 + r and its product two, 1 + exp one, the
-// reciprocal two, the last product one.  (Through expf and the division operator the epilogue took longer than the MMAs: 32768 tokens x 512 of
+// quotient with the hardware's reciprocal.  From g = -87 on silu is off by ten half-steps of fp32 at most: ex2 four, 1 + r and its product two, 1 + exp one, the
+// reciprocal two, the last product one.  Below about -87.3 the denominator passes 2^126, its reciprocal is subnormal and comes out as 0, and so does silu: off by less than
+// 88 * 2^-126.  (Through expf and the division operator the epilogue took longer than the MMAs: 32768 tokens x 512 of
 // 2048 122 us, plain results of the same sums 59.)
 __device__ __forceinline__ void silu_mul2(float g0, float g1, float u0, float u1, float (&y)[2]) {
     float a = -g0, b = -g1;
@@ -1369,7 +1370,13 @@ int launch_matmul(const MatmulCall& c, bool pdl, cudaStream_t stream) {
     if (few_tokens(c)) return launch_rows_any(c, nullptr, 0, pdl, stream);
     if (!encoder()) return -6;
     const int sms = sm_count();
-    // Pairs of CTAs: dense batches of more than 128 tokens with sixteen tiles or more, grouped ones of 32 tokens per group or more on average.
+    // Pairs of CTAs: dense batches of more than 128 tokens with sixteen tiles or more, grouped ones of 32 tokens per group or more on average.  us, by pairs / by single CTAs:
+    //   dense    4096 x 2048 (16 tiles up to 256 tokens) 128 tokens 11.1 / 9.0, 192: 11.0 / 11.1, 384: 11.4 / 14.5; 8192 x 4096 (32) 128: 16.0 / 14.3, 192: 15.8 / 20.4;
+    //            2048 x 4096 256 tokens (8) 15.5 / 10.6, 384 (16) 15.6 / 14.1; 2048 x 2048 384 (16) 11.1 / 11.1
+    //   grouped  gate and up + down of experts of 512 x 2048.  256 groups, even: 16 tokens each 176 / 143, 32: 188 / 163, 48: 187 / 187, 64: 192 / 241; with Zipf routing (some 30
+    //            groups in use) 16: 38 / 64, 32: 56 / 92, 64: 79 / 163.  64 even groups of 16: 53 / 43, 32: 55 / 50, 64: 59 / 64.  4 groups of 32: 19.7 / 16.9, 64: 20.7 / 20.4,
+    //            128: 22.4 / 21.9; 16 of 32: 22.1 / 21.9, 128: 26.2 / 33.9.  128 even groups of 1856 x 2688, 32 each: 263 / 218, 64: 269 / 248.
+    //            The average does not see how the rows are spread: the line lies between what even and skewed routing would ask for.
     const int outs = c.dual ? 128 : 256;
     const int64_t wide = token_tiles(c, kW_Tokens) * ((c.p.N + outs - 1) / outs);
     if (c.p.offsets ? c.p.M >= 32 * (int64_t)c.p.E : c.p.M > 128 && wide >= 16) {

@@ -153,7 +153,8 @@ def matmul_w8a8_grouped(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor,
                         act: int = abi.ACT_NONE, out_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                         out_dtype: Optional[torch.dtype] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same with a matrix per group of rows: rows offsets[e] .. offsets[e + 1] of q (int32 [E + 1], ascending, as the router's dispatch leaves them) by w[e];
-    w int8 [E, N or 2 N, K], w_scale and bias f32 [E, N or 2 N].  With out_rows (int32 [M]) row i goes to row out_rows[i] of `out`.  Rows that belong to no
+    w int8 [E, N or 2 N, K], w_scale and bias f32 [E, N or 2 N].  With out_rows (int32 [M]) row i goes to row out_rows[i] of `out` (no index
+    twice, or either row's values may end up there).  Rows that belong to no
     group, and rows with an index outside `out`, are not written: `out` keeps what it held there (without `out` those rows are not initialised)."""
     _need(q.is_cuda and q.dim() == 2 and w.dim() == 3 and q.shape[1] == w.shape[2], "q [M, K] and w [E, N, K] on a CUDA device")
     index, (M, K), (E, R) = q.get_device(), q.shape, w.shape[:2]

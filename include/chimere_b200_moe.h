@@ -366,8 +366,8 @@ int chimere_b200_moe_ep_pack_sorted(const chimere_moe_layer* w, int T, chimere_m
 /* ------------------------------------------------------------ W8A8 ---------------------- */
 /* Matrices of 8-bit integers with one f32 scale per output channel, times rows of 8-bit integers with one f32 scale per token: the
  * form int8 checkpoints have for the projections around the MoE layer and for experts.  No counterpart in the reference, whose weights
- * are ggml blocks.  Rows of int8 start on 16-byte boundaries (base and row stride multiples of 16 bytes; the bytes behind a row's K values
- * are not looked at); K <= 131071, so that every sum is exact in 32 bits.  *_type: CHIMERE_TYPE_F32, _F16 or _BF16.  M = 0 is no work;
+ * are ggml blocks.  Rows of int8 start on 16-byte boundaries (base and row stride multiples of 16 bytes; bytes behind a row's K
+ * values, up to the next boundary, may be read and count for nothing); K <= 131071, so that every sum is exact in 32 bits.  *_type: CHIMERE_TYPE_F32, _F16 or _BF16.  M = 0 is no work;
  * a product takes up to 0x7FFFFF00 rows.
  * Outputs and scratch share no memory with anything else a call reads or writes, except where its comment allows it.
  * d_status (may be NULL): raised if a bounded wait ran out; the outputs concerned are NaN then.
@@ -380,14 +380,15 @@ int chimere_b200_quantize_i8(const void* d_x, int x_type, int64_t ldx, int64_t x
                              int64_t M, int K, int8_t* d_q, int64_t ldq, float* d_scale, cudaStream_t stream);
 
 /* y[m][n] = act((sum_k x[m][k] * w[n][k]) * x_scale[m] * w_scale[n] + bias[n]), m < M, n < N.  CHIMERE_ACT_NONE; CHIMERE_ACT_RELU2; CHIMERE_ACT_SWIGLU: w,
- * w_scale and bias have 2 N rows, N of the gate and then N of the up matrix, and y = silu(gate) * up.  d_bias may be NULL.  ldx, ldw in
+ * w_scale and bias have 2 N rows, N of the gate and then N of the up matrix, and y = silu(gate) * up.  The exact sum is rounded to f32, multiplied by w_scale[n] and then
+ * by x_scale[m], a rounding each (with a bias the last product and its addition are one), in every batch size alike.  d_bias may be NULL.  ldx, ldw in
  * bytes, ldy in elements. */
 int chimere_b200_matmul_w8a8(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, const float* d_w_scale,
                              const float* d_bias, int64_t M, int N, int K, int act, void* d_y, int y_type, int64_t ldy,
                              int32_t* d_status, cudaStream_t stream);
 /* The same with a matrix per group of rows: rows d_offsets[e] .. d_offsets[e + 1] (device int32 [E + 1], as chimere_b200_moe_route leaves them in
  * ws->offsets: ascending, and cut to [0, M]; E <= 1024) by matrix e, which starts e * stride_w bytes behind the first; w_scale and bias [E][N or 2 N].  With d_out_rows row i goes to row
- * d_out_rows[i] of y.  Rows in no group, and rows whose index is not in [0, y_rows), are not written. */
+ * d_out_rows[i] of y; an index that stands twice leaves either row's values there, value by value.  Rows in no group, and rows whose index is not in [0, y_rows), are not written. */
 int chimere_b200_matmul_w8a8_grouped(const int8_t* d_x, int64_t ldx, const float* d_x_scale, const int8_t* d_w, int64_t ldw, int64_t stride_w,
                                      const float* d_w_scale, const float* d_bias, const int32_t* d_offsets, int E, int64_t M, int N, int K,
                                      int act, void* d_y, int y_type, int64_t ldy, int64_t y_rows, const int32_t* d_out_rows,

@@ -86,3 +86,91 @@ def test_sizes_beyond_32_bits_are_refused():
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"call {i} was taken")
+
+
+# ---- weights and rows that the launches in front make ----
+def weights_of(wf):
+    return w8a8.quantize_i8(wf)
+
+
+@pytest.mark.parametrize("M,K,N", [(7, 2688, 1000), (9, 512, 512), (61, 4096, 2048), (300, 1000, 2000), (2000, 512, 4096)])
+def test_weights_made_by_the_launch_in_front(M, K, N):
+    """Products in a launch of their own fetch weights and scales before the rows are there: what made the weights must be complete by then all the same."""
+    g = gen(M + K)
+    x = torch.randn(M, K, generator=g, device="cuda")
+    q, s = w8a8.quantize_i8(x)
+    for _ in range(10):
+        wf = torch.randn(N, K, generator=g, device="cuda")
+        y = w8a8.linear_w8a8(x, *weights_of(wf))
+        wq, ws = weights_of(wf)
+        torch.cuda.synchronize()
+        assert torch.equal(y, w8a8.matmul_w8a8(q, s, wq, ws))
+
+
+@pytest.mark.parametrize("T,E,k,H,F", [(1, 8, 2, 512, 256), (16, 32, 4, 512, 256), (200, 8, 2, 512, 320), (3000, 6, 3, 1024, 512)])
+def test_experts_whose_weights_and_rows_the_launches_in_front_make(T, E, k, H, F):
+    g = gen(T)
+    ids = torch.randint(0, E, (T * k,), generator=g, device="cuda")
+    perm = torch.sort(ids, stable=True).indices.to(torch.int32)
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    off[1:] = torch.bincount(ids, minlength=E).cumsum(0)
+
+    def stack(rows, K):
+        q, s = w8a8.quantize_i8(torch.randn(E * rows, K, generator=g, device="cuda"))
+        return q.view(E, rows, K), s.view(E, rows) * 0.05
+
+    for _ in range(10):
+        wu, su = stack(2 * F, H)
+        wd, sd = stack(H, F)
+        x = torch.randn(T, H, generator=g, device="cuda")
+        y = w8a8.experts_w8a8(x, perm, off, k, wu, su, wd, sd)
+        torch.cuda.synchronize()
+        q, s = w8a8.quantize_i8(x, perm, k)
+        torch.cuda.synchronize()
+        h = w8a8.matmul_w8a8_grouped(q, s, wu, su, off, act=abi.ACT_SWIGLU)
+        torch.cuda.synchronize()
+        hq, hs = w8a8.quantize_i8(h)
+        torch.cuda.synchronize()
+        assert torch.equal(y, w8a8.matmul_w8a8_grouped(hq, hs, wd, sd, off, out_rows=perm, out=torch.empty_like(y)))
+
+
+# ---- the order of the roundings ----
+@pytest.mark.parametrize("M,K,N", [(1, 2048, 512), (4, 4100, 515), (8, 512, 96), (17, 100, 130), (61, 4096, 2048), (300, 640, 1000), (2300, 1000, 1024)])
+@pytest.mark.parametrize("act", [abi.ACT_NONE, abi.ACT_RELU2])
+def test_products_round_in_the_stated_order(M, K, N, act):
+    """The sum to f32, times the channel's scale, times the row's: one rounding each, the same bits in every kernel."""
+    g = gen(M + K + N)
+    q, w, sx, sw = i8(g, M, K), i8(g, N, K), scales(g, M), scales(g, N)
+    want = (q.double() @ w.double().T).float() * sw * sx[:, None]
+    if act == abi.ACT_RELU2:
+        want = want.clamp_min(0).square()
+    for dtype in TYPES:
+        assert torch.equal(w8a8.matmul_w8a8(q, sx, w, sw, act=act, out_dtype=dtype), want.to(dtype))
+    off = torch.tensor([0, M // 3, M // 3, M], dtype=torch.int32, device="cuda")
+    stack, scale = w8a8.padded_i8(torch.stack([w] * 3)), torch.stack([sw] * 3).contiguous()
+    assert torch.equal(w8a8.matmul_w8a8_grouped(q, sx, stack, scale, off, act=act), want)
+
+
+def test_relu2_experts_are_the_formula_bit_for_bit():
+    """Activations next to a half step go to one whole number or its neighbour by their last bit, so the order of the two scales decides there: channel first."""
+    T, E, k, H, F = 100, 8, 3, 1344, 480
+    g = gen(17)
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    wu, su, wd, sd = i8(g, E, F, H), scales(g, E, F), i8(g, E, H, F), scales(g, E, H)
+    ids = torch.randint(0, E, (T * k,), generator=g, device="cuda")
+    perm = torch.sort(ids, stable=True).indices
+    counts = torch.bincount(ids, minlength=E).tolist()
+    off = torch.tensor([sum(counts[:e]) for e in range(E + 1)], dtype=torch.int32, device="cuda")
+    y = w8a8.experts_w8a8(x, perm.to(torch.int32), off, k, wu, su, wd, sd, act=abi.ACT_RELU2)
+
+    def rows(v):
+        v = v.double()
+        s = (v.abs().amax(1, keepdim=True) / 127).float().double()
+        return (v / s).float().double().round(), s.float()
+
+    for e in range(E):
+        pairs = perm[off[e]:off[e + 1]]
+        q, s = rows(x[pairs // k].float())
+        h = ((q @ wu[e].double().T).float() * su[e] * s).clamp_min(0).square()
+        q, s = rows(h)
+        assert torch.equal(y[pairs], ((q @ wd[e].double().T).float() * sd[e] * s).to(torch.bfloat16))
