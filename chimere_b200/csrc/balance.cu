@@ -333,11 +333,11 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
     }
     __syncthreads();
     if (grad) {
-        int all = 0;
-        for (int e = lane; e < p.E; e += 32) all += sh.hist[e];
-        all = __reduce_add_sync(0xffffffffu, all);
+        int low = 0, high = 0;   // (the counts of several ranks may add up to more than 31 bits)
+        for (int e = lane; e < p.E; e += 32) { low += sh.hist[e] & 0xFFFF; high += sh.hist[e] >> 16; }
+        const double all = (double)__reduce_add_sync(0xffffffffu, high) * 65536.0 + __reduce_add_sync(0xffffffffu, low);
         const double n = sh.hist[p.E], c = n > 0 ? (double)p.coef * p.E / (p.k * n * n) * (p.d_loss ? (double)p.d_loss[s] : 1.0) : 0.0;
-        for (int e = tid; e < p.E; e += kB_Threads) sh.g[e] = (float)(c * (sh.hist[e] - (double)all / p.E));
+        for (int e = tid; e < p.E; e += kB_Threads) sh.g[e] = (float)(c * (sh.hist[e] - all / p.E));
         __syncthreads();
     }
     uint64_t g[G][2], acc[G][2];

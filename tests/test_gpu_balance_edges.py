@@ -93,3 +93,25 @@ def test_the_longest_sequence():
     ids[-3:] = -1
     r = balance.balance_loss(logits, ids, mask=mask, route_mode=abi.ROUTE_SIGMOID_NORM_SCALE)
     assert r.tokens.item() == 1002 and r.counts.item() == 999 and r.prob.item() == 1 and abs(r.loss.item() - 999 / 1002) <= 2 * U
+
+
+@pytest.mark.parametrize("E", [8, 200])
+def test_counts_of_many_ranks(E):
+    """Counts that add up to more than 31 bits, near an even load: the gradient hangs on their differences."""
+    k, n = 2, 2 * 10 ** 9
+    g = torch.Generator(device="cuda").manual_seed(E)
+    logits = torch.randn(50, E, generator=g, device="cuda")
+    counts = (k * n // E + torch.randint(-1000, 1001, (E,), generator=g, device="cuda")).to(torch.int32)
+    tokens = torch.tensor(n, dtype=torch.int32, device="cuda")
+    d = balance.balance_loss_backward(logits, counts, tokens, k, grad_loss=torch.tensor(1e15, device="cuda"))
+    l = logits.double()
+    p = torch.softmax(l, 1)
+    off = l.amax(1, keepdim=True) - l
+    ep = p * (off + (p * off).sum(1, keepdim=True) + 32) * U             # (as in the bounds of the other tests)
+    f = counts.double()
+    slope = 1e15 * E / (k * float(n) ** 2) * (f - f.mean())
+    dot = (p * slope).sum(1, keepdim=True)
+    e_dot = (ep * slope.abs() + p * slope.abs() * 24 * U).sum(1, keepdim=True)
+    want = p * (slope - dot)
+    bound = ep * (slope - dot).abs() + (p + ep) * (2 * U * slope.abs() + e_dot + U * (slope - dot).abs()) + 5 * U * want.abs()
+    assert ((d.double() - want).abs() <= bound * 1.01).all(), ((d.double() - want).abs() / bound).max()
