@@ -12,7 +12,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from . import abi
 from .w8a8 import _TYPES, _call, _ints
@@ -33,7 +33,7 @@ def _check(logits, topk_idx, mask, route_mode, coef) -> _Args:
     shape, index = logits.shape, logits.get_device()
     if index < 0 or len(shape) not in (2, 3) or logits.dtype not in _TYPES:
         raise ValueError("logits: [T, E] or [S, L, E] of float32, float16 or bfloat16 on a CUDA device")
-    if unpack_dual(logits).tangent is not None:
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(logits).tangent is not None:     # (below 0: no dual tensors at all)
         raise NotImplementedError("logits: a dual tensor (there is no forward mode, its tangent would be lost)")
     if logits.stride(-1) != 1 and shape[-1] != 1:
         raise ValueError("logits: the values of a row lie side by side")
@@ -42,7 +42,7 @@ def _check(logits, topk_idx, mask, route_mode, coef) -> _Args:
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.get_device() != index or mask.shape != shape[:-1] or not mask.is_contiguous()):
         raise ValueError("mask: contiguous bool or uint8, one value per row of logits")
     S, L, E = shape if len(shape) == 3 else (1, *shape)
-    _ints(E, topk_idx.shape[-1], route_mode)
+    _ints(E | topk_idx.shape[-1] | route_mode)
     return S, L, E, topk_idx.shape[-1], route_mode, float(coef)
 
 

@@ -37,10 +37,10 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _ints(*sizes: int) -> None:
-    """Sizes the C ABI takes as 32-bit integers (ctypes would cut them)."""
-    if max(sizes) > 0x7FFFFFFF or min(sizes) < -0x80000000:
-        raise ValueError(f"sizes and options are 32-bit integers: {sizes}")
+def _ints(all_bits: int) -> None:
+    """Of sizes and options that the C ABI takes as 32-bit integers, or-ed together: ctypes would cut what is wider."""
+    if all_bits >> 31:
+        raise ValueError("sizes and options: whole numbers from 0 to 2^31 - 1")
 
 
 def _vector(t: Optional[torch.Tensor], name: str, shape: tuple, dtype: torch.dtype, index: int) -> Optional[int]:
@@ -106,7 +106,7 @@ def quantize_i8(x: torch.Tensor, rows: Optional[torch.Tensor] = None, rows_div: 
     the device.  With `rows` (int32 [M]) row i is row rows[i] // rows_div of x -- a dispatch permutation and top_k, say; an index outside x gives
     a row of zeros with scale 0.  A row with an infinity or a NaN has scale NaN.  q is a view of rows padded to 16 bytes."""
     n, K, xp, kind, ldx = _floats(x, "x")
-    _ints(K, rows_div)
+    _ints(K | rows_div)
     index = x.get_device()
     M = n if rows is None else rows.numel()
     rp = _vector(rows, "rows", (M,), torch.int32, index)
@@ -123,7 +123,7 @@ def matmul_w8a8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
     for ACT_SWIGLU; w_scale and bias f32, one per row of w.  The integer sums are exact.  out_dtype: float32 unless given."""
     _need(q.is_cuda and q.dim() == 2 and w.dim() == 2 and q.shape[1] == w.shape[1], "q [M, K] and w [N, K] on a CUDA device")
     index, (M, K), R = q.get_device(), q.shape, w.shape[0]
-    _ints(K, R, act)
+    _ints(K | R | act + 1)
     N = _outputs(R, act)
     out, yp, kind, ldy = _output(out, M, N, out_dtype or (None if out is not None else torch.float32), q)
     xp, ldx = _weight(q, "q", index)
@@ -158,7 +158,7 @@ def matmul_w8a8_grouped(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor,
     group, and rows with an index outside `out`, are not written: `out` keeps what it held there (without `out` those rows are not initialised)."""
     _need(q.is_cuda and q.dim() == 2 and w.dim() == 3 and q.shape[1] == w.shape[2], "q [M, K] and w [E, N, K] on a CUDA device")
     index, (M, K), (E, R) = q.get_device(), q.shape, w.shape[:2]
-    _ints(K, R, E, act)
+    _ints(K | R | E | act + 1)
     N = _outputs(R, act)
     y_rows = M if out is None or out_rows is None else out.shape[0]
     out, yp, kind, ldy = _output(out, y_rows, N, out_dtype or (None if out is not None else torch.float32), q)
@@ -177,7 +177,7 @@ def linear_w8a8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
     M, K, xp, x_kind, ldx = _floats(x, "x")
     _need(w.dim() == 2 and w.shape[1] == K, "x [M, K] and w [N, K]")
     index, R = x.get_device(), w.shape[0]
-    _ints(K, R, act)
+    _ints(K | R | act + 1)
     N = _outputs(R, act)
     given = out
     out, yp, kind, ldy = _output(out, M, N, out_dtype or (None if out is not None else x.dtype), x)
@@ -235,7 +235,7 @@ def experts_w8a8(x: torch.Tensor, perm: torch.Tensor, offsets: torch.Tensor, top
     index, (E, R, K), F = x.get_device(), w_up.shape, w_down.shape[2]
     _need(K == H and R == (2 * F if act == abi.ACT_SWIGLU else F) and w_down.shape[0] == E and w_down.shape[1] == H, "w_up [E, F or 2 F, H], w_down [E, H, F]")
     _need(top_k >= 1, "top_k: at least 1")
-    _ints(E, R, H, F, top_k)
+    _ints(E | R | H | F | top_k)
     P = T * top_k
     out, yp, kind, ldy = _output(out, P, H, out_dtype or (None if out is not None else x.dtype), x)
     up, ld_up, plane_up = _stack(w_up, "w_up", index)
