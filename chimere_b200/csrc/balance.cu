@@ -272,8 +272,9 @@ __device__ __forceinline__ void finish_sequence(const BalanceParams& p, Shared& 
 // A row by LANES lanes, G groups of four values each: lane i owns values 4 (i + LANES g) .. + 3.
 // FULL: as many logits as the lanes hold, rows that are read and written four values at a time: no lane looks at what it has.
 // LONG: pieces of more than kB_LongTurns turns of a warp.  A lane adds up a probability per row of its own, off by their number in half-steps of fp32 at most (mean
-// probabilities of 2^23 equal rows were 437 off), so there the sums of kB_Turns turns are added up in fp64.  A kernel of its own: in the other one the second loop costs up to a
-// quarter in spilled registers (8 x 8192 x 255 bf16 sigmoid 37.5 us, 48.6 with it) and 0.4 us of 4 in small calls.
+// probabilities of 2^23 equal rows were 437 off), so there the sums of kB_Turns turns are added up in fp64.  us, without / with them: 60 x 9001 x 256 bf16, gradient 195 / 190, f32 269 / 275;
+// 57 x 70003 x 31 f32 318 / 359, bf16 549 / 545.  A kernel of its own: in the other one these sums cost 0.4 us of 4 in small calls and up to a quarter in spilled registers (8 x
+// 8192 x 255 bf16 sigmoid 37.5, 48.6 with a loop around the turns).
 template <int G> __host__ __device__ constexpr int rows_at_a_time() { return G == 2 ? 2 : 4; }
 template <int LANES, int G> __host__ __device__ constexpr int turn_rows() { return kB_Warps * (32 / LANES) * rows_at_a_time<G>(); }
 template <int TYPE, int LANES, int G, bool SIGMOID, bool FULL, bool LONG>
@@ -354,12 +355,35 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
         for (int e = lane; e < p.E; e += 32) sh.part[warp][e] = 0;
         __syncwarp();
     }
-    int row0 = row_first;
+    auto fold = [&]() {   // the sums of these turns over the rows of a warp
+        int t = tid;
+        if (LONG) asm volatile("mov.u32 %0, %%tid.x;" : "=r"(t));   // (asked for again, so that no place of these sums is kept in registers through the turns)
+        const int w = t >> 5, mine = (t & 31) / LANES, first = 4 * ((t & 31) % LANES);
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float a, b;
+                unpack2(acc[j][i / 2], a, b);
+                float v = i & 1 ? b : a;
+#pragma unroll
+                for (int d = LANES; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+                const int e = first + 4 * LANES * j + i;
+                if (mine == 0 && e < p.E) {
+                    if (LONG) sh.part[w][e] += v;
+                    else sh.part[w][e] = v;
+                }
+            }
+    };
+    int turns = 0;
 #pragma unroll 1
-    do {
-    const int turns_end = LONG && r1 - row0 > kB_Turns * kStep ? row0 + kB_Turns * kStep : r1;   // (no sum beyond r1: it may pass 31 bits)
-#pragma unroll 1
-    for (; row0 < turns_end; row0 += kStep) {
+    for (int row0 = row_first; row0 < r1; row0 += kStep) {
+        if (LONG && turns++ == kB_Turns) {
+            fold();
+#pragma unroll
+            for (int j = 0; j < G; ++j) acc[j][0] = acc[j][1] = 0;
+            turns = 1;
+        }
         uint64_t v[kU][G][2];   // two values each
         // step by step for all of the warp's rows, so that one row's exchanges between lanes pass behind the others'
         float mx[kU], sum[kU], dot[kU];
@@ -446,32 +470,11 @@ __global__ void __launch_bounds__(kB_Threads, kB_CtasPerSm) balance_kernel(Balan
             }
         }
     }
-    if (!LONG) {
-        griddep_launch();
-        if (!stats) return;
-    }
-    // the sums of these turns over the rows of a warp
-#pragma unroll
-    for (int j = 0; j < G; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float a, b;
-            unpack2(acc[j][i / 2], a, b);
-            float v = i & 1 ? b : a;
-#pragma unroll
-            for (int d = LANES; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-            const int e = i4 + 4 * LANES * j + i;
-            if (sub == 0 && e < p.E) {
-                if (LONG) sh.part[warp][e] += v;
-                else sh.part[warp][e] = v;
-            }
-        }
-    if (LONG) {
-#pragma unroll
-        for (int j = 0; j < G; ++j) acc[j][0] = acc[j][1] = 0;
-    }
-    } while (LONG && row0 < r1);
-    if (LONG) griddep_launch();
+    griddep_launch();
+    if (!stats) return;
+    fold();
+
+    // the piece's sums
     __syncthreads();
     auto of_piece = [&](int e) {
         double v = 0.0;
