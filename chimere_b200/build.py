@@ -12,6 +12,8 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -33,12 +35,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB
     nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", LIB] + [os.path.join(CSRC, s) for s in SOURCES]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
-    if verbose:
-        print(r.stderr)
+
+    def run(args: list) -> None:
+        r = subprocess.run([nvcc, *args], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
+        if verbose:
+            print(r.stderr)
+
+    with tempfile.TemporaryDirectory() as objects:      # the sources side by side, the longest take a minute or two each
+        compile_flags = [f for f in NVCC_FLAGS if f != "-shared"] + (["-Xptxas", "-v"] if verbose else [])
+        paths = [os.path.join(objects, s + ".o") for s in SOURCES]
+        with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+            list(pool.map(lambda s, o: run([*compile_flags, "-c", "-o", o, os.path.join(CSRC, s)]), SOURCES, paths))
+        run([*NVCC_FLAGS, "-o", LIB, *paths])
     return LIB
 
 
