@@ -67,6 +67,23 @@ def test_mean_probabilities_of_long_pieces(S, L, E, mode):
 
 
 @pytest.mark.parametrize("mode", [abi.ROUTE_SOFTMAX_RENORM, abi.ROUTE_SIGMOID_NORM_SCALE])
+@pytest.mark.parametrize("S,L,E", [(1, 40000, 256), (1, 100000, 8), (3, 1025, 130), (1, 1024, 33), (5, 5000, 60), (60, 700, 40), (1, 2049, 200), (2, 8191, 97), (55, 1500, 128), (1, 33, 5)])
+def test_every_row_counts_once(S, L, E, mode):
+    """Equal rows again, in pieces of up to 64 rows per lane: a row lost or taken twice at an edge of a piece moves the mean probability by 1 / L, at least 10^-5, which the bound above
+    (115 u, 7 10^-6) does not hide.  The last row differs, so that it is seen whose place it takes."""
+    logits = torch.zeros(S, L, E, device="cuda")
+    logits[..., 0] = 1.0
+    logits[:, -1, :] = logits[:, -1, :].flip(-1)
+    ids = torch.zeros(S, L, 1, dtype=torch.int32, device="cuda")
+    r = balance.balance_loss(logits, ids, route_mode=mode)
+    z = logits.double() if mode == abi.ROUTE_SOFTMAX_RENORM else torch.nn.functional.logsigmoid(logits.double())
+    p = torch.softmax(z, 2).mean(1)
+    off = ((r.prob.double() - p) / p).abs().max().item()
+    assert off <= 115 * U, off / U
+    assert (r.tokens == L).all() and (r.counts[:, 0] == L).all()
+
+
+@pytest.mark.parametrize("mode", [abi.ROUTE_SOFTMAX_RENORM, abi.ROUTE_SIGMOID_NORM_SCALE])
 @pytest.mark.parametrize("S,L,E,k,dtype", [(60, 9001, 256, 2, torch.float32), (1, 700001, 130, 1, torch.bfloat16), (57, 70003, 31, 3, torch.float16), (60, 30001, 64, 2, torch.bfloat16)])
 def test_long_pieces_against_64_bits(S, L, E, k, dtype, mode):
     logits, ids = inputs(S, L, E, k, seed=L)
